@@ -249,6 +249,97 @@ typedef struct sdxlq_layer_norm_desc {
 } sdxlq_layer_norm_desc;
 int sdxlq_layer_norm(sdxlq_context* ctx, const sdxlq_layer_norm_desc* desc);
 
+/* ---- keys and values of attention ---------------------------------------------------------- */
+
+/* Keys and values of `slots` sequences of up to `capacity` tokens: a cache in one of the library's types, or FP16 tensors as
+ * the to_k / to_v projections write them. Element d of head h of token t of slot s is at
+ * s * slot_stride + t * token_stride + h * head_stride + d, in k and in v alike (strides in elements).
+ * 8-bit types hold a scale for each vector of a head: value = element * scales[s, h, t].
+ * head_dim is a multiple of 8 (FP16) or 16 (8-bit types) and at most 128; k, v and the strides are multiples of 16 bytes
+ * (SDXLQ_ERR_UNSUPPORTED_SHAPE otherwise). */
+typedef struct sdxlq_kv_cache {
+    void* k;
+    void* v;
+    float* k_scales;             /* FP32 [slots, heads, capacity]; NULL for FP16 */
+    float* v_scales;
+    uint64_t slots;
+    uint64_t capacity;           /* tokens per slot */
+    uint64_t heads;
+    uint64_t head_dim;
+    uint64_t slot_stride;
+    uint64_t token_stride;
+    uint64_t head_stride;
+    int32_t dtype;               /* SDXLQ_FP16, SDXLQ_INT8, SDXLQ_FP8_E4M3 or SDXLQ_FP8_E5M2 */
+    int32_t reserved;
+} sdxlq_kv_cache;
+
+/* FP16 keys and values [rows, tokens, heads, head_dim] beside a cache: row r belongs to slot first_slot + r, its tokens to
+ * the cache's tokens positions[r], positions[r] + 1, ... (`start` for every row when positions is NULL). */
+typedef struct sdxlq_kv_tokens {
+    void* k;
+    void* v;
+    uint64_t rows;
+    uint64_t tokens;
+    uint64_t row_stride;         /* elements */
+    uint64_t token_stride;
+    uint64_t head_stride;
+    const int32_t* positions;    /* device [rows] or NULL */
+    const int32_t* counts;       /* device [rows] or NULL: only the first counts[r] tokens of row r exist */
+    uint64_t first_slot;
+    uint64_t start;
+} sdxlq_kv_tokens;
+
+/* Quantises tokens into a cache. For each vector x of a head, with a = max |x| over finite values (scale 1 when a == 0):
+ *   INT8  scale = a / 127, element = rn(x / scale) of the exact quotient (ties to even); infinities saturate, NaN gives 0
+ *   FP8   scale = the smallest power of two with a / scale <= the format's largest value, element = FP8_satfinite(x / scale)
+ *   FP16  copied
+ * Tokens behind counts[r], and those whose place lies outside the slot, are not written; the rest of the cache stays as it
+ * was. `tokens->k` and `v` must not overlap the cache. */
+int sdxlq_kv_cache_write(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens);
+
+/* Reads tokens back: half_rn(element * scale), saturating. Tokens that sdxlq_kv_cache_write would not write read as zeros. */
+int sdxlq_kv_cache_read(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens);
+
+/* Attention of FP16 queries over a prefix that several batch entries share and over keys and values of each entry's own:
+ *   y[b, i, h] = sum_j softmax_j(scale * q[b, i, h] . k_j) v_j
+ * over the tokens of prefix slot b / (batch / prefix.slots), then those of own slot b. Key head h / (q_heads / heads) serves
+ * query head h. A row that sees no key gives zeros. Keys and values behind a length, or hidden by the causal mask, take no
+ * part, whatever they hold.
+ *   prefix  slots == 0: none. batch must be a multiple of prefix.slots.
+ *   own     slots == 0: none. own.slots == batch.
+ *   prefix_lengths, own_lengths   device INT32 [slots] or NULL (all of the capacity); clamped to [0, capacity]
+ *   causal  query i sees own token j when j <= length - q_tokens + i: the queries are the last q_tokens of the sequence
+ * The two parts may differ in type. Rows of several entries that share a prefix are multiplied with it together where that
+ * reads it fewer times, and long keys are split over the GPU's SMs; both leave shares of the result in `scratch`
+ * (sdxlq_shared_prefix_attention_scratch bytes; NULL: the context's workspace, which calls on other streams and captured
+ * graphs of the same context share). Results do not depend on the schedule. q, y and their strides are multiples of 16 bytes,
+ * as above; y may not overlap the inputs, except that it may be q itself. */
+typedef struct sdxlq_attention_desc {
+    const void* q;               /* FP16 [batch, q_tokens, q_heads, head_dim] */
+    void* y;                     /* FP16 [batch, q_tokens, q_heads, head_dim] */
+    uint64_t batch;
+    uint64_t q_tokens;
+    uint64_t q_heads;
+    uint64_t head_dim;
+    uint64_t q_batch_stride;     /* elements */
+    uint64_t q_token_stride;
+    uint64_t q_head_stride;
+    uint64_t y_batch_stride;
+    uint64_t y_token_stride;
+    uint64_t y_head_stride;
+    sdxlq_kv_cache prefix;
+    sdxlq_kv_cache own;
+    const int32_t* prefix_lengths;
+    const int32_t* own_lengths;
+    float scale;                 /* usually 1 / sqrt(head_dim) */
+    int32_t causal;
+    void* scratch;               /* 16-byte aligned */
+    uint64_t scratch_bytes;
+} sdxlq_attention_desc;
+int sdxlq_shared_prefix_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc);
+/* Scratch bytes of that call (host arithmetic); 0 where it needs none or is refused. */
+size_t sdxlq_shared_prefix_attention_scratch(const sdxlq_context* ctx, const sdxlq_attention_desc* desc);
+
 /* ---- harness scaffolding (not part of the projection path) --------------------------------- */
 
 /* GroupNorm, optionally followed by SiLU, over channels-last FP16 activations x[batch, rows, channels]
@@ -330,7 +421,7 @@ enum {
     SDXLQ_KERNEL_GEMM = 2,
     SDXLQ_KERNEL_SMALL = 3,
     SDXLQ_KERNEL_LAYER_NORM = 4,
-    SDXLQ_KERNEL_HARNESS = 5,         /* sdxlq_group_norm_nhwc */
+    SDXLQ_KERNEL_HARNESS = 5,         /* what is no projection: sdxlq_group_norm_nhwc, the kv cache's copies, attention */
     SDXLQ_KERNEL_CLASSES = 6
 };
 typedef struct sdxlq_kernel_times {

@@ -126,6 +126,37 @@ class _CGroupNormDesc(ctypes.Structure):
     ]
 
 
+class _CKvCache(ctypes.Structure):
+    """sdxlq_kv_cache."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+        ("slots", ctypes.c_uint64), ("capacity", ctypes.c_uint64), ("heads", ctypes.c_uint64), ("head_dim", ctypes.c_uint64),
+        ("slot_stride", ctypes.c_uint64), ("token_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64),
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class _CKvTokens(ctypes.Structure):
+    """sdxlq_kv_tokens."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("rows", ctypes.c_uint64), ("tokens", ctypes.c_uint64),
+        ("row_stride", ctypes.c_uint64), ("token_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64),
+        ("positions", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("first_slot", ctypes.c_uint64), ("start", ctypes.c_uint64),
+    ]
+
+
+class _CAttentionDesc(ctypes.Structure):
+    """sdxlq_attention_desc."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("y", ctypes.c_void_p), ("batch", ctypes.c_uint64), ("q_tokens", ctypes.c_uint64),
+        ("q_heads", ctypes.c_uint64), ("head_dim", ctypes.c_uint64), ("q_batch_stride", ctypes.c_uint64),
+        ("q_token_stride", ctypes.c_uint64), ("q_head_stride", ctypes.c_uint64), ("y_batch_stride", ctypes.c_uint64),
+        ("y_token_stride", ctypes.c_uint64), ("y_head_stride", ctypes.c_uint64), ("prefix", _CKvCache), ("own", _CKvCache),
+        ("prefix_lengths", ctypes.c_void_p), ("own_lengths", ctypes.c_void_p), ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64),
+    ]
+
+
 class _CKernelTimes(ctypes.Structure):
     _fields_ = [("milliseconds", ctypes.c_double * 6), ("launches", ctypes.c_uint64 * 6)]
 
@@ -141,6 +172,7 @@ EXPORTED_SYMBOLS = [
     "sdxlq_workspace_bytes", "sdxlq_build_info", "sdxlq_context_set_tile_n",
     "sdxlq_selftest_bounded_wait", "sdxlq_profile_enable", "sdxlq_profile_read", "sdxlq_linear_static",
     "sdxlq_context_set_pair_mode", "sdxlq_layer_norm", "sdxlq_group_norm_nhwc", "sdxlq_harness_bias_residual_add",
+    "sdxlq_kv_cache_write", "sdxlq_kv_cache_read", "sdxlq_shared_prefix_attention", "sdxlq_shared_prefix_attention_scratch",
 ]
 
 _lib: Optional[ctypes.CDLL] = None
@@ -195,6 +227,11 @@ def load_library() -> ctypes.CDLL:
     lib.sdxlq_layer_norm.argtypes = [vp, ctypes.POINTER(_CLayerNormDesc)]
     lib.sdxlq_group_norm_nhwc.argtypes = [vp, ctypes.POINTER(_CGroupNormDesc)]
     lib.sdxlq_harness_bias_residual_add.argtypes = [vp, vp, vp, vp, vp, u64, u64]
+    lib.sdxlq_kv_cache_write.argtypes = [vp, ctypes.POINTER(_CKvCache), ctypes.POINTER(_CKvTokens)]
+    lib.sdxlq_kv_cache_read.argtypes = [vp, ctypes.POINTER(_CKvCache), ctypes.POINTER(_CKvTokens)]
+    lib.sdxlq_shared_prefix_attention.argtypes = [vp, ctypes.POINTER(_CAttentionDesc)]
+    lib.sdxlq_shared_prefix_attention_scratch.argtypes = [vp, ctypes.POINTER(_CAttentionDesc)]
+    lib.sdxlq_shared_prefix_attention_scratch.restype = sz
     _lib = lib
     return lib
 
@@ -334,6 +371,71 @@ class LinearCall:
     keep: list = field(default_factory=list)
 
 
+_KV_TORCH = {ScalarType.Float8E4M3: torch.float8_e4m3fn, ScalarType.Float8E5M2: torch.float8_e5m2,
+             ScalarType.Int8: torch.int8, ScalarType.Float16: torch.float16}
+
+
+def _strides(tensor: torch.Tensor) -> tuple:
+    """Strides of [rows, tokens, heads, head_dim]; that of a dimension of one is never used."""
+    return tuple(0 if tensor.shape[i] == 1 else int(tensor.stride(i)) for i in range(3))
+
+
+@dataclass
+class KVCache:
+    """Keys and values of some sequences, as attention reads them: a cache in one of the library's types
+    (Ops.kv_cache), or FP16 tensors as the to_k / to_v projections write them (KVCache.of)."""
+
+    k: torch.Tensor                          # [slots, capacity, heads, head_dim], any strides, the head's elements together
+    v: torch.Tensor
+    type: ScalarType = ScalarType.Float16
+    k_scales: Optional[torch.Tensor] = None  # float32 [slots, heads, capacity], for each vector of a head; None for FP16
+    v_scales: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        k, v = self.k, self.v
+        if self.type not in _KV_TORCH or k.dtype != _KV_TORCH[self.type] or v.dtype != k.dtype:
+            raise CudaError("kv cache: expects FP16, INT8 or FP8 elements of the stated type")
+        if k.dim() != 4 or v.shape != k.shape or v.device != k.device:
+            raise CudaError("kv cache: keys and values must be alike, [slots, capacity, heads, head_dim]")
+        if (k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1)) or _strides(k) != _strides(v):
+            raise CudaError("kv cache: a head's elements must lie together, and keys and values have the same strides")
+        if self.type == ScalarType.Float16:
+            if self.k_scales is not None or self.v_scales is not None:
+                raise CudaError("kv cache: FP16 elements have no scales")
+        else:
+            for scales in (self.k_scales, self.v_scales):
+                if scales is None or scales.dtype != torch.float32 or not scales.is_contiguous() or scales.device != k.device or \
+                        tuple(scales.shape) != (k.shape[0], k.shape[2], k.shape[1]):
+                    raise CudaError("kv cache: an 8-bit cache needs contiguous FP32 scales [slots, heads, capacity]")
+
+    @staticmethod
+    def of(key: torch.Tensor, value: torch.Tensor, heads: int) -> "KVCache":
+        """FP16 keys and values [rows, tokens, heads * head_dim], where they are."""
+        if key.dim() != 3 or heads <= 0 or key.shape[2] % heads != 0 or value.shape != key.shape:
+            raise CudaError("kv cache: keys and values must be alike, [rows, tokens, heads * head_dim]")
+        return KVCache(key.unflatten(2, (heads, -1)), value.unflatten(2, (heads, -1)))
+
+    @property
+    def slots(self) -> int:
+        return int(self.k.shape[0])
+
+    @property
+    def capacity(self) -> int:
+        return int(self.k.shape[1])
+
+    @property
+    def heads(self) -> int:
+        return int(self.k.shape[2])
+
+    @property
+    def head_dim(self) -> int:
+        return int(self.k.shape[3])
+
+    def c_struct(self) -> _CKvCache:
+        return _CKvCache(self.k.data_ptr(), self.v.data_ptr(), _ptr(self.k_scales), _ptr(self.v_scales), *self.k.shape,
+                         *_strides(self.k), int(self.type), 0)
+
+
 class Context:
     """Owns an ``sdxlq_context``: device, stream and scratch workspace (the part of the
     reference ``Runtime`` the operator needs, include/sdxl/cuda/runtime.hpp:120-163)."""
@@ -346,8 +448,8 @@ class Context:
         self.address = 0                       # of the sdxlq_context, for the native front
         self.device = device
         self.stream = stream
-        stream_ptr = ctypes.c_void_p(stream.cuda_stream) if stream is not None else \
-            ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+        self.stream_address = stream.cuda_stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
+        stream_ptr = ctypes.c_void_p(self.stream_address)
         status = self._lib.sdxlq_context_create(device, stream_ptr, workspace_bytes, ctypes.byref(self._handle))
         if status != STATUS_OK:
             raise CudaError(f"sdxlq_context_create failed: {self._lib.sdxlq_status_string(status).decode()}", status)
@@ -373,8 +475,18 @@ class Context:
         if status != STATUS_OK:
             raise CudaError(self._lib.sdxlq_last_error(self._handle).decode(), status)
 
+    def scratch(self, size: int) -> torch.Tensor:
+        """Memory for the kernels of one call: in the pool of the stream that they run on, whichever stream is current, so that
+        its next owner comes behind them."""
+        device = torch.device("cuda", self.device)
+        if torch.cuda.current_stream(device).cuda_stream == self.stream_address:
+            return torch.empty(size, dtype=torch.uint8, device=device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(self.stream_address, device=device)):
+            return torch.empty(size, dtype=torch.uint8, device=device)
+
     def set_stream(self, stream: torch.cuda.Stream) -> None:
         self.stream = stream
+        self.stream_address = stream.cuda_stream
         self.raise_for(self._lib.sdxlq_context_set_stream(self._handle, ctypes.c_void_p(stream.cuda_stream)))
 
     def check(self) -> None:
@@ -607,6 +719,126 @@ class Ops:
             self.ctx.handle, input.data_ptr(), bias.data_ptr(), residual.data_ptr(), out.data_ptr(),
             batch * height * width, channels))
         return out
+
+    # -- keys and values of attention ----------------------------------------------------------------------
+    def _on_device(self, what: str, *tensors) -> None:
+        for tensor in tensors:
+            if tensor is not None and (tensor.device.type != "cuda" or tensor.device.index != self.ctx.device):
+                raise CudaError(f"{what}: every tensor must be on the context's device")
+
+    def _int32_vector(self, what: str, vector, count: int) -> None:
+        if vector is not None and (not torch.is_tensor(vector) or vector.dtype != torch.int32 or tuple(vector.shape) != (count,)
+                                   or not vector.is_contiguous()):
+            raise CudaError(f"{what}: expects a contiguous INT32 tensor of {count} elements")
+
+    def kv_cache(self, slots: int, capacity: int, heads: int, head_dim: int, type: ScalarType = ScalarType.Float16) -> KVCache:
+        """An empty cache for `slots` sequences of up to `capacity` tokens. The tokens of a head lie behind one another."""
+        if type not in _KV_TORCH:
+            raise CudaError("kv cache: expects FP16, INT8 or FP8 elements of the stated type")
+        device = torch.device("cuda", self.ctx.device)
+        k, v = (torch.zeros((slots, heads, capacity, head_dim), dtype=_KV_TORCH[type], device=device).transpose(1, 2) for _ in "kv")
+        scales = (None, None)
+        if type != ScalarType.Float16:
+            scales = tuple(torch.ones((slots, heads, capacity), dtype=torch.float32, device=device) for _ in "kv")
+        return KVCache(k, v, type, *scales)
+
+    def _kv_tokens(self, what: str, cache: KVCache, key: torch.Tensor, value: torch.Tensor, positions, counts, first_slot: int) -> _CKvTokens:
+        if key.dtype != torch.float16 or value.dtype != torch.float16 or key.dim() != 4 or key.shape != value.shape or \
+                tuple(key.shape[2:]) != (cache.heads, cache.head_dim):
+            raise CudaError(f"{what}: keys and values must be FP16 [rows, tokens, heads, head_dim] with the cache's heads")
+        if (key.shape[3] > 1 and (key.stride(3) != 1 or value.stride(3) != 1)) or _strides(key) != _strides(value):
+            raise CudaError(f"{what}: a head's elements must lie together, and keys and values have the same strides")
+        rows, start = int(key.shape[0]), 0
+        if positions is not None and not torch.is_tensor(positions):
+            start, positions = int(positions), None
+        self._int32_vector(f"{what}: positions", positions, rows)
+        self._int32_vector(f"{what}: counts", counts, rows)
+        if start < 0 or first_slot < 0:
+            raise CudaError(f"{what}: tokens in front of the cache")
+        self._on_device(what, cache.k, key, value, positions, counts)
+        return _CKvTokens(key.data_ptr(), value.data_ptr(), rows, int(key.shape[1]), *_strides(key), _ptr(positions), _ptr(counts),
+                          first_slot, start)
+
+    def kv_cache_write(self, cache: KVCache, key: torch.Tensor, value: torch.Tensor, positions=None,
+                       counts: Optional[torch.Tensor] = None, first_slot: int = 0) -> None:
+        """Quantises FP16 keys and values [rows, tokens, heads, head_dim] into `cache`, each vector of a head with a scale of its
+        own (INT8: max / 127; FP8: a power of two). Row r goes to slot first_slot + r, from token positions[r] on (an int: the
+        same for all rows; None: 0); with `counts`, only its first counts[r] tokens. Tokens whose place lies outside the
+        slot are not written, and what is not written stays as it was."""
+        tokens = self._kv_tokens("kv_cache_write", cache, key, value, positions, counts, first_slot)
+        if any(cache.k.stride(i) == 0 and cache.k.shape[i] > 1 for i in range(4)):
+            raise CudaError("kv_cache_write: the cache's tokens overlap in memory")
+        descriptor = cache.c_struct()
+        self.ctx.raise_for(self._lib.sdxlq_kv_cache_write(self.ctx.handle, ctypes.byref(descriptor), ctypes.byref(tokens)))
+
+    def kv_cache_read(self, cache: KVCache, tokens: int, positions=None, counts: Optional[torch.Tensor] = None,
+                      rows: Optional[int] = None, first_slot: int = 0) -> tuple:
+        """(key, value): FP16 [rows, tokens, heads, head_dim], the inverse of kv_cache_write up to its rounding. Rows default
+        to all slots from first_slot on. Tokens that kv_cache_write would not have written are zeros."""
+        rows = cache.slots - first_slot if rows is None else rows
+        if rows < 0 or tokens < 0:
+            raise CudaError("kv_cache_read: negative extent")
+        shape = (rows, tokens, cache.heads, cache.head_dim)
+        key, value = (torch.empty(shape, dtype=torch.float16, device=cache.k.device) for _ in "kv")
+        if self.poison_outputs:
+            key.fill_(float("nan"))
+            value.fill_(float("nan"))
+        described = self._kv_tokens("kv_cache_read", cache, key, value, positions, counts, first_slot)
+        descriptor = cache.c_struct()
+        self.ctx.raise_for(self._lib.sdxlq_kv_cache_read(self.ctx.handle, ctypes.byref(descriptor), ctypes.byref(described)))
+        return key, value
+
+    # -- attention ------------------------------------------------------------------------------------------
+    def shared_prefix_attention(self, query: torch.Tensor, own: Optional[KVCache] = None, prefix: Optional[KVCache] = None, *,
+                                own_lengths: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None,
+                                causal: bool = False, scale: Optional[float] = None,
+                                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """softmax(scale * q k^T) v for FP16 queries [batch, tokens, q_heads, head_dim] over a prefix that several batch entries
+        share, then over keys and values of each entry's own. Either part may be missing.
+
+        prefix   entry b reads slot b // (batch / prefix.slots); all entries of a slot are worked on together where that
+                 reads it fewer times
+        own      one slot per entry
+        lengths  INT32 on the device, the tokens that a slot holds (None: its capacity)
+        causal   query i of an entry sees its own token j when j <= own_length - tokens + i; the prefix is seen by all
+        scale    1 / sqrt(head_dim) by default
+
+        q_heads is a multiple of the key heads, and key head h serves the query heads h * n .. h * n + n - 1. The parts may be of
+        unlike types. What lies behind a length or is hidden by the causal mask takes no part, whatever it holds, and a query
+        that sees no key gives zeros. `out` may be `query`."""
+        if query.dtype != torch.float16 or query.dim() != 4 or (query.shape[3] > 1 and query.stride(3) != 1):
+            raise CudaError("attention: expects FP16 queries [batch, tokens, q_heads, head_dim], a head's elements together")
+        y = out
+        if y is None:
+            y = torch.empty(query.shape, dtype=torch.float16, device=query.device)
+            if self.poison_outputs:
+                y.fill_(float("nan"))
+        elif y.dtype != torch.float16 or y.shape != query.shape or (y.shape[3] > 1 and y.stride(3) != 1) or \
+                any(y.stride(i) == 0 and y.shape[i] > 1 for i in range(3)):
+            raise CudaError("attention: the output must be like the queries")
+        batch, q_tokens, q_heads, head_dim = (int(n) for n in query.shape)
+        empty = _CKvCache()
+        parts = []
+        for part, lengths, what in ((prefix, prefix_lengths, "attention: prefix_lengths"), (own, own_lengths, "attention: own_lengths")):
+            if part is None and lengths is not None:
+                raise CudaError(f"{what} without the part that they are of")
+            if part is not None:
+                if part.slots == 0 and batch > 0:
+                    raise CudaError("attention: a part with no slots")
+                self._int32_vector(what, lengths, part.slots)
+                self._on_device("attention", part.k, lengths)
+            parts.append(empty if part is None else part.c_struct())
+        self._on_device("attention", query, y)
+        desc = _CAttentionDesc(query.data_ptr(), y.data_ptr(), batch, q_tokens, q_heads, head_dim, *_strides(query), *_strides(y),
+                               parts[0], parts[1], _ptr(prefix_lengths), _ptr(own_lengths),
+                               scale if scale is not None else (head_dim or 1) ** -0.5, int(causal), None, 0)
+        needed = self._lib.sdxlq_shared_prefix_attention_scratch(self.ctx.handle, ctypes.byref(desc))
+        if needed:
+            # of the call's own, so that calls on other streams and captured graphs share none of it
+            scratch = self.ctx.scratch(needed)
+            desc.scratch, desc.scratch_bytes = scratch.data_ptr(), needed
+        self.ctx.raise_for(self._lib.sdxlq_shared_prefix_attention(self.ctx.handle, ctypes.byref(desc)))
+        return y
 
     # -- Ops::quantize_fp8 / quantize_e4m3 / quantize_e5m2 ------------------------------------------
     def quantize_fp8(self, input: torch.Tensor, fp8_type: ScalarType) -> Weight:

@@ -1,0 +1,139 @@
+// Structures of the attention operators shared by the host dispatch and the kernels, and the arithmetic of a cache's
+// 8-bit types.
+#pragma once
+
+#include "fp8_math.cuh"
+#include "int8_math.cuh"
+#include "quantize.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace sdxlq {
+
+// Element type of a cache: the values of sdxlq_dtype.
+enum KvFormat : int { KV_E4M3 = 0, KV_E5M2 = 1, KV_INT8 = 2, KV_F16 = 3 };
+
+// Keys and values of some sequences. Strides in bytes.
+struct KvView {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scales;             // [slots, heads, capacity], null for FP16
+    float* v_scales;
+    const int32_t* lengths;      // [slots] or null: every slot holds `capacity` tokens (attention only)
+    int64_t slot_stride, token_stride, head_stride;
+    uint32_t slots, capacity;
+};
+
+// ---- writing and reading a cache ------------------------------------------------------------------------
+struct KvCopyLaunch {
+    KvView cache;
+    __half* k;                   // FP16 tokens
+    __half* v;
+    int64_t row_stride, token_stride, head_stride;      // elements
+    const int32_t* positions;    // [rows] or null: `start`
+    const int32_t* counts;       // [rows] or null: all `tokens`
+    uint32_t rows, tokens, heads, dim;
+    uint32_t first_slot, start;
+    uint32_t format;             // KvFormat
+};
+cudaError_t launch_kv_write(const KvCopyLaunch& launch, cudaStream_t stream, bool early_launch);
+cudaError_t launch_kv_read(const KvCopyLaunch& launch, cudaStream_t stream, bool early_launch);
+
+// ---- attention ------------------------------------------------------------------------------------------
+// Query rows of one key head are numbered r = (member * q_tokens + token) * repeat + head within the key head's group:
+// rows of several batch entries that read the same keys stand behind one another.
+//
+// A launch runs one or two passes. A pass takes `members` batch entries together (all that share a prefix, or one) over
+// the prefix, over the entries' own keys (members == 1), or over the one and then the other. Each of its items is a tile of
+// rows of one key head over one of `splits` shares of the keys. Where a row gets its result from one item alone, the item
+// writes it; else every item leaves its share in a slot of the scratch and the join kernel adds them up.
+struct AttentionPass {
+    uint32_t members, groups;    // batch = members * groups
+    uint32_t rows;               // members * q_tokens * repeat
+    uint32_t row_tiles, splits;
+    uint32_t items;              // row_tiles * splits * kv_heads * groups
+    uint32_t first_slot;         // scratch slot of split 0
+    uint32_t with_prefix, with_own;
+};
+
+struct AttentionParams {
+    const __half* q;
+    __half* y;
+    int64_t q_batch, q_token, q_head;        // strides, elements
+    int64_t y_batch, y_token, y_head;
+    KvView prefix, own;
+    uint32_t batch, q_tokens, q_heads, kv_heads, repeat, dim;
+    uint32_t rows_per_prefix;    // batch entries that share a prefix
+    uint32_t causal;
+    float scale_log2;            // softmax scale * log2(e)
+    uint32_t pass_count;
+    AttentionPass pass[2];
+    float* part_o;               // [slots, batch * q_tokens * q_heads, dim] shares, each divided by its own sum; null: no join
+    float* part_lse;             // [slots, batch * q_tokens * q_heads] log2 of the sum of 2^score, -inf for an empty share
+    uint32_t slots;
+    uint32_t y_vector;           // rows of y are 16-byte aligned
+};
+
+cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
+                                  bool early_launch);
+cudaError_t launch_attention_join(const AttentionParams& params, cudaStream_t stream, bool early_launch);
+
+// Where query row r of a pass's group lies.
+struct QueryRow {
+    uint32_t batch, token, head;
+};
+
+__device__ __forceinline__ QueryRow locate_row(const AttentionParams& p, uint32_t first_member, uint32_t kv_head, uint32_t r) {
+    const uint32_t head = r % p.repeat, position = r / p.repeat;
+    return {first_member + position / p.q_tokens, position % p.q_tokens, kv_head * p.repeat + head};
+}
+
+__device__ __forceinline__ uint32_t length_of(const KvView& view, uint32_t slot) {
+    if (view.lengths == nullptr) return view.capacity;
+    const int32_t length = __ldg(view.lengths + slot);
+    return length < 0 ? 0u : min(static_cast<uint32_t>(length), view.capacity);
+}
+
+// How many of `length` own keys query `token` sees under the causal mask: the queries are the last q_tokens of the
+// sequence. The prefix is seen by all.
+__device__ __forceinline__ uint32_t causal_limit(uint32_t length, uint32_t q_tokens, uint32_t token) {
+    const int64_t last = static_cast<int64_t>(length) - q_tokens + token + 1;
+    return last <= 0 ? 0u : static_cast<uint32_t>(last);
+}
+
+// Four bytes of a cache -> two words of FP16 pairs (bytes 0, 1 and bytes 2, 3) without their scale, exact. INT8: the byte
+// with its sign bit flipped is q + 128, and 0x6400 | u is the half 1024 + u; E5M2 is the upper byte of a half.
+template <int kFormat>
+__device__ __forceinline__ uint2 widen4(uint32_t bytes) {
+    uint2 r;
+    if constexpr (kFormat == KV_INT8) {
+        bytes ^= 0x80808080u;
+        const __half2 offset = __float2half2_rn(1152.0f);
+        const uint32_t lo = __byte_perm(bytes, 0x64646464u, 0x4140), hi = __byte_perm(bytes, 0x64646464u, 0x4342);
+        const __half2 a = __hsub2(as_half2(lo), offset), b = __hsub2(as_half2(hi), offset);
+        r.x = *reinterpret_cast<const uint32_t*>(&a);
+        r.y = *reinterpret_cast<const uint32_t*>(&b);
+    } else if constexpr (kFormat == KV_E5M2) {
+        r.x = __byte_perm(bytes, 0u, 0x1404);
+        r.y = __byte_perm(bytes, 0u, 0x3424);
+    } else {
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+            : "=r"(r.x), "=r"(r.y) : "r"(bytes));
+    }
+    return r;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+}  // namespace sdxlq

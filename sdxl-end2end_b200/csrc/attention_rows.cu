@@ -1,0 +1,597 @@
+// Attention of few query rows per key head over long keys: tokens of sequences that share a prefix (see attention.cuh for
+// rows, passes and items), and the kernel that joins the shares of the keys.
+//
+//   s_j = scale * q . k_j,  y = sum_j 2^(s_j log2 e - m) v_j / sum_j 2^(s_j log2 e - m)
+// in one pass over the keys with a running m. The sums stay as they are when m grows by less than 2^7: weights are kept
+// as halves, up to 2^6 at m and 2^13 above it, so that the smallest that a half resolves is 2^-31 of the weight at m.
+//
+// What bounds it: the bytes of the cache. Every warp of a block takes every fourth group of 16 (FP16) or 32 (8-bit) keys
+// and keeps its own sums, so that no warp waits for another before the end; keys and values go from global memory to the
+// registers of the warp's MMAs, 4 KB (heads of 64) or 8 KB (128) of them in flight per warp, and through no shared
+// memory. That works because the products do not care about the order of what they sum over:
+//   S = Q K^T: lane (g = lane / 4, t = lane % 4) holds for key g of a group of eight 16 consecutive bytes of the head, so
+//   the k index of the m16n8k16 MMA is a permutation of the head's dimensions, the same for Q.
+//   O = P V: the lane holds for keys 2t, 2t + 1, 2t + 8, 2t + 9 eight consecutive dimensions 8g .. 8g + 7, and MMA j takes
+//   the j-th of them, so its column g is dimension 8g + j.
+// An 8-bit cache enters the MMAs as exact halves without its scales. A key's scale multiplies its column of S; a value's
+// multiplies its weight, relative to the largest value scale so far (else weights of small-scaled values would fall
+// below the halves), which the sums are divided by.
+
+#include "attention.cuh"
+
+namespace sdxlq {
+
+namespace {
+
+constexpr uint32_t kWarps = 4;
+constexpr float kWeightBits = 6.0f;      // a weight at the running maximum is 2^6
+constexpr float kSlackBits = 7.0f;       // the maximum may be passed by this much before the sums are rescaled
+constexpr float kScaleSlack = 4.0f;      // the same for the largest value scale
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 load_vector16(const uint8_t* base, bool inside) {
+    return inside ? __ldg(reinterpret_cast<const uint4*>(base)) : make_uint4(0u, 0u, 0u, 0u);
+}
+__device__ __forceinline__ uint2 load_vector8(const uint8_t* base, bool inside) {
+    return inside ? __ldg(reinterpret_cast<const uint2*>(base)) : make_uint2(0u, 0u);
+}
+
+// A group of keys in registers, as the MMAs take it.
+template <int kDim, int kFormat>
+struct KeyBlock {
+    static constexpr bool kHalf = kFormat == KV_F16;
+    static constexpr int kKeys = kHalf ? 16 : 32;
+    static constexpr int kTiles = kKeys / 8;             // groups of eight keys
+    static constexpr int kVectors = kHalf ? kDim / 32 : kDim / 64;
+    uint4 word[kTiles][kVectors];
+    float scale[kHalf ? 1 : kTiles][2];
+
+    __device__ __forceinline__ void load(const KvView& view, const uint8_t* keys, const float* scales, uint32_t first, uint32_t end,
+                                         uint32_t dim, uint32_t g, uint32_t t) {
+#pragma unroll
+        for (int tile = 0; tile < kTiles; ++tile) {
+            const uint32_t key = first + tile * 8u + g;
+            const uint8_t* const row = keys + key * view.token_stride;
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) {
+                const uint32_t d = kHalf ? v * 32u + t * 8u : v * 64u + t * 16u;
+                word[tile][v] = load_vector16(row + d * (kHalf ? 2u : 1u), key < end && d < dim);
+            }
+            if constexpr (!kHalf) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t column = first + tile * 8u + 2u * t + i;
+                    scale[tile][i] = column < end ? __ldg(scales + column) : 0.0f;
+                }
+            }
+        }
+    }
+
+    // The B operand of MMA step `step` (16 dimensions) for group `tile`.
+    __device__ __forceinline__ uint2 operand(int tile, int step) const {
+        if constexpr (kHalf) {
+            const uint4 w = word[tile][step / 2];
+            return step % 2 == 0 ? make_uint2(w.x, w.y) : make_uint2(w.z, w.w);
+        } else {
+            const uint4 w = word[tile][step / 4];
+            const uint32_t bytes = step % 4 == 0 ? w.x : step % 4 == 1 ? w.y : step % 4 == 2 ? w.z : w.w;
+            return widen4<kFormat>(bytes);
+        }
+    }
+
+    // First of the four dimensions that lane t has in MMA step `step`.
+    static __device__ __forceinline__ uint32_t dimension(int step, uint32_t t) {
+        return kHalf ? step / 2 * 32u + t * 8u + step % 2 * 4u : step / 4 * 64u + t * 16u + step % 4 * 4u;
+    }
+};
+
+template <int kDim, int kFormat>
+struct ValueBlock {
+    static constexpr bool kHalf = kFormat == KV_F16;
+    static constexpr int kKeys = kHalf ? 16 : 32;
+    static constexpr int kVectors = kDim / 64;
+    uint4 word16[kHalf ? kKeys / 4 : 1][kVectors];
+    uint2 word8[kHalf ? 1 : kKeys / 4][kVectors];
+    float scale[kHalf ? 1 : kKeys / 4];
+
+    // the lane's i-th key of the group
+    static __device__ __forceinline__ uint32_t key_of(int i, uint32_t t) { return i / 4 * 16u + i / 2 % 2 * 8u + 2u * t + i % 2; }
+
+    __device__ __forceinline__ void load(const KvView& view, const uint8_t* values, const float* scales, uint32_t first, uint32_t end,
+                                         uint32_t dim, uint32_t g, uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 4; ++i) {
+            const uint32_t key = first + key_of(i, t);
+            const uint8_t* const row = values + key * view.token_stride;
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) {
+                const uint32_t d = v * 64u + g * 8u;
+                if constexpr (kHalf) word16[i][v] = load_vector16(row + d * 2u, key < end && d < dim);
+                else word8[i][v] = load_vector8(row + d, key < end && d < dim);
+            }
+            if constexpr (!kHalf) scale[i] = key < end ? __ldg(scales + key) : 0.0f;
+        }
+    }
+
+    // The B operands of the 16 keys `step` for dimensions 4 `quad` .. + 3 of the lane's eight in vector v: four MMAs.
+    __device__ __forceinline__ void operands(int step, int v, int quad, uint32_t (&b0)[4], uint32_t (&b1)[4]) const {
+        if constexpr (kHalf) {
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 x = word16[step * 4 + i][v];
+                    w[i] = quad == 0 ? (pair == 0 ? x.x : x.y) : (pair == 0 ? x.z : x.w);
+                }
+                b0[pair * 2] = __byte_perm(w[0], w[1], 0x5410);
+                b0[pair * 2 + 1] = __byte_perm(w[0], w[1], 0x7632);
+                b1[pair * 2] = __byte_perm(w[2], w[3], 0x5410);
+                b1[pair * 2 + 1] = __byte_perm(w[2], w[3], 0x7632);
+            }
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = quad == 0 ? word8[step * 4 + i][v].x : word8[step * 4 + i][v].y;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t select = half == 0 ? 0x5140u : 0x7362u;
+                const uint2 a = widen4<kFormat>(__byte_perm(w[0], w[1], select)), b = widen4<kFormat>(__byte_perm(w[2], w[3], select));
+                b0[half * 2] = a.x;
+                b0[half * 2 + 1] = a.y;
+                b1[half * 2] = b.x;
+                b1[half * 2 + 1] = b.y;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ bool has_non_finite(uint32_t pair) {
+    return (pair & 0x7C00u) == 0x7C00u || (pair & 0x7C000000u) == 0x7C000000u;
+}
+
+// kRowTiles: tiles of 16 rows per warp.
+template <int kDim, int kFormat, int kRowTiles>
+__global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
+    using Keys = KeyBlock<kDim, kFormat>;
+    using Values = ValueBlock<kDim, kFormat>;
+    constexpr int kSteps = kDim / 16, kKeys = Keys::kKeys, kTiles = Keys::kTiles;
+    constexpr int kTileRows = 16 * kRowTiles, kPitch = kDim + 4;
+    constexpr bool kScaled = kFormat != KV_F16;
+    extern __shared__ float shared[];
+    float* const shared_o = shared;                                      // [kWarps][kTileRows][kPitch]
+    float* const shared_m = shared + kWarps * kTileRows * kPitch;        // [kWarps][kTileRows]
+    float* const shared_l = shared_m + kWarps * kTileRows;
+
+    wait_for_prior_kernels_then_release_next();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
+    const AttentionPass& pass = p.pass[second ? 1 : 0];
+    uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
+    const uint32_t row_tile = item % pass.row_tiles;
+    item /= pass.row_tiles;
+    const uint32_t split = item % pass.splits;
+    item /= pass.splits;
+    const uint32_t kv_head = item % p.kv_heads, first_member = item / p.kv_heads * pass.members;
+    const uint32_t first_row = row_tile * kTileRows;
+
+    // the keys of the item: blocks of the prefix, then of the entry's own keys
+    const uint32_t prefix_slot = pass.with_prefix ? first_member / p.rows_per_prefix : 0u;
+    const uint32_t prefix_length = pass.with_prefix ? length_of(p.prefix, prefix_slot) : 0u;
+    const uint32_t own_length = pass.with_own ? length_of(p.own, first_member) : 0u;
+    const uint32_t prefix_blocks = (prefix_length + kKeys - 1) / kKeys, own_blocks = (own_length + kKeys - 1) / kKeys;
+    const uint64_t blocks = static_cast<uint64_t>(prefix_blocks) + own_blocks;
+    const uint32_t block_begin = static_cast<uint32_t>(blocks * split / pass.splits);
+    const uint32_t block_end = static_cast<uint32_t>(blocks * (split + 1) / pass.splits);
+
+    // Q, and how many own keys each of the lane's rows sees
+    uint32_t q[kRowTiles][kSteps][4];
+    uint32_t limit[kRowTiles][2];
+    uint32_t least_limit = own_length;
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t r = first_row + rt * 16u + half * 8u + g;
+            const bool inside = r < pass.rows;
+            const QueryRow at = locate_row(p, first_member, kv_head, inside ? r : 0u);
+            const __half* const row = p.q + at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head;
+#pragma unroll
+            for (int step = 0; step < kSteps; ++step) {
+                const uint32_t d = Keys::dimension(step, t);
+                const uint2 x = inside && d < p.dim ? __ldg(reinterpret_cast<const uint2*>(row + d)) : make_uint2(0u, 0u);
+                q[rt][step][half] = x.x;
+                q[rt][step][half + 2] = x.y;
+            }
+            limit[rt][half] = p.causal ? causal_limit(own_length, p.q_tokens, at.token) : own_length;
+            least_limit = min(least_limit, limit[rt][half]);
+        }
+    }
+    least_limit = __reduce_min_sync(0xffffffffu, least_limit);
+
+    float o[kRowTiles][kDim / 8][4] = {};
+    float row_max[kRowTiles][2], row_sum[kRowTiles][2];
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt) {
+        row_max[rt][0] = row_max[rt][1] = __int_as_float(0xff800000);
+        row_sum[rt][0] = row_sum[rt][1] = 0.0f;
+    }
+    float scale_reference = 0.0f;        // the value scale that the sums are relative to (8-bit caches)
+
+    const auto rescale = [&](int rt, float factor0, float factor1) {
+#pragma unroll
+        for (int n = 0; n < kDim / 8; ++n) {
+            o[rt][n][0] *= factor0;
+            o[rt][n][1] *= factor0;
+            o[rt][n][2] *= factor1;
+            o[rt][n][3] *= factor1;
+        }
+    };
+
+    // where a block's keys are
+    struct Place {
+        const uint8_t* k;
+        const uint8_t* v;
+        const float* k_scales;
+        const float* v_scales;
+        uint32_t first, end;
+    };
+    const auto view_of = [&](uint32_t block) -> const KvView& { return block < prefix_blocks ? p.prefix : p.own; };
+    const auto place = [&](uint32_t block) {
+        const bool in_prefix = block < prefix_blocks;
+        const KvView& view = view_of(block);
+        const int64_t slot = in_prefix ? prefix_slot : first_member;
+        const int64_t base = slot * view.slot_stride + kv_head * view.head_stride;
+        const int64_t scales = (slot * p.kv_heads + kv_head) * view.capacity;
+        Place at;
+        at.k = view.k + base;
+        at.v = view.v + base;
+        at.k_scales = kScaled ? view.k_scales + scales : nullptr;
+        at.v_scales = kScaled ? view.v_scales + scales : nullptr;
+        at.first = (in_prefix ? block : block - prefix_blocks) * kKeys;
+        at.end = in_prefix ? prefix_length : own_length;
+        return at;
+    };
+
+    Keys keys;
+    Values values;
+    uint32_t block = block_begin + warp;
+    if (block < block_end) {
+        const Place at = place(block);
+        keys.load(view_of(block), at.k, at.k_scales, at.first, at.end, p.dim, g, t);
+        values.load(view_of(block), at.v, at.v_scales, at.first, at.end, p.dim, g, t);
+    }
+    while (block < block_end) {
+        const bool in_prefix = block < prefix_blocks;
+        const uint32_t first = (in_prefix ? block : block - prefix_blocks) * kKeys;
+        const uint32_t next = block + kWarps;
+
+        float s[kRowTiles][kTiles][4] = {};
+#pragma unroll
+        for (int tile = 0; tile < kTiles; ++tile) {
+#pragma unroll
+            for (int step = 0; step < kSteps; ++step) {
+                const uint2 b = keys.operand(tile, step);
+#pragma unroll
+                for (int rt = 0; rt < kRowTiles; ++rt) mma_f16(s[rt][tile], q[rt][step], b.x, b.y);
+            }
+        }
+        float key_scale[kTiles][2];
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                key_scale[tile][0] = keys.scale[tile][0] * p.scale_log2;
+                key_scale[tile][1] = keys.scale[tile][1] * p.scale_log2;
+            }
+        }
+        if (next < block_end) {          // the next keys travel while this block is worked on
+            const Place at = place(next);
+            keys.load(view_of(next), at.k, at.k_scales, at.first, at.end, p.dim, g, t);
+        }
+
+        const uint32_t seen_by_all = in_prefix ? prefix_length : least_limit;
+        const bool masked = first + kKeys > seen_by_all;
+        float value_factor = 1.0f;
+        if constexpr (kScaled) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kKeys / 4; ++i) largest = fmaxf(largest, values.scale[i]);
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            if (largest > kScaleSlack * scale_reference) {
+                const float factor = scale_reference / largest;
+                scale_reference = largest;
+#pragma unroll
+                for (int rt = 0; rt < kRowTiles; ++rt) rescale(rt, factor, factor);
+            }
+            value_factor = scale_reference > 0.0f ? 1.0f / scale_reference : 0.0f;
+        }
+
+        uint32_t weights[kRowTiles][kTiles / 2][4];
+#pragma unroll
+        for (int rt = 0; rt < kRowTiles; ++rt) {
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    s[rt][tile][c] *= kScaled ? key_scale[tile][c & 1] : p.scale_log2;
+                    if (masked) {
+                        const uint32_t key = first + tile * 8u + 2u * t + (c & 1);
+                        if (key >= (in_prefix ? prefix_length : limit[rt][c >> 1])) s[rt][tile][c] = __int_as_float(0xff800000);
+                    }
+                }
+            }
+            float shift[2];
+            float grow[2];
+            bool grown = false;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float largest = __int_as_float(0xff800000);
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) largest = fmaxf(largest, fmaxf(s[rt][tile][2 * half], s[rt][tile][2 * half + 1]));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                grow[half] = 1.0f;
+                if (largest > row_max[rt][half] + kSlackBits) {
+                    grow[half] = exp2_approx(row_max[rt][half] - largest);
+                    row_max[rt][half] = largest;
+                    grown = true;
+                }
+                shift[half] = row_max[rt][half] > __int_as_float(0xff800000) ? kWeightBits - row_max[rt][half] : 0.0f;
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+                row_sum[rt][0] *= grow[0];
+                row_sum[rt][1] *= grow[1];
+                rescale(rt, grow[0], grow[1]);
+            }
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                float w[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    w[c] = exp2_approx(s[rt][tile][c] + shift[c >> 1]);
+                    row_sum[rt][c >> 1] += w[c];
+                    if constexpr (kScaled) {
+                        const float factor = values.scale[tile / 2 * 4 + tile % 2 * 2 + (c & 1)] * value_factor;
+                        w[c] = s[rt][tile][c] == __int_as_float(0xff800000) ? 0.0f : w[c] * factor;
+                    }
+                }
+                weights[rt][tile / 2][tile % 2 * 2] = pack_half2(w[0], w[1]);
+                weights[rt][tile / 2][tile % 2 * 2 + 1] = pack_half2(w[2], w[3]);
+            }
+        }
+
+        // A value that is not finite makes 0 * v a NaN, also where the weight is 0 because the row does not see the key.
+        // Keys behind a sequence's end were loaded as zeros; those that the causal mask hides from some rows of the tile
+        // and not from others are looked through here.
+        bool row_by_row = false;
+        if (kFormat != KV_INT8 && masked && !in_prefix && p.causal) {
+            bool found = false;
+#pragma unroll
+            for (int step = 0; step < kKeys / 16; ++step) {
+#pragma unroll
+                for (int v = 0; v < Values::kVectors; ++v) {
+#pragma unroll
+                    for (int quad = 0; quad < 2; ++quad) {
+                        uint32_t b0[4], b1[4];
+                        values.operands(step, v, quad, b0, b1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) found = found || has_non_finite(b0[i]) || has_non_finite(b1[i]);
+                    }
+                }
+            }
+            row_by_row = __any_sync(0xffffffffu, found);
+        }
+        if (!row_by_row) {
+#pragma unroll
+            for (int step = 0; step < kKeys / 16; ++step) {
+#pragma unroll
+                for (int v = 0; v < Values::kVectors; ++v) {
+#pragma unroll
+                    for (int quad = 0; quad < 2; ++quad) {
+                        uint32_t b0[4], b1[4];
+                        values.operands(step, v, quad, b0, b1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                            for (int rt = 0; rt < kRowTiles; ++rt) mma_f16(o[rt][v * 8 + quad * 4 + i], weights[rt][step], b0[i], b1[i]);
+                        }
+                    }
+                }
+            }
+        } else {
+            // one row at a time, the keys that it does not see as zeros
+            for (int rt = 0; rt < kRowTiles; ++rt) {
+                for (uint32_t r = 0; r < 16; ++r) {
+                    const uint32_t mine = r < 8 ? limit[0][0] : limit[0][1];
+                    const uint32_t other = kRowTiles > 1 ? (r < 8 ? limit[kRowTiles - 1][0] : limit[kRowTiles - 1][1]) : mine;
+                    const uint32_t seen = __shfl_sync(0xffffffffu, rt == 0 ? mine : other, (r & 7u) * 4u);
+#pragma unroll
+                    for (int step = 0; step < kKeys / 16; ++step) {
+                        const uint32_t key = first + step * 16u + 2u * t;
+                        const uint32_t keep0 = (key < seen ? 0xFFFFu : 0u) | (key + 1u < seen ? 0xFFFF0000u : 0u);
+                        const uint32_t keep1 = (key + 8u < seen ? 0xFFFFu : 0u) | (key + 9u < seen ? 0xFFFF0000u : 0u);
+#pragma unroll
+                        for (int v = 0; v < Values::kVectors; ++v) {
+#pragma unroll
+                            for (int quad = 0; quad < 2; ++quad) {
+                                uint32_t b0[4], b1[4];
+                                values.operands(step, v, quad, b0, b1);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int n = v * 8 + quad * 4 + i;
+#pragma unroll
+                                    for (int tile = 0; tile < kRowTiles; ++tile) {
+                                        float sum[4] = {};
+                                        mma_f16(sum, weights[tile][step], b0[i] & keep0, b1[i] & keep1);
+                                        if (tile == rt && g == (r & 7u)) {
+                                            if (r < 8) {
+                                                o[tile][n][0] += sum[0];
+                                                o[tile][n][1] += sum[1];
+                                            } else {
+                                                o[tile][n][2] += sum[2];
+                                                o[tile][n][3] += sum[3];
+                                            }
+                                        }
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (next < block_end) {
+            const Place at = place(next);
+            values.load(view_of(next), at.v, at.v_scales, at.first, at.end, p.dim, g, t);
+        }
+        block = next;
+    }
+
+    // the warps' sums meet in shared memory
+#pragma unroll
+    for (int rt = 0; rt < kRowTiles; ++rt) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float sum = row_sum[rt][half];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const uint32_t r = rt * 16u + half * 8u + g;
+            if (t == 0) {
+                shared_m[warp * kTileRows + r] = row_max[rt][half];
+                shared_l[warp * kTileRows + r] = sum;
+            }
+            float* const row = shared_o + (warp * kTileRows + r) * kPitch;
+#pragma unroll
+            for (int v = 0; v < kDim / 64; ++v) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float unit = kScaled ? scale_reference : 1.0f;
+                    row[v * 64 + 16u * t + j] = o[rt][v * 8 + j][2 * half] * unit;
+                    row[v * 64 + 16u * t + 8 + j] = o[rt][v * 8 + j][2 * half + 1] * unit;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (uint32_t index = threadIdx.x; index < kTileRows * (kDim / 8); index += 32 * kWarps) {
+        const uint32_t r = index / (kDim / 8), d = index % (kDim / 8) * 8u;
+        if (first_row + r >= pass.rows || d >= p.dim) continue;
+        float largest = __int_as_float(0xff800000);
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) largest = fmaxf(largest, shared_m[w * kTileRows + r]);
+        float total = 0.0f, sum[8] = {};
+        if (largest > __int_as_float(0xff800000)) {
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                const float share = exp2_approx(shared_m[w * kTileRows + r] - largest);
+                total = fmaf(shared_l[w * kTileRows + r], share, total);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] = fmaf(shared_o[(w * kTileRows + r) * kPitch + d + j], share, sum[j]);
+            }
+        } else {
+            // no score above -inf: an empty row, or one whose scores are all NaN or -inf, which carries its sums' NaN
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                total += shared_l[w * kTileRows + r];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += shared_o[(w * kTileRows + r) * kPitch + d + j];
+            }
+        }
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        const QueryRow at = locate_row(p, first_member, kv_head, first_row + r);
+        if (p.part_o == nullptr) {
+            __half* const row = p.y + at.batch * p.y_batch + at.token * p.y_token + at.head * p.y_head + d;
+            const uint4 packed = make_uint4(pack_half2(sum[0] * inverse, sum[1] * inverse), pack_half2(sum[2] * inverse, sum[3] * inverse),
+                                            pack_half2(sum[4] * inverse, sum[5] * inverse), pack_half2(sum[6] * inverse, sum[7] * inverse));
+            *reinterpret_cast<uint4*>(row) = packed;
+        } else {
+            const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
+            const uint64_t row = (static_cast<uint64_t>(at.batch) * p.q_tokens + at.token) * p.q_heads + at.head;
+            const uint64_t place_in_slot = (pass.first_slot + split) * rows + row;
+            float4* const out = reinterpret_cast<float4*>(p.part_o + place_in_slot * p.dim + d);
+            out[0] = make_float4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
+            out[1] = make_float4(sum[4] * inverse, sum[5] * inverse, sum[6] * inverse, sum[7] * inverse);
+            if (d == 0) p.part_lse[place_in_slot] = total == 0.0f ? __int_as_float(0xff800000) : largest + log2f(total) - kWeightBits;
+        }
+    }
+}
+
+// y = sum_s 2^lse_s o_s / sum_s 2^lse_s over the shares of each row, in the order of the slots. A lane takes eight
+// dimensions of a row.
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+    wait_for_prior_kernels_then_release_next();
+    const uint32_t vectors = p.dim / 8;
+    const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
+    const uint64_t index = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const uint64_t row = index / vectors;
+    if (row >= rows) return;
+    const uint32_t d = static_cast<uint32_t>(index % vectors) * 8u;
+    float largest = __int_as_float(0xff800000);
+    for (uint32_t s = 0; s < p.slots; ++s) largest = fmaxf(largest, p.part_lse[s * rows + row]);
+    float total = 0.0f, sum[8] = {};
+    for (uint32_t s = 0; s < p.slots; ++s) {
+        const float lse = p.part_lse[s * rows + row];
+        if (lse == __int_as_float(0xff800000)) continue;         // an empty share
+        const float share = exp2_approx(lse - largest);
+        const float4* const part = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.dim + d);
+        const float4 a = part[0], b = part[1];
+        total += share;
+        sum[0] = fmaf(a.x, share, sum[0]); sum[1] = fmaf(a.y, share, sum[1]); sum[2] = fmaf(a.z, share, sum[2]); sum[3] = fmaf(a.w, share, sum[3]);
+        sum[4] = fmaf(b.x, share, sum[4]); sum[5] = fmaf(b.y, share, sum[5]); sum[6] = fmaf(b.z, share, sum[6]); sum[7] = fmaf(b.w, share, sum[7]);
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const uint32_t head = static_cast<uint32_t>(row % p.q_heads);
+    const uint64_t position = row / p.q_heads;
+    const uint64_t b = position / p.q_tokens, token = position % p.q_tokens;
+    __half* const out = p.y + b * p.y_batch + token * p.y_token + head * p.y_head + d;
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack_half2(sum[0] * inverse, sum[1] * inverse), pack_half2(sum[2] * inverse, sum[3] * inverse),
+                                                pack_half2(sum[4] * inverse, sum[5] * inverse), pack_half2(sum[6] * inverse, sum[7] * inverse));
+}
+
+template <int kDim, int kFormat, int kRowTiles>
+cudaError_t launch_tile(const AttentionParams& params, cudaStream_t stream, bool early_launch) {
+    constexpr size_t bytes = sizeof(float) * kWarps * 16 * kRowTiles * (kDim + 4 + 2);
+    auto* const kernel = attention_rows_kernel<kDim, kFormat, kRowTiles>;
+    if constexpr (bytes > 48 * 1024) {
+        const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+        if (error != cudaSuccess) return error;
+    }
+    uint32_t blocks = 0;
+    for (uint32_t i = 0; i < params.pass_count; ++i) blocks += params.pass[i].items;
+    return launch_behind(kernel, blocks, 32 * kWarps, bytes, stream, early_launch, params);
+}
+
+template <int kFormat>
+cudaError_t launch_format(const AttentionParams& params, uint32_t row_tile, cudaStream_t stream, bool early_launch) {
+    if (params.dim <= 64) {
+        return row_tile == 16 ? launch_tile<64, kFormat, 1>(params, stream, early_launch) : launch_tile<64, kFormat, 2>(params, stream, early_launch);
+    }
+    return row_tile == 16 ? launch_tile<128, kFormat, 1>(params, stream, early_launch) : launch_tile<128, kFormat, 2>(params, stream, early_launch);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
+                                  bool early_launch) {
+    switch (format) {
+    case KV_E4M3: return launch_format<KV_E4M3>(params, row_tile, stream, early_launch);
+    case KV_E5M2: return launch_format<KV_E5M2>(params, row_tile, stream, early_launch);
+    case KV_INT8: return launch_format<KV_INT8>(params, row_tile, stream, early_launch);
+    default: return launch_format<KV_F16>(params, row_tile, stream, early_launch);
+    }
+}
+
+cudaError_t launch_attention_join(const AttentionParams& params, cudaStream_t stream, bool early_launch) {
+    const uint64_t threads = static_cast<uint64_t>(params.batch) * params.q_tokens * params.q_heads * (params.dim / 8);
+    const uint64_t blocks = (threads + 127) / 128;
+    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    return launch_behind(attention_join_kernel, static_cast<uint32_t>(blocks), 128, 0, stream, early_launch, params);
+}
+
+}  // namespace sdxlq

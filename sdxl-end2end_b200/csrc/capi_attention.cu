@@ -1,0 +1,319 @@
+// C ABI of the attention operators: validation and dispatch of the cache's copies and of shared-prefix attention.
+
+#include "attention.cuh"
+#include "context.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+using namespace sdxlq;
+
+namespace {
+
+// The context's device is the current one while this lives.
+class DeviceScope {
+public:
+    explicit DeviceScope(const sdxlq_context* ctx) {
+        if (cudaGetDevice(&previous_) != cudaSuccess) return;
+        changed_ = previous_ != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess;
+    }
+    ~DeviceScope() {
+        if (changed_) cudaSetDevice(previous_);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+
+private:
+    int previous_ = 0;
+    bool changed_ = false;
+};
+
+constexpr uint64_t kMaxExtent = 0x7FFFFFFFull;
+constexpr uint64_t kMaxStride = uint64_t(1) << 40;       // elements: offsets stay within 63 bits for any extents below
+
+bool is_kv_type(int32_t dtype) { return is_fp8(dtype) || dtype == SDXLQ_INT8 || dtype == SDXLQ_FP16; }
+uint64_t element_bytes(int32_t dtype) { return dtype == SDXLQ_FP16 ? 2 : 1; }
+bool aligned16(const void* pointer) { return reinterpret_cast<uintptr_t>(pointer) % 16 == 0; }
+bool strides_ok(uint64_t bytes, uint64_t a, uint64_t b, uint64_t c) {
+    return a <= kMaxStride && b <= kMaxStride && c <= kMaxStride && a * bytes % 16 == 0 && b * bytes % 16 == 0 && c * bytes % 16 == 0;
+}
+
+bool absent(const sdxlq_kv_cache& c) { return c.slots == 0; }
+
+// The checks that every reader and writer of a cache makes.
+int validate_cache(sdxlq_context* ctx, const sdxlq_kv_cache& c) {
+    if (!is_kv_type(c.dtype)) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: expects FP16, INT8 or FP8 elements");
+    // a cache without room for a token has no memory
+    if (c.capacity != 0 && (c.k == nullptr || c.v == nullptr)) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: null keys or values");
+    if (c.capacity != 0 && c.dtype != SDXLQ_FP16 && (c.k_scales == nullptr || c.v_scales == nullptr)) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: an 8-bit cache needs scales");
+    }
+    if (c.heads == 0 || c.head_dim == 0) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: no heads");
+    if (c.slots > kMaxExtent || c.capacity > kMaxExtent || c.heads > kMaxExtent) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "kv cache: dimensions too large");
+    }
+    const uint64_t unit = c.dtype == SDXLQ_FP16 ? 8 : 16;
+    if (c.head_dim % unit != 0 || c.head_dim > 128) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE,
+                    "kv cache: heads of at most 128 elements, a multiple of 8 for FP16 and of 16 for 8-bit types");
+    }
+    if (!aligned16(c.k) || !aligned16(c.v) || !strides_ok(element_bytes(c.dtype), c.slot_stride, c.token_stride, c.head_stride)) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "kv cache: keys, values and their strides must be multiples of 16 bytes");
+    }
+    return SDXLQ_OK;
+}
+
+KvView view_of(const sdxlq_kv_cache& c, const int32_t* lengths) {
+    const int64_t bytes = static_cast<int64_t>(element_bytes(c.dtype));
+    KvView v{};
+    v.k = static_cast<uint8_t*>(c.k);
+    v.v = static_cast<uint8_t*>(c.v);
+    v.k_scales = c.k_scales;
+    v.v_scales = c.v_scales;
+    v.lengths = lengths;
+    v.slot_stride = static_cast<int64_t>(c.slot_stride) * bytes;
+    v.token_stride = static_cast<int64_t>(c.token_stride) * bytes;
+    v.head_stride = static_cast<int64_t>(c.head_stride) * bytes;
+    v.slots = static_cast<uint32_t>(c.slots);
+    v.capacity = static_cast<uint32_t>(c.capacity);
+    return v;
+}
+
+bool early(const sdxlq_context* ctx) { return ctx->early_launch && !ctx->profiling; }
+
+int copy_tokens(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens, bool write) {
+    if (cache == nullptr || tokens == nullptr) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: null descriptor");
+    const sdxlq_kv_tokens& t = *tokens;
+    if (t.rows == 0 || t.tokens == 0) return SDXLQ_OK;
+    const int status = validate_cache(ctx, *cache);
+    if (status != SDXLQ_OK) return status;
+    if (t.k == nullptr || t.v == nullptr) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: null tokens");
+    if (t.first_slot > cache->slots || t.rows > cache->slots - t.first_slot) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: more rows than slots");
+    }
+    if (t.tokens > kMaxExtent || t.start > kMaxExtent) return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "kv cache: dimensions too large");
+    if (t.positions == nullptr && (t.start > cache->capacity || t.tokens > cache->capacity - t.start)) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: tokens behind the capacity");
+    }
+    if (!aligned16(t.k) || !aligned16(t.v) || !strides_ok(2, t.row_stride, t.token_stride, t.head_stride)) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "kv cache: tokens and their strides must be multiples of 16 bytes");
+    }
+    KvCopyLaunch launch{};
+    launch.cache = view_of(*cache, nullptr);
+    launch.k = static_cast<__half*>(t.k);
+    launch.v = static_cast<__half*>(t.v);
+    launch.row_stride = static_cast<int64_t>(t.row_stride);
+    launch.token_stride = static_cast<int64_t>(t.token_stride);
+    launch.head_stride = static_cast<int64_t>(t.head_stride);
+    launch.positions = t.positions;
+    launch.counts = t.counts;
+    launch.rows = static_cast<uint32_t>(t.rows);
+    launch.tokens = static_cast<uint32_t>(t.tokens);
+    launch.heads = static_cast<uint32_t>(cache->heads);
+    launch.dim = static_cast<uint32_t>(cache->head_dim);
+    launch.first_slot = static_cast<uint32_t>(t.first_slot);
+    launch.start = static_cast<uint32_t>(t.start);
+    launch.format = static_cast<uint32_t>(cache->dtype);
+    const DeviceScope device(ctx);
+    LaunchTimer timer(ctx, SDXLQ_KERNEL_HARNESS);
+    const cudaError_t error = write ? launch_kv_write(launch, ctx->stream, early(ctx)) : launch_kv_read(launch, ctx->stream, early(ctx));
+    if (error == cudaErrorInvalidConfiguration) return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "kv cache: too many vectors for one call");
+    if (error != cudaSuccess) return fail_cuda(ctx, error, "kv cache launch");
+    return SDXLQ_OK;
+}
+
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// A call's passes, and what its launches need.
+struct AttentionPlan {
+    AttentionParams params{};
+    KvFormat format[2] = {KV_F16, KV_F16};       // of each pass
+    uint32_t row_tile = 16;
+    uint64_t scratch_bytes = 0;
+};
+
+int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc& d, AttentionPlan& plan) {
+    if (d.q == nullptr || d.y == nullptr) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: null query or output pointer");
+    if (d.q_heads == 0 || d.head_dim == 0) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: no heads");
+    if (d.batch > kMaxExtent || d.q_tokens > kMaxExtent || d.q_heads > kMaxExtent || d.batch * d.q_tokens > kMaxExtent ||
+        d.batch * d.q_tokens * d.q_heads > kMaxExtent) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: dimensions too large");
+    }
+    if (d.head_dim % 8 != 0 || d.head_dim > 128) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: heads of at most 128 elements, a multiple of 8");
+    }
+    if (!aligned16(d.q) || !aligned16(d.y) || !strides_ok(2, d.q_batch_stride, d.q_token_stride, d.q_head_stride) ||
+        !strides_ok(2, d.y_batch_stride, d.y_token_stride, d.y_head_stride)) {
+        return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: queries, outputs and their strides must be multiples of 16 bytes");
+    }
+    if (!std::isfinite(d.scale)) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: the scale must be finite");
+    const bool with_prefix = !absent(d.prefix), with_own = !absent(d.own);
+    if (!with_prefix && !with_own) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: neither a prefix nor keys of its own");
+    for (const sdxlq_kv_cache* part : {with_prefix ? &d.prefix : nullptr, with_own ? &d.own : nullptr}) {
+        if (part == nullptr) continue;
+        const int status = validate_cache(ctx, *part);
+        if (status != SDXLQ_OK) return status;
+        if (part->head_dim != d.head_dim) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: queries and keys differ in head size");
+        if (d.q_heads % part->heads != 0) {
+            return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: query heads must be a multiple of key heads");
+        }
+    }
+    if (with_prefix && with_own && d.prefix.heads != d.own.heads) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: prefix and own keys differ in heads");
+    }
+    if (with_own && d.own.slots != d.batch) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: own keys must have a slot per batch entry");
+    if (with_prefix && d.batch % d.prefix.slots != 0) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: the batch must be a multiple of the prefixes");
+    }
+
+    AttentionParams& p = plan.params;
+    p.q = static_cast<const __half*>(d.q);
+    p.y = static_cast<__half*>(d.y);
+    p.q_batch = static_cast<int64_t>(d.q_batch_stride);
+    p.q_token = static_cast<int64_t>(d.q_token_stride);
+    p.q_head = static_cast<int64_t>(d.q_head_stride);
+    p.y_batch = static_cast<int64_t>(d.y_batch_stride);
+    p.y_token = static_cast<int64_t>(d.y_token_stride);
+    p.y_head = static_cast<int64_t>(d.y_head_stride);
+    if (with_prefix) p.prefix = view_of(d.prefix, d.prefix_lengths);
+    if (with_own) p.own = view_of(d.own, d.own_lengths);
+    p.batch = static_cast<uint32_t>(d.batch);
+    p.q_tokens = static_cast<uint32_t>(d.q_tokens);
+    p.q_heads = static_cast<uint32_t>(d.q_heads);
+    p.kv_heads = static_cast<uint32_t>(with_prefix ? d.prefix.heads : d.own.heads);
+    p.repeat = p.q_heads / p.kv_heads;
+    p.dim = static_cast<uint32_t>(d.head_dim);
+    p.rows_per_prefix = with_prefix ? p.batch / static_cast<uint32_t>(d.prefix.slots) : 1u;
+    p.causal = d.causal != 0 ? 1u : 0u;
+    p.scale_log2 = d.scale * 1.4426950408889634f;
+    if (d.batch == 0 || d.q_tokens == 0) return SDXLQ_OK;
+
+    const uint64_t entry_rows = static_cast<uint64_t>(p.q_tokens) * p.repeat;
+    plan.row_tile = p.dim <= 64 && entry_rows * p.rows_per_prefix > 16 ? 32 : 16;
+    // Rows of the entries that share a prefix are taken together over it where that makes fewer tiles of rows; a part that
+    // is of another type has to be a pass of its own.
+    const uint64_t together = ceil_div(entry_rows * p.rows_per_prefix, plan.row_tile);
+    const uint64_t apart = p.rows_per_prefix * ceil_div(entry_rows, plan.row_tile);
+    const bool two_types = with_prefix && with_own && d.prefix.dtype != d.own.dtype;
+    const bool fold = with_prefix && (together < apart || two_types);
+    const auto add_pass = [&](uint32_t members, bool prefix, bool own) {
+        AttentionPass& pass = p.pass[p.pass_count];
+        plan.format[p.pass_count++] = static_cast<KvFormat>(prefix ? d.prefix.dtype : d.own.dtype);
+        pass.members = members;
+        pass.groups = p.batch / members;
+        pass.rows = static_cast<uint32_t>(members * entry_rows);
+        pass.row_tiles = static_cast<uint32_t>(ceil_div(pass.rows, plan.row_tile));
+        pass.with_prefix = prefix ? 1u : 0u;
+        pass.with_own = own ? 1u : 0u;
+    };
+    if (fold) {
+        add_pass(p.rows_per_prefix, true, false);
+        if (with_own) add_pass(1, false, true);
+    } else {
+        add_pass(1, with_prefix, with_own);
+    }
+    // Each pass's keys are split so that the items of the launch come to about three blocks per SM of like size, none
+    // of less than 16 groups of keys.
+    uint64_t groups_of_keys[2] = {}, items[2] = {}, work = 0;
+    for (uint32_t i = 0; i < p.pass_count; ++i) {
+        AttentionPass& pass = p.pass[i];
+        const uint32_t keys = plan.format[i] == KV_F16 ? 16 : 32;
+        groups_of_keys[i] = (pass.with_prefix ? ceil_div(p.prefix.capacity, keys) : 0) + (pass.with_own ? ceil_div(p.own.capacity, keys) : 0);
+        items[i] = static_cast<uint64_t>(pass.row_tiles) * p.kv_heads * pass.groups;
+        work += items[i] * groups_of_keys[i];
+    }
+    const uint64_t share = std::max<uint64_t>(16, ceil_div(work, 3ull * sm_count));
+    p.slots = 0;
+    for (uint32_t i = 0; i < p.pass_count; ++i) {
+        AttentionPass& pass = p.pass[i];
+        pass.splits = static_cast<uint32_t>(std::clamp<uint64_t>(ceil_div(groups_of_keys[i], share), 1, 256));
+        pass.first_slot = p.slots;
+        p.slots += pass.splits;
+        if (items[i] * pass.splits > kMaxExtent / 2) return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: dimensions too large");
+        pass.items = static_cast<uint32_t>(items[i] * pass.splits);
+    }
+    if (p.slots > 1) {
+        plan.scratch_bytes = static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * (p.dim + 1) * sizeof(float);
+    }
+    return SDXLQ_OK;
+}
+
+int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
+    if (desc == nullptr) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: null descriptor");
+    const sdxlq_attention_desc& d = *desc;
+    if (d.batch == 0 || d.q_tokens == 0) return SDXLQ_OK;
+    AttentionPlan plan;
+    int status = plan_attention(ctx, ctx->sm_count, d, plan);
+    if (status != SDXLQ_OK) return status;
+    AttentionParams& p = plan.params;
+    if (p.slots > 1) {
+        void* const scratch = d.scratch != nullptr ? d.scratch : ctx->workspace;
+        const uint64_t room = d.scratch != nullptr ? d.scratch_bytes : ctx->workspace_bytes;
+        if (plan.scratch_bytes > room || !aligned16(scratch)) {
+            return fail(ctx, SDXLQ_ERR_WORKSPACE, "attention: needs " + std::to_string(plan.scratch_bytes) + " bytes of 16-byte aligned scratch");
+        }
+        p.part_o = static_cast<float*>(scratch);
+        p.part_lse = p.part_o + static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * p.dim;
+    }
+    const DeviceScope device(ctx);
+    const bool one_launch = p.pass_count == 1 || plan.format[0] == plan.format[1];
+    LaunchTimer timer(ctx, SDXLQ_KERNEL_HARNESS, (one_launch ? 1 : 2) + (p.slots > 1 ? 1 : 0));
+    cudaError_t error = cudaSuccess;
+    if (one_launch) {
+        error = launch_attention_rows(p, plan.format[0], plan.row_tile, ctx->stream, early(ctx));
+    } else {
+        for (uint32_t i = 0; i < 2 && error == cudaSuccess; ++i) {
+            AttentionParams one = p;
+            one.pass_count = 1;
+            one.pass[0] = p.pass[i];
+            error = launch_attention_rows(one, plan.format[i], plan.row_tile, ctx->stream, early(ctx));
+        }
+    }
+    if (error == cudaSuccess && p.slots > 1) error = launch_attention_join(p, ctx->stream, early(ctx));
+    if (error != cudaSuccess) return fail_cuda(ctx, error, "attention launch");
+    return SDXLQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sdxlq_kv_cache_write(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens) {
+    if (ctx == nullptr) return SDXLQ_ERR_INVALID_ARGUMENT;
+    try {
+        return copy_tokens(ctx, cache, tokens, true);
+    } catch (...) {
+        return SDXLQ_ERR_CUDA;
+    }
+}
+
+int sdxlq_kv_cache_read(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens) {
+    if (ctx == nullptr) return SDXLQ_ERR_INVALID_ARGUMENT;
+    try {
+        return copy_tokens(ctx, cache, tokens, false);
+    } catch (...) {
+        return SDXLQ_ERR_CUDA;
+    }
+}
+
+int sdxlq_shared_prefix_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
+    if (ctx == nullptr) return SDXLQ_ERR_INVALID_ARGUMENT;
+    try {
+        return run_attention(ctx, desc);
+    } catch (...) {
+        return SDXLQ_ERR_CUDA;
+    }
+}
+
+size_t sdxlq_shared_prefix_attention_scratch(const sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
+    if (ctx == nullptr || desc == nullptr || desc->batch == 0 || desc->q_tokens == 0) return 0;
+    try {
+        AttentionPlan plan;
+        return plan_attention(nullptr, ctx->sm_count, *desc, plan) == SDXLQ_OK ? static_cast<size_t>(plan.scratch_bytes) : 0;
+    } catch (...) {
+        return 0;
+    }
+}
+
+}
