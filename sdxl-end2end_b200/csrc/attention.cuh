@@ -73,11 +73,12 @@ struct AttentionParams {
     float* part_o;               // [slots, batch * q_tokens * q_heads, dim] shares, each divided by its own sum; null: no join
     float* part_lse;             // [slots, batch * q_tokens * q_heads] log2 of the sum of 2^score, -inf for an empty share
     uint32_t slots;
-    uint32_t y_vector;           // rows of y are 16-byte aligned
 };
 
 cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
                                   bool early_launch);
+cudaError_t launch_attention_tiles(const AttentionParams& params, KvFormat format, uint32_t* error_word, long long wait_limit_cycles,
+                                   cudaStream_t stream, bool early_launch);
 cudaError_t launch_attention_join(const AttentionParams& params, cudaStream_t stream, bool early_launch);
 
 // Where query row r of a pass's group lies.

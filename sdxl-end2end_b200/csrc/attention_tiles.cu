@@ -1,0 +1,657 @@
+// Attention of many query rows per key head (image tokens, long questions): tiles of 128 rows on the tensor memory. See
+// attention.cuh for rows, passes and items, attention_rows.cu for few rows.
+//
+// A CTA takes 128 rows over its share of the keys, in tiles of 128 keys (heads of up to 64) or 64 (up to 128):
+//   loader warps   K and V tiles into a ring of four slots, as SWIZZLE_128B operands: FP16 by cp.async, which fills what
+//                  lies behind a length or behind the head's size with zeros; 8-bit caches through registers, widened to
+//                  exact halves without their scales
+//   MMA warp       S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V as it lies, MN-major)
+//   softmax warps  a thread per row: S from tensor memory, the weights back into it as halves
+// S, P and O share 256 columns, so that two CTAs work on an SM and the one's MMAs run under the other's exponentials.
+//
+// With M the row's running reference, a weight is 2^(s_j log2 e - M); M is the running maximum minus 6, and only moves when a
+// tile's maximum passes it by more than 2^7: then O, in tensor memory, and the sum are multiplied by 2^(M_old - M). Weights
+// of an 8-bit cache are multiplied by their value's scale, and M contains the logarithm of the tile's largest value scale,
+// so that they stay within the halves; O / l is the same for any M.
+//
+// What bounds it: for heads of 64 the exponentials, 1024 clocks of the SM's 16 lanes a clock for a tile of 128 x 128, whose
+// MMAs take 512; for short keys the bytes of Q and of the output.
+
+#include "attention.cuh"
+#include "internal.cuh"
+#include "ptx.cuh"
+
+#include <type_traits>
+
+namespace sdxlq {
+
+namespace {
+
+constexpr uint32_t kTileRows = 128;
+constexpr uint32_t kSlots = 4;                   // K0 V0 K1 V1
+constexpr uint32_t kScaleRing = 4;               // key tiles whose scales are held
+constexpr uint32_t kSoftmaxWarps = 4;
+constexpr uint32_t kColumns = 256;
+constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
+
+// Tensor-memory columns of a CTA: S [0, keys), P [keys, keys + keys / 2), O behind it.
+template <int kDim>
+struct Shape {
+    static constexpr uint32_t kKeys = kDim == 64 ? 128 : 64;
+    static constexpr uint32_t kColumnS = 0;
+    static constexpr uint32_t kColumnP = kKeys;
+    static constexpr uint32_t kColumnO = kDim == 64 ? 192 : 128;
+    static constexpr uint32_t kTileBytes = kKeys * kDim * 2;         // 16 KB
+    static constexpr uint32_t kQueryBytes = kTileRows * kDim * 2;
+};
+
+struct TileControl {
+    uint64_t query_ready, score_ready, score_free, weight_ready, value_done, vote, drained;
+    uint64_t full[kSlots], empty[kSlots], scales_full[kScaleRing];
+    uint32_t tmem_base;
+    uint32_t abort;
+    uint32_t skip[2];                            // of even and odd tiles: the softmax warps add the tile's values themselves
+};
+
+struct TileParams {
+    AttentionParams a;
+    uint32_t* error_word;
+    long long wait_limit_cycles;
+};
+
+// Byte of 16-byte chunk `chunk` of row `row` in a tile of `rows` rows of 128-byte swizzle spans.
+__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk, uint32_t rows) {
+    return (chunk >> 3) * rows * 128u + row * 128u + (((chunk & 7u) ^ (row & 7u)) << 4);
+}
+
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ bool half_not_finite(uint32_t pair) {
+    return (pair & 0x7C00u) == 0x7C00u || (pair & 0x7C000000u) == 0x7C000000u;
+}
+
+// The item's place and the tiles of keys that it walks over.
+template <int kDim>
+struct Item {
+    uint32_t kv_head, first_member, first_row, rows, split, slot;
+    uint32_t prefix_slot, prefix_length, own_length, own_seen;       // own_seen: keys that any row of the tile sees
+    uint32_t least_limit;                                            // own keys that all its rows see
+    uint32_t prefix_tiles, tile_begin, tile_end;
+
+    __device__ __forceinline__ explicit Item(const AttentionParams& p) {
+        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
+        const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
+        const AttentionPass& pass = p.pass[second ? 1 : 0];
+        uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
+        const uint32_t row_tile = item % pass.row_tiles;
+        item /= pass.row_tiles;
+        split = item % pass.splits;
+        item /= pass.splits;
+        kv_head = item % p.kv_heads;
+        first_member = item / p.kv_heads * pass.members;
+        first_row = row_tile * kTileRows;
+        rows = min(kTileRows, pass.rows - first_row);
+        slot = pass.first_slot + split;
+        prefix_slot = pass.with_prefix ? first_member / p.rows_per_prefix : 0u;
+        prefix_length = pass.with_prefix ? length_of(p.prefix, prefix_slot) : 0u;
+        own_length = own_seen = least_limit = pass.with_own ? length_of(p.own, first_member) : 0u;
+        if (p.causal && pass.with_own) {
+            own_seen = causal_limit(own_length, p.q_tokens, (first_row + rows - 1) / p.repeat);
+            least_limit = causal_limit(own_length, p.q_tokens, first_row / p.repeat);
+        }
+        prefix_tiles = (prefix_length + kKeys - 1) / kKeys;
+        const uint64_t tiles = static_cast<uint64_t>(prefix_tiles) + (own_seen + kKeys - 1) / kKeys;
+        tile_begin = static_cast<uint32_t>(tiles * split / pass.splits);
+        tile_end = static_cast<uint32_t>(tiles * (split + 1) / pass.splits);
+    }
+
+    struct Tile {
+        bool in_prefix;
+        uint32_t first, end;         // first key of the tile, end of the part's keys
+        uint32_t columns;            // keys of the tile, rounded up to the MMA's 16
+    };
+    __device__ __forceinline__ Tile tile(uint32_t index) const {
+        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
+        Tile t;
+        t.in_prefix = index < prefix_tiles;
+        t.first = (t.in_prefix ? index : index - prefix_tiles) * kKeys;
+        t.end = t.in_prefix ? prefix_length : own_seen;
+        t.columns = min(kKeys, (t.end - t.first + 15u) & ~15u);
+        return t;
+    }
+};
+
+template <int kDim, int kFormat, int kLoaderWarps>
+__global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) attention_tiles_kernel(const __grid_constant__ TileParams params) {
+    using S = Shape<kDim>;
+    constexpr uint32_t kKeys = S::kKeys;
+    constexpr bool kScaled = kFormat != KV_F16;
+    const AttentionParams& p = params.a;
+    extern __shared__ __align__(1024) uint8_t dynamic_smem[];
+    __shared__ TileControl control;
+    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][2][kScaled ? kKeys : 1];       // key scales * softmax scale, value scales
+    const uint32_t query_base = ptx::smem_u32(dynamic_smem), slots_base = query_base + S::kQueryBytes;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    volatile uint32_t* const abort_word = &control.abort;
+    const long long limit = params.wait_limit_cycles;
+
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
+        ptx::mbar_init(ptx::smem_u32(&control.score_ready), 1);
+        ptx::mbar_init(ptx::smem_u32(&control.score_free), kSoftmaxWarps);
+        ptx::mbar_init(ptx::smem_u32(&control.weight_ready), kSoftmaxWarps);
+        ptx::mbar_init(ptx::smem_u32(&control.value_done), 1);
+        ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
+        ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
+        for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kLoaderWarps);
+        for (uint32_t s = 0; s < kSlots; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&control.full[s]), kLoaderWarps);
+            ptx::mbar_init(ptx::smem_u32(&control.empty[s]), 1);
+        }
+        control.abort = 0;
+        control.skip[0] = control.skip[1] = 0;
+        ptx::fence_mbar_init();
+    }
+    if (warp == kSoftmaxWarps) {
+        ptx::tmem_alloc(ptx::smem_u32(&control.tmem_base), kColumns);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&control.tmem_base);
+    wait_for_prior_kernels_then_release_next();
+
+    const Item<kDim> item(p);
+    const uint32_t tiles = item.tile_end - item.tile_begin;
+    const auto give_up = [&](uint32_t code) {
+        *abort_word = 1;
+        atomicCAS(params.error_word, 0u, code);
+    };
+
+    if (warp > kSoftmaxWarps) {
+        // ---------------------------------------- loaders ----------------------------------------
+        const uint32_t thread = threadIdx.x - 32u * (kSoftmaxWarps + 1);
+        constexpr uint32_t kThreads = 32u * kLoaderWarps;
+        const uint32_t full = ptx::smem_u32(&control.full[0]), empty = ptx::smem_u32(&control.empty[0]);
+        const auto slot_free = [&](uint32_t unit) {
+            return ptx::warp_wait_bounded(empty + (unit % kSlots) * 8u, ((unit / kSlots) & 1u) ^ 1u, abort_word, limit);
+        };
+        const auto announce = [&](uint32_t unit) {
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(full + (unit % kSlots) * 8u);
+        };
+        const auto source = [&](uint32_t unit, typename Item<kDim>::Tile& t) -> const uint8_t* {
+            t = item.tile(item.tile_begin + unit / 2);
+            const KvView& view = t.in_prefix ? p.prefix : p.own;
+            const int64_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
+            return (unit % 2 == 0 ? view.k : view.v) + slot * view.slot_stride + item.kv_head * view.head_stride +
+                   static_cast<int64_t>(t.first) * view.token_stride;
+        };
+        if constexpr (!kScaled) {
+            constexpr uint32_t kChunks = kDim / 8;                       // of a key
+            constexpr uint32_t kStep = kThreads / kChunks;               // keys per round
+            static_assert(kKeys % kStep == 0);
+            const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
+            const bool in_head = chunk * 8u < p.dim;
+            uint32_t announced = 0;
+            bool ok = true;
+            for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
+                // a slot that is not free yet is not waited for before what has been loaded is passed on
+                const uint32_t bar = empty + (unit % kSlots) * 8u, parity = ((unit / kSlots) & 1u) ^ 1u;
+                if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) {
+                    ptx::cp_async_wait<0>();
+                    for (; announced < unit; ++announced) announce(announced);
+                    if (!slot_free(unit)) { ok = false; break; }
+                }
+                typename Item<kDim>::Tile t;
+                const uint8_t* const base = source(unit, t);
+                const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
+                const uint8_t* from = base + first_key * stride + chunk * 16u;
+                const uint32_t to = slots_base + (unit % kSlots) * S::kTileBytes;
+                for (uint32_t key = first_key; key < t.columns; key += kStep, from += kStep * stride) {
+                    const bool inside = in_head && t.first + key < t.end;
+                    ptx::cp_async16(to + swizzled(key, chunk, kKeys), inside ? from : base, inside);
+                }
+                ptx::cp_async_commit();
+                if (announced < unit) {
+                    ptx::cp_async_wait<1>();
+                    for (; announced < unit; ++announced) announce(announced);
+                }
+            }
+            ptx::cp_async_wait<0>();
+            if (ok) {
+                for (; announced < 2 * tiles; ++announced) announce(announced);
+            } else {
+                give_up(DEV_TIMEOUT_PRODUCER);
+            }
+        } else {
+            constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
+            constexpr uint32_t kStep = kThreads / kChunks;
+            constexpr uint32_t kRounds = kKeys / kStep;
+            static_assert(kStep % 8 == 0 && kKeys % kStep == 0);
+            const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
+            const bool in_head = chunk * 16u < p.dim;
+            const uint32_t target0 = swizzled(first_key, 2u * chunk, kKeys), target1 = swizzled(first_key, 2u * chunk + 1u, kKeys);
+            uint4 ahead[kRounds];
+            float ahead_scale[2] = {0.0f, 0.0f};
+            const auto fetch = [&](uint32_t unit) {
+                typename Item<kDim>::Tile t;
+                const uint8_t* const base = source(unit, t);
+                const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
+                const uint8_t* from = base + first_key * stride + chunk * 16u;
+#pragma unroll
+                for (uint32_t i = 0; i < kRounds; ++i, from += kStep * stride) {
+                    const bool inside = in_head && t.first + first_key + i * kStep < t.end;
+                    ahead[i] = inside ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                if (unit % 2 == 0 && thread < kKeys) {
+                    const KvView& view = t.in_prefix ? p.prefix : p.own;
+                    const int64_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
+                    const int64_t at = (slot * p.kv_heads + item.kv_head) * view.capacity + t.first + thread;
+                    const bool inside = t.first + thread < t.end;
+                    ahead_scale[0] = inside ? __ldg(view.k_scales + at) * fabsf(p.scale_log2) : 0.0f;
+                    ahead_scale[1] = inside ? __ldg(view.v_scales + at) : 0.0f;
+                }
+            };
+            static_assert(kThreads >= kKeys);
+            if (tiles != 0) fetch(0);
+            for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
+                if (!slot_free(unit)) {
+                    give_up(DEV_TIMEOUT_PRODUCER);
+                    break;
+                }
+                uint32_t to = slots_base + (unit % kSlots) * S::kTileBytes;
+#pragma unroll
+                for (uint32_t i = 0; i < kRounds; ++i, to += kStep * 128u) {
+                    const uint2 a = widen4<kFormat>(ahead[i].x), b = widen4<kFormat>(ahead[i].y), c = widen4<kFormat>(ahead[i].z),
+                                d = widen4<kFormat>(ahead[i].w);
+                    ptx::st_shared16(to + target0, make_uint4(a.x, a.y, b.x, b.y));
+                    ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
+                }
+                // The ring of scales is written this far ahead of its readers: the slot of this tile's K was freed by the
+                // MMA of the tile two before it, which waited for the softmax warps to have read the scores, and with
+                // them the scales, of the tile before that one.
+                if (unit % 2 == 0 && thread < kKeys) {
+                    scales[unit / 2 % kScaleRing][0][thread] = ahead_scale[0];
+                    scales[unit / 2 % kScaleRing][1][thread] = ahead_scale[1];
+                }
+                if (unit % 2 == 0) {
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&control.scales_full[unit / 2 % kScaleRing]));
+                }
+                if (unit + 1 < 2 * tiles) fetch(unit + 1);
+                announce(unit);
+            }
+        }
+    } else if (warp == kSoftmaxWarps) {
+        // ---------------------------------------- MMA issuer ----------------------------------------
+        const uint32_t full = ptx::smem_u32(&control.full[0]), empty = ptx::smem_u32(&control.empty[0]);
+        const auto wait = [&](const uint64_t& bar, uint32_t parity) {
+            return ptx::warp_wait_bounded(ptx::smem_u32(&bar), parity, abort_word, limit);
+        };
+        const auto wait_full = [&](uint32_t unit) {
+            return ptx::warp_wait_bounded(full + (unit % kSlots) * 8u, (unit / kSlots) & 1u, abort_word, limit);
+        };
+        const auto multiply_scores = [&](uint32_t index) {
+            const uint32_t unit = 2 * index, columns = item.tile(item.tile_begin + index).columns;
+            const uint32_t idesc = ptx::umma_instr_desc(1, 0, 0, kTileRows, columns);
+            if (ptx::elect_one()) {
+                const uint32_t a = ptx::umma_desc_lo(query_base), b = ptx::umma_desc_lo(slots_base + (unit % kSlots) * S::kTileBytes);
+#pragma unroll
+                for (uint32_t step = 0; step < kDim / 16; ++step) {
+                    const uint32_t within = step % 4 * 2;                // 32 bytes of a swizzle span
+                    ptx::umma_f16_ss(tmem + S::kColumnS, a + step / 4 * (kTileRows * 128 / 16) + within, ptx::kUmmaDescHiSw128,
+                                     b + step / 4 * (kKeys * 128 / 16) + within, ptx::kUmmaDescHiSw128, idesc, step != 0);
+                }
+                ptx::umma_commit(empty + (unit % kSlots) * 8u);
+                ptx::umma_commit(ptx::smem_u32(&control.score_ready));
+            }
+            __syncwarp();
+        };
+        bool ok = true;
+        if (tiles != 0) {
+            ok = wait(control.query_ready, 0) && wait_full(0);
+            ptx::tc_fence_after();
+            if (ok) multiply_scores(0);
+        }
+        for (uint32_t j = 0; ok && j < tiles; ++j) {
+            if (j + 1 < tiles) {
+                ok = wait(control.score_free, j & 1u) && wait_full(2 * (j + 1));
+                if (!ok) break;
+                ptx::tc_fence_after();
+                multiply_scores(j + 1);
+            }
+            const uint32_t unit = 2 * j + 1;
+            ok = wait(control.weight_ready, j & 1u) && wait_full(unit);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t columns = item.tile(item.tile_begin + j).columns;
+            // V is the B operand with its head dimension together (MN-major: bit 16); 64 of it to an MMA
+            constexpr uint32_t idesc = ptx::umma_instr_desc(1, 0, 0, kTileRows, 64) | (1u << 16);
+            const bool skip = *reinterpret_cast<volatile uint32_t*>(&control.skip[j & 1u]) != 0;
+            if (ptx::elect_one()) {
+                if (!skip) {
+                    const uint32_t b = ptx::umma_desc_lo(slots_base + (unit % kSlots) * S::kTileBytes);
+                    for (uint32_t step = 0; step < columns / 16; ++step) {
+#pragma unroll
+                        for (uint32_t part = 0; part < kDim / 64; ++part) {
+                            ptx::umma_f16_ts(tmem + S::kColumnO + part * 64, tmem + S::kColumnP + step * 8,
+                                             b + part * (kKeys * 128 / 16) + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, idesc,
+                                             (j | step) != 0);
+                        }
+                    }
+                }
+                ptx::umma_commit(empty + (unit % kSlots) * 8u);
+                ptx::umma_commit(ptx::smem_u32(&control.value_done));
+            }
+            __syncwarp();
+        }
+        if (!ok) {
+            give_up(DEV_TIMEOUT_MMA);
+            if (ptx::elect_one()) ptx::umma_commit(ptx::smem_u32(&control.drained));         // what was issued ends before its memory goes
+            __syncwarp();
+            uint32_t never = 0;
+            ptx::mbar_wait_bounded(ptx::smem_u32(&control.drained), 0, &never, limit);
+        }
+    } else {
+        // ---------------------------------------- softmax ----------------------------------------
+        const uint32_t row = threadIdx.x;                                // of the tile, and lane of tensor memory
+        const uint32_t my_tmem = tmem + ((warp * 32u) << 16);
+        const bool warp_active = warp * 32u < item.rows;
+        const auto wait = [&](const uint64_t& bar, uint32_t parity) {
+            return ptx::warp_wait_bounded(ptx::smem_u32(&bar), parity, abort_word, limit);
+        };
+        const auto arrive = [&](uint64_t& bar) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bar));
+        };
+        {
+            // Q: a negative softmax scale turns the queries' signs, so that scores are multiplied by its magnitude
+            const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+            constexpr uint32_t kChunks = kDim / 8;
+            for (uint32_t i = threadIdx.x; i < kTileRows * kChunks; i += 32 * kSoftmaxWarps) {
+                const uint32_t r = i / kChunks, chunk = i % kChunks;
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (r < item.rows && chunk * 8u < p.dim) {
+                    const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + r);
+                    x = __ldg(reinterpret_cast<const uint4*>(p.q + at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head + chunk * 8u));
+                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                }
+                ptx::st_shared16(query_base + swizzled(r, chunk, kTileRows), x);
+            }
+            ptx::fence_proxy_async();
+            arrive(control.query_ready);
+        }
+        const float scale = fabsf(p.scale_log2);
+        const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + min(row, item.rows - 1));
+        const uint32_t own_limit = p.causal ? causal_limit(item.own_length, p.q_tokens, at.token) : item.own_length;
+        const float kNone = __int_as_float(0xff800000);
+        float reference = kNone, sum = 0.0f;
+        uint32_t votes = 0;
+        bool ok = true;
+        for (uint32_t j = 0; j < tiles; ++j) {
+            const typename Item<kDim>::Tile t = item.tile(item.tile_begin + j);
+            const uint32_t seen_by_all = t.in_prefix ? item.prefix_length : item.least_limit;
+            const bool masked = t.first + kKeys > seen_by_all;
+            const bool ragged = p.causal && !t.in_prefix && masked;      // rows differ in what they see of the tile
+            const uint32_t seen = t.in_prefix ? item.prefix_length : own_limit;
+            const uint32_t visible = seen > t.first ? min(seen - t.first, kKeys) : 0u;       // columns that this row sees
+            const float* const key_scales = scales[j % kScaleRing][0];
+            const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
+            if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
+            ok = ok && wait(control.score_ready, j & 1u);
+            if (!ok) break;
+            ptx::tc_fence_after();
+
+            const uint32_t chunks = (t.columns + 31u) / 32u;
+            float grow = 1.0f;
+            if (warp_active) {
+                float largest = kNone;
+                for (uint32_t c = 0; c < chunks; ++c) {
+                    uint32_t s[32];
+                    ptx::tmem_ld_32x32b_x32(my_tmem + S::kColumnS + c * 32u, s);
+                    ptx::tmem_ld_wait(s);
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float x = __uint_as_float(s[i]);
+                            if constexpr (kScaled) x *= key_scales[c * 32u + i];
+                            if (c * 32u + i < visible) largest = fmaxf(largest, x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(s[i + e]);
+                            if constexpr (kScaled) {
+                                const float4 k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
+                                x[0] *= k.x; x[1] *= k.y; x[2] *= k.z; x[3] *= k.w;
+                            }
+                            largest = fmaxf(largest, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+                        }
+                    }
+                }
+                float wanted = (kScaled ? largest : largest * scale) - kWeightBits;
+                if constexpr (kScaled) {
+                    float top = 1e-20f;
+#pragma unroll
+                    for (uint32_t i = 0; i < kKeys; i += 32) top = fmaxf(top, value_scales[i + lane]);
+#pragma unroll
+                    for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+                    wanted += log2_approx(top);
+                }
+                if (wanted > reference + kSlackBits) {
+                    grow = exp2_approx(reference - wanted);
+                    reference = wanted;
+                    sum *= grow;
+                }
+            }
+            if (j != 0) {
+                ok = wait(control.value_done, (j - 1) & 1u);             // O is whole, P is free
+                if (!ok) break;
+                ptx::tc_fence_after();
+                if (warp_active && __any_sync(0xffffffffu, grow != 1.0f)) {
+#pragma unroll
+                    for (uint32_t c = 0; c < kDim; c += 16) {
+                        uint32_t o[16];
+                        ptx::tmem_ld_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                        ptx::tmem_ld_wait(o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * grow);
+                        ptx::tmem_st_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                    }
+                }
+            }
+            if (warp_active) {
+                const float shift = reference > kNone ? reference : 0.0f;
+                float part[2] = {0.0f, 0.0f};
+                for (uint32_t c = 0; c < chunks; ++c) {
+                    uint32_t s[32], w[16];
+                    ptx::tmem_ld_32x32b_x32(my_tmem + S::kColumnS + c * 32u, s);
+                    ptx::tmem_ld_wait(s);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float x[4];
+                        float4 k = make_float4(scale, scale, scale, scale), v = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                        if constexpr (kScaled) {
+                            k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
+                            v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
+                        }
+                        x[0] = fmaf(__uint_as_float(s[i]), k.x, -shift);
+                        x[1] = fmaf(__uint_as_float(s[i + 1]), k.y, -shift);
+                        x[2] = fmaf(__uint_as_float(s[i + 2]), k.z, -shift);
+                        x[3] = fmaf(__uint_as_float(s[i + 3]), k.w, -shift);
+                        if (masked) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e]);
+                        part[0] += x[0] + x[1];
+                        part[1] += x[2] + x[3];
+                        if constexpr (kScaled) {
+                            x[0] *= v.x; x[1] *= v.y; x[2] *= v.z; x[3] *= v.w;
+                            if (masked) {                                // a hidden key's scale may be anything
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : 0.0f;
+                            }
+                        }
+                        w[i / 2] = pack_half2(x[0], x[1]);
+                        w[i / 2 + 1] = pack_half2(x[2], x[3]);
+                    }
+                    ptx::tmem_st_32x32b_x16(my_tmem + S::kColumnP + c * 16u, w);
+                }
+                sum += part[0] + part[1];
+            }
+            arrive(control.score_free);
+            ptx::tmem_st_wait();
+
+            // A value that is not finite makes 0 * v a NaN, also in rows that the causal mask hides it from (what lies behind
+            // a length was loaded as zeros). Tiles that such a mask divides are looked through, and one that holds such a value
+            // is multiplied here, row by row over the keys that the row sees.
+            if (kFormat != KV_INT8 && p.causal && threadIdx.x == 0) control.skip[(j + 1) & 1u] = 0;
+            if (kFormat != KV_INT8 && ragged) {
+                const uint32_t unit = 2 * j + 1, base = slots_base + (unit % kSlots) * S::kTileBytes;
+                volatile uint32_t* const skip = &control.skip[j & 1u];
+                ok = wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
+                if (!ok) break;
+                bool found = false;
+                for (uint32_t i = threadIdx.x; i < t.columns * (kDim / 8); i += 32 * kSoftmaxWarps) {
+                    const uint4 x = ptx::ld_shared16(base + swizzled(i / (kDim / 8), i % (kDim / 8), kKeys));
+                    found = found || half_not_finite(x.x) || half_not_finite(x.y) || half_not_finite(x.z) || half_not_finite(x.w);
+                }
+                if (found) *skip = 1;
+                arrive(control.vote);
+                ok = wait(control.vote, votes & 1u);
+                if (!ok) break;
+                ++votes;
+                if (*skip != 0 && warp_active) {
+                    for (uint32_t c = 0; c < kDim; c += 8) {
+                        uint32_t o[8];
+                        ptx::tmem_ld_32x32b_x8(my_tmem + S::kColumnO + c, o);
+                        ptx::tmem_ld_wait(o);
+                        float total[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) total[i] = j == 0 ? 0.0f : __uint_as_float(o[i]);
+                        for (uint32_t key = 0; key < t.columns; ++key) {
+                            uint32_t pair;
+                            ptx::tmem_ld_32x32b_x1(my_tmem + S::kColumnP + key / 2, pair);
+                            ptx::tmem_ld_wait(pair);
+                            const float w = key % 2 == 0 ? half_lo(pair) : half_hi(pair);
+                            const uint4 x = ptx::ld_shared16(base + swizzled(key, c / 8, kKeys));
+                            if (key < visible) {
+                                total[0] = fmaf(w, half_lo(x.x), total[0]); total[1] = fmaf(w, half_hi(x.x), total[1]);
+                                total[2] = fmaf(w, half_lo(x.y), total[2]); total[3] = fmaf(w, half_hi(x.y), total[3]);
+                                total[4] = fmaf(w, half_lo(x.z), total[4]); total[5] = fmaf(w, half_hi(x.z), total[5]);
+                                total[6] = fmaf(w, half_lo(x.w), total[6]); total[7] = fmaf(w, half_hi(x.w), total[7]);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(total[i]);
+                        ptx::tmem_st_32x32b_x8(my_tmem + S::kColumnO + c, o);
+                    }
+                    ptx::tmem_st_wait();
+                }
+            }
+            arrive(control.weight_ready);
+        }
+        // from here on the room of Q is free: the last product has read it, or (no keys) all warps have written theirs
+        if (ok) ok = tiles != 0 ? wait(control.value_done, (tiles - 1) & 1u) : wait(control.query_ready, 0);
+        ptx::tc_fence_after();
+        if (!ok) {
+            give_up(DEV_TIMEOUT_EPILOGUE);
+        } else if (warp_active) {
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const bool empty = tiles == 0;                               // O was never written
+            if (p.part_o == nullptr) {
+                // the warp's rows of Q make room for its rows of the output, which leave in whole lines
+#pragma unroll
+                for (uint32_t c = 0; c < kDim; c += 16) {
+                    uint32_t o[16];
+                    ptx::tmem_ld_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                    ptx::tmem_ld_wait(o);
+                    float x[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = empty || sum == 0.0f ? 0.0f : __uint_as_float(o[i]) * inverse;
+                    ptx::st_shared16(query_base + swizzled(row, c / 8, kTileRows),
+                                     make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7])));
+                    ptx::st_shared16(query_base + swizzled(row, c / 8 + 1, kTileRows),
+                                     make_uint4(pack_half2(x[8], x[9]), pack_half2(x[10], x[11]), pack_half2(x[12], x[13]), pack_half2(x[14], x[15])));
+                }
+                __syncwarp();
+                constexpr uint32_t kChunks = kDim / 8;
+                for (uint32_t i = lane; i < 32 * kChunks; i += 32) {
+                    const uint32_t r = warp * 32u + i / kChunks, chunk = i % kChunks;
+                    if (r >= item.rows || chunk * 8u >= p.dim) continue;
+                    const QueryRow to = locate_row(p, item.first_member, item.kv_head, item.first_row + r);
+                    *reinterpret_cast<uint4*>(p.y + to.batch * p.y_batch + to.token * p.y_token + to.head * p.y_head + chunk * 8u) =
+                        ptx::ld_shared16(query_base + swizzled(r, chunk, kTileRows));
+                }
+            } else {
+                const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
+                const uint64_t place = item.slot * rows + (static_cast<uint64_t>(at.batch) * p.q_tokens + at.token) * p.q_heads + at.head;
+#pragma unroll
+                for (uint32_t c = 0; c < kDim; c += 16) {
+                    uint32_t o[16];
+                    ptx::tmem_ld_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                    ptx::tmem_ld_wait(o);
+                    float4* const out = reinterpret_cast<float4*>(p.part_o + place * p.dim + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (row < item.rows && c + 4u * i < p.dim) {
+                            out[i] = empty || sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                          : make_float4(__uint_as_float(o[4 * i]) * inverse, __uint_as_float(o[4 * i + 1]) * inverse,
+                                                                        __uint_as_float(o[4 * i + 2]) * inverse, __uint_as_float(o[4 * i + 3]) * inverse);
+                        }
+                    }
+                }
+                if (row < item.rows) p.part_lse[place] = sum == 0.0f ? kNone : (reference > kNone ? reference : 0.0f) + log2f(sum);
+            }
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == kSoftmaxWarps) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, kColumns);
+    }
+}
+
+template <int kDim, int kFormat>
+cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 2 : 4;
+    constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
+    auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps>;
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (error != cudaSuccess) return error;
+    uint32_t blocks = 0;
+    for (uint32_t i = 0; i < params.a.pass_count; ++i) blocks += params.a.pass[i].items;
+    return launch_behind(kernel, blocks, 32 * (kSoftmaxWarps + 1 + kLoaderWarps), bytes, stream, early_launch, params);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_tiles(const AttentionParams& params, KvFormat format, uint32_t* error_word, long long wait_limit_cycles,
+                                   cudaStream_t stream, bool early_launch) {
+    const TileParams tile_params{params, error_word, wait_limit_cycles};
+    const auto run = [&](auto dim) {
+        constexpr int kDim = decltype(dim)::value;
+        switch (format) {
+        case KV_E4M3: return launch_tiles<kDim, KV_E4M3>(tile_params, stream, early_launch);
+        case KV_E5M2: return launch_tiles<kDim, KV_E5M2>(tile_params, stream, early_launch);
+        case KV_INT8: return launch_tiles<kDim, KV_INT8>(tile_params, stream, early_launch);
+        default: return launch_tiles<kDim, KV_F16>(tile_params, stream, early_launch);
+        }
+    };
+    return params.dim <= 64 ? run(std::integral_constant<int, 64>{}) : run(std::integral_constant<int, 128>{});
+}
+
+}  // namespace sdxlq

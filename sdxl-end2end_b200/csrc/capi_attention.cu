@@ -123,13 +123,22 @@ int copy_tokens(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_
     return SDXLQ_OK;
 }
 
-uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+uint64_t ceil_div(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
+
+// Rows of a tile of the kernel that takes passes of so many rows: attention_rows.cu's with 16 or (heads of up to 64) 32, or
+// attention_tiles.cu's with 128.
+constexpr uint32_t kTensorTile = 128;
+uint32_t row_tile_for(uint64_t rows, uint32_t dim) {
+    if (rows <= 16) return 16;
+    if (rows <= 32) return dim <= 64 ? 32 : 16;
+    return kTensorTile;
+}
 
 // A call's passes, and what its launches need.
 struct AttentionPlan {
     AttentionParams params{};
     KvFormat format[2] = {KV_F16, KV_F16};       // of each pass
-    uint32_t row_tile = 16;
+    uint32_t row_tile[2] = {};
     uint64_t scratch_bytes = 0;
 };
 
@@ -190,20 +199,25 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     if (d.batch == 0 || d.q_tokens == 0) return SDXLQ_OK;
 
     const uint64_t entry_rows = static_cast<uint64_t>(p.q_tokens) * p.repeat;
-    plan.row_tile = p.dim <= 64 && entry_rows * p.rows_per_prefix > 16 ? 32 : 16;
-    // Rows of the entries that share a prefix are taken together over it where that makes fewer tiles of rows; a part that
-    // is of another type has to be a pass of its own.
-    const uint64_t together = ceil_div(entry_rows * p.rows_per_prefix, plan.row_tile);
-    const uint64_t apart = p.rows_per_prefix * ceil_div(entry_rows, plan.row_tile);
-    const bool two_types = with_prefix && with_own && d.prefix.dtype != d.own.dtype;
-    const bool fold = with_prefix && (together < apart || two_types);
+    // Rows of the entries that share a prefix are taken together over it where that saves more than the join of the two
+    // parts costs, which is about the time of four tiles of 128 keys for every tile of rows; a part that is of another
+    // type has to be a pass of its own.
+    bool fold = false;
+    if (with_prefix) {
+        const uint64_t rows = entry_rows * p.rows_per_prefix;
+        const uint64_t together = ceil_div(rows, row_tile_for(rows, p.dim));
+        const uint64_t apart = p.rows_per_prefix * ceil_div(entry_rows, row_tile_for(entry_rows, p.dim));
+        fold = (with_own && d.prefix.dtype != d.own.dtype) ||
+               (together < apart && (!with_own || (apart - together) * ceil_div(p.prefix.capacity, 128) > 4 * apart));
+    }
     const auto add_pass = [&](uint32_t members, bool prefix, bool own) {
         AttentionPass& pass = p.pass[p.pass_count];
-        plan.format[p.pass_count++] = static_cast<KvFormat>(prefix ? d.prefix.dtype : d.own.dtype);
         pass.members = members;
         pass.groups = p.batch / members;
         pass.rows = static_cast<uint32_t>(members * entry_rows);
-        pass.row_tiles = static_cast<uint32_t>(ceil_div(pass.rows, plan.row_tile));
+        plan.format[p.pass_count] = static_cast<KvFormat>(prefix ? d.prefix.dtype : d.own.dtype);
+        plan.row_tile[p.pass_count] = row_tile_for(pass.rows, p.dim);
+        pass.row_tiles = static_cast<uint32_t>(ceil_div(pass.rows, plan.row_tile[p.pass_count++]));
         pass.with_prefix = prefix ? 1u : 0u;
         pass.with_own = own ? 1u : 0u;
     };
@@ -213,21 +227,21 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     } else {
         add_pass(1, with_prefix, with_own);
     }
-    // Each pass's keys are split so that the items of the launch come to about three blocks per SM of like size, none
-    // of less than 16 groups of keys.
-    uint64_t groups_of_keys[2] = {}, items[2] = {}, work = 0;
+    // Each pass's keys are split so that the items of all passes come to about three blocks per SM of like size (two on the
+    // tensor memory), none of less than 256 (512) keys.
+    uint64_t keys[2] = {}, items[2] = {}, work = 0;
     for (uint32_t i = 0; i < p.pass_count; ++i) {
         AttentionPass& pass = p.pass[i];
-        const uint32_t keys = plan.format[i] == KV_F16 ? 16 : 32;
-        groups_of_keys[i] = (pass.with_prefix ? ceil_div(p.prefix.capacity, keys) : 0) + (pass.with_own ? ceil_div(p.own.capacity, keys) : 0);
+        keys[i] = (pass.with_prefix ? p.prefix.capacity : 0ull) + (pass.with_own ? p.own.capacity : 0ull);
         items[i] = static_cast<uint64_t>(pass.row_tiles) * p.kv_heads * pass.groups;
-        work += items[i] * groups_of_keys[i];
+        work += items[i] * keys[i];
     }
-    const uint64_t share = std::max<uint64_t>(16, ceil_div(work, 3ull * sm_count));
     p.slots = 0;
     for (uint32_t i = 0; i < p.pass_count; ++i) {
         AttentionPass& pass = p.pass[i];
-        pass.splits = static_cast<uint32_t>(std::clamp<uint64_t>(ceil_div(groups_of_keys[i], share), 1, 256));
+        const bool tensor = plan.row_tile[i] == kTensorTile;
+        const uint64_t share = std::max<uint64_t>(tensor ? 512 : 256, ceil_div(work, (tensor ? 2ull : 3ull) * sm_count));
+        pass.splits = static_cast<uint32_t>(std::clamp<uint64_t>(keys[i] / share, 1, 256));
         pass.first_slot = p.slots;
         p.slots += pass.splits;
         if (items[i] * pass.splits > kMaxExtent / 2) return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: dimensions too large");
@@ -257,17 +271,23 @@ int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
         p.part_lse = p.part_o + static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * p.dim;
     }
     const DeviceScope device(ctx);
-    const bool one_launch = p.pass_count == 1 || plan.format[0] == plan.format[1];
+    const bool one_launch = p.pass_count == 1 || (plan.format[0] == plan.format[1] && plan.row_tile[0] == plan.row_tile[1]);
     LaunchTimer timer(ctx, SDXLQ_KERNEL_HARNESS, (one_launch ? 1 : 2) + (p.slots > 1 ? 1 : 0));
     cudaError_t error = cudaSuccess;
+    const auto launch = [&](const AttentionParams& params, uint32_t pass) {
+        if (error != cudaSuccess) return;
+        error = plan.row_tile[pass] == kTensorTile
+                    ? launch_attention_tiles(params, plan.format[pass], ctx->control, ctx->wait_limit_cycles, ctx->stream, early(ctx))
+                    : launch_attention_rows(params, plan.format[pass], plan.row_tile[pass], ctx->stream, early(ctx));
+    };
     if (one_launch) {
-        error = launch_attention_rows(p, plan.format[0], plan.row_tile, ctx->stream, early(ctx));
+        launch(p, 0);
     } else {
-        for (uint32_t i = 0; i < 2 && error == cudaSuccess; ++i) {
+        for (uint32_t i = 0; i < 2; ++i) {
             AttentionParams one = p;
             one.pass_count = 1;
             one.pass[0] = p.pass[i];
-            error = launch_attention_rows(one, plan.format[i], plan.row_tile, ctx->stream, early(ctx));
+            launch(one, i);
         }
     }
     if (error == cudaSuccess && p.slots > 1) error = launch_attention_join(p, ctx->stream, early(ctx));
