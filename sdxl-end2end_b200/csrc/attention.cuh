@@ -6,6 +6,7 @@
 #include "int8_math.cuh"
 #include "quantize.cuh"
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -71,14 +72,24 @@ struct AttentionParams {
     uint32_t pass_count;
     AttentionPass pass[2];
     float* part_o;               // [slots, batch * q_tokens * q_heads, dim] shares, each divided by its own sum; null: no join
-    float* part_lse;             // [slots, batch * q_tokens * q_heads] log2 of the sum of 2^score, -inf for an empty share
+    float2* part_lse;            // [slots, batch * q_tokens * q_heads] log2 of the sum of 2^score in two parts, which scores of
+                                 // any size leave exact; -inf in the first for an empty share
     uint32_t slots;
 };
 
 cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
                                   bool early_launch);
-cudaError_t launch_attention_tiles(const AttentionParams& params, KvFormat format, uint32_t* error_word, long long wait_limit_cycles,
-                                   cudaStream_t stream, bool early_launch);
+
+// Tensor maps of FP16 keys and values, [slot, token, head, d], whose box is a tile of 64 tokens of one head (64 of its
+// dimensions). usable: the part has them (its strides can be described).
+struct AttentionMaps {
+    CUtensorMap map[2][2];       // prefix, own; keys, values
+    uint32_t usable[2];
+};
+constexpr uint32_t kMapTokens = 64;
+
+cudaError_t launch_attention_tiles(const AttentionParams& params, const AttentionMaps& maps, KvFormat format, uint32_t* error_word,
+                                   long long wait_limit_cycles, cudaStream_t stream, bool early_launch);
 cudaError_t launch_attention_join(const AttentionParams& params, cudaStream_t stream, bool early_launch);
 
 // Where query row r of a pass's group lies.

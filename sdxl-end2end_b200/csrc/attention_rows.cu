@@ -519,7 +519,10 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
             float4* const out = reinterpret_cast<float4*>(p.part_o + place_in_slot * p.dim + d);
             out[0] = make_float4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
             out[1] = make_float4(sum[4] * inverse, sum[5] * inverse, sum[6] * inverse, sum[7] * inverse);
-            if (d == 0) p.part_lse[place_in_slot] = total == 0.0f ? __int_as_float(0xff800000) : largest + log2f(total) - kWeightBits;
+            if (d == 0) {
+                const float kNone = __int_as_float(0xff800000);
+                p.part_lse[place_in_slot] = make_float2(total == 0.0f ? kNone : largest > kNone ? largest : 0.0f, log2f(total) - kWeightBits);
+            }
         }
     }
 }
@@ -534,13 +537,16 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const uint64_t row = index / vectors;
     if (row >= rows) return;
     const uint32_t d = static_cast<uint32_t>(index % vectors) * 8u;
-    float largest = __int_as_float(0xff800000);
-    for (uint32_t s = 0; s < p.slots; ++s) largest = fmaxf(largest, p.part_lse[s * rows + row]);
+    float2 largest = make_float2(__int_as_float(0xff800000), 0.0f);
+    for (uint32_t s = 0; s < p.slots; ++s) {
+        const float2 lse = p.part_lse[s * rows + row];
+        if ((lse.x - largest.x) + (lse.y - largest.y) > 0.0f) largest = lse;
+    }
     float total = 0.0f, sum[8] = {};
     for (uint32_t s = 0; s < p.slots; ++s) {
-        const float lse = p.part_lse[s * rows + row];
-        if (lse == __int_as_float(0xff800000)) continue;         // an empty share
-        const float share = exp2_approx(lse - largest);
+        const float2 lse = p.part_lse[s * rows + row];
+        if (lse.x == __int_as_float(0xff800000)) continue;       // an empty share
+        const float share = exp2_approx((lse.x - largest.x) + (lse.y - largest.y));
         const float4* const part = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.dim + d);
         const float4 a = part[0], b = part[1];
         total += share;

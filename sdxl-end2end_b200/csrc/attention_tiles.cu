@@ -28,33 +28,36 @@ namespace sdxlq {
 namespace {
 
 constexpr uint32_t kTileRows = 128;
-constexpr uint32_t kSlots = 4;                   // K0 V0 K1 V1
-constexpr uint32_t kScaleRing = 4;               // key tiles whose scales are held
+constexpr uint32_t kKeys = 64;                   // of a tile
+constexpr uint32_t kScaleRing = 8;               // key tiles whose scales are held
 constexpr uint32_t kSoftmaxWarps = 4;
 constexpr uint32_t kColumns = 256;
 constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
 
-// Tensor-memory columns of a CTA: S [0, keys), P [keys, keys + keys / 2), O behind it.
+// Tensor-memory columns of a CTA: one or two buffers of S (64 columns) and P (32), and O. Shared memory: Q and a ring of slots
+// that take K and V tiles in turn.
 template <int kDim>
 struct Shape {
-    static constexpr uint32_t kKeys = kDim == 64 ? 128 : 64;
+    static constexpr uint32_t kBuffers = kDim == 64 ? 2 : 1;
     static constexpr uint32_t kColumnS = 0;
-    static constexpr uint32_t kColumnP = kKeys;
+    static constexpr uint32_t kColumnP = kBuffers * kKeys;
     static constexpr uint32_t kColumnO = kDim == 64 ? 192 : 128;
-    static constexpr uint32_t kTileBytes = kKeys * kDim * 2;         // 16 KB
+    static constexpr uint32_t kSlots = kDim == 64 ? 8 : 4;
+    static constexpr uint32_t kTileBytes = kKeys * kDim * 2;
     static constexpr uint32_t kQueryBytes = kTileRows * kDim * 2;
 };
 
 struct TileControl {
-    uint64_t query_ready, score_ready, score_free, weight_ready, value_done, vote, drained;
-    uint64_t full[kSlots], empty[kSlots], scales_full[kScaleRing];
+    uint64_t query_ready, score_ready[2], weight_ready[2], value_done[2], vote, drained;
+    uint64_t full[8], empty[8], scales_full[kScaleRing];
     uint32_t tmem_base;
     uint32_t abort;
-    uint32_t skip[2];                            // of even and odd tiles: the softmax warps add the tile's values themselves
+    uint32_t skip[4];                            // [j % 4] == j + 1: the softmax warps add the values of tile j themselves
 };
 
 struct TileParams {
     AttentionParams a;
+    AttentionMaps maps;
     uint32_t* error_word;
     long long wait_limit_cycles;
 };
@@ -83,7 +86,6 @@ struct Item {
     uint32_t prefix_tiles, tile_begin, tile_end;
 
     __device__ __forceinline__ explicit Item(const AttentionParams& p) {
-        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
         const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
         const AttentionPass& pass = p.pass[second ? 1 : 0];
         uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
@@ -115,7 +117,6 @@ struct Item {
         uint32_t columns;            // keys of the tile, rounded up to the MMA's 16
     };
     __device__ __forceinline__ Tile tile(uint32_t index) const {
-        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
         Tile t;
         t.in_prefix = index < prefix_tiles;
         t.first = (t.in_prefix ? index : index - prefix_tiles) * kKeys;
@@ -128,7 +129,7 @@ struct Item {
 template <int kDim, int kFormat, int kLoaderWarps>
 __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) attention_tiles_kernel(const __grid_constant__ TileParams params) {
     using S = Shape<kDim>;
-    constexpr uint32_t kKeys = S::kKeys;
+    constexpr uint32_t kSlots = S::kSlots, kBuffers = S::kBuffers;
     constexpr bool kScaled = kFormat != KV_F16;
     const AttentionParams& p = params.a;
     extern __shared__ __align__(1024) uint8_t dynamic_smem[];
@@ -141,10 +142,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 
     if (threadIdx.x == 0) {
         ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&control.score_ready), 1);
-        ptx::mbar_init(ptx::smem_u32(&control.score_free), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&control.weight_ready), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&control.value_done), 1);
+        for (uint32_t b = 0; b < kBuffers; ++b) {
+            ptx::mbar_init(ptx::smem_u32(&control.score_ready[b]), 1);
+            ptx::mbar_init(ptx::smem_u32(&control.weight_ready[b]), kSoftmaxWarps);
+            ptx::mbar_init(ptx::smem_u32(&control.value_done[b]), 1);
+        }
         ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
         for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kLoaderWarps);
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             ptx::mbar_init(ptx::smem_u32(&control.empty[s]), 1);
         }
         control.abort = 0;
-        control.skip[0] = control.skip[1] = 0;
+        for (uint32_t i = 0; i < 4; ++i) control.skip[i] = 0;
         ptx::fence_mbar_init();
     }
     if (warp == kSoftmaxWarps) {
@@ -194,42 +196,39 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                    static_cast<int64_t>(t.first) * view.token_stride;
         };
         if constexpr (!kScaled) {
-            constexpr uint32_t kChunks = kDim / 8;                       // of a key
-            constexpr uint32_t kStep = kThreads / kChunks;               // keys per round
-            static_assert(kKeys % kStep == 0);
-            const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
-            const bool in_head = chunk * 8u < p.dim;
-            uint32_t announced = 0;
+            static_assert(kLoaderWarps == 1);
             bool ok = true;
             for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
-                // a slot that is not free yet is not waited for before what has been loaded is passed on
-                const uint32_t bar = empty + (unit % kSlots) * 8u, parity = ((unit / kSlots) & 1u) ^ 1u;
-                if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) {
-                    ptx::cp_async_wait<0>();
-                    for (; announced < unit; ++announced) announce(announced);
-                    if (!slot_free(unit)) { ok = false; break; }
-                }
+                if (!slot_free(unit)) { ok = false; break; }
                 typename Item<kDim>::Tile t;
                 const uint8_t* const base = source(unit, t);
-                const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
-                const uint8_t* from = base + first_key * stride + chunk * 16u;
-                const uint32_t to = slots_base + (unit % kSlots) * S::kTileBytes;
-                for (uint32_t key = first_key; key < t.columns; key += kStep, from += kStep * stride) {
-                    const bool inside = in_head && t.first + key < t.end;
-                    ptx::cp_async16(to + swizzled(key, chunk, kKeys), inside ? from : base, inside);
-                }
-                ptx::cp_async_commit();
-                if (announced < unit) {
-                    ptx::cp_async_wait<1>();
-                    for (; announced < unit; ++announced) announce(announced);
+                const uint32_t to = slots_base + unit % kSlots * S::kTileBytes, bar = full + unit % kSlots * 8u;
+                const uint32_t part = t.in_prefix ? 0u : 1u;
+                if (t.first + kKeys <= t.end && params.maps.usable[part]) {
+                    if (ptx::elect_one()) {
+                        const uint32_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
+                        ptx::mbar_expect_tx(bar, S::kTileBytes);
+#pragma unroll
+                        for (uint32_t d = 0; d < kDim; d += 64) {
+                            ptx::tma_load_4d(to + d * (kKeys * 2), &params.maps.map[part][unit % 2], bar, static_cast<int32_t>(d),
+                                             static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(slot));
+                        }
+                    }
+                    __syncwarp();
+                } else {
+                    // the end of a part: what lies behind it (and within its memory) has to be zeros
+                    const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
+                    for (uint32_t i = lane; i < t.columns * (kDim / 8); i += 32) {
+                        const uint32_t key = i / (kDim / 8), chunk = i % (kDim / 8);
+                        const bool inside = chunk * 8u < p.dim && t.first + key < t.end;
+                        ptx::cp_async16(to + swizzled(key, chunk, kKeys), inside ? base + key * stride + chunk * 16u : base, inside);
+                    }
+                    ptx::cp_async_commit();
+                    ptx::cp_async_wait<0>();
+                    announce(unit);
                 }
             }
-            ptx::cp_async_wait<0>();
-            if (ok) {
-                for (; announced < 2 * tiles; ++announced) announce(announced);
-            } else {
-                give_up(DEV_TIMEOUT_PRODUCER);
-            }
+            if (!ok) give_up(DEV_TIMEOUT_PRODUCER);
         } else {
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     ahead_scale[1] = inside ? __ldg(view.v_scales + at) : 0.0f;
                 }
             };
-            static_assert(kThreads >= kKeys);
+            static_assert(kThreads >= kKeys && kScaleRing >= kSlots / 2 + kBuffers);
             if (tiles != 0) fetch(0);
             for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
                 if (!slot_free(unit)) {
@@ -274,9 +273,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     ptx::st_shared16(to + target0, make_uint4(a.x, a.y, b.x, b.y));
                     ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
                 }
-                // The ring of scales is written this far ahead of its readers: the slot of this tile's K was freed by the
-                // MMA of the tile two before it, which waited for the softmax warps to have read the scores, and with
-                // them the scales, of the tile before that one.
+                // The ring of scales is longer than its writer can be ahead of its readers: this tile's slot was freed by the
+                // MMA of the tile that had it before, kSlots / 2 tiles back, and that had waited for the softmax warps to be
+                // through with the tile kBuffers before it.
                 if (unit % 2 == 0 && thread < kKeys) {
                     scales[unit / 2 % kScaleRing][0][thread] = ahead_scale[0];
                     scales[unit / 2 % kScaleRing][1][thread] = ahead_scale[1];
@@ -298,59 +297,57 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         const auto wait_full = [&](uint32_t unit) {
             return ptx::warp_wait_bounded(full + (unit % kSlots) * 8u, (unit / kSlots) & 1u, abort_word, limit);
         };
-        const auto multiply_scores = [&](uint32_t index) {
-            const uint32_t unit = 2 * index, columns = item.tile(item.tile_begin + index).columns;
+        // V is the B operand with its head dimension together (MN-major: bit 16); 64 of it to an MMA
+        constexpr uint32_t kValueIdesc = ptx::umma_instr_desc(1, 0, 0, kTileRows, 64) | (1u << 16);
+        const uint32_t query_lo = ptx::umma_desc_lo(query_base), slots_lo = ptx::umma_desc_lo(slots_base);
+        const auto multiply_scores = [&](uint32_t j) {
+            const uint32_t slot = 2 * j % kSlots, columns = item.tile(item.tile_begin + j).columns;
             const uint32_t idesc = ptx::umma_instr_desc(1, 0, 0, kTileRows, columns);
             if (ptx::elect_one()) {
-                const uint32_t a = ptx::umma_desc_lo(query_base), b = ptx::umma_desc_lo(slots_base + (unit % kSlots) * S::kTileBytes);
+                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16), d = tmem + S::kColumnS + j % kBuffers * kKeys;
 #pragma unroll
-                for (uint32_t step = 0; step < kDim / 16; ++step) {
-                    const uint32_t within = step % 4 * 2;                // 32 bytes of a swizzle span
-                    ptx::umma_f16_ss(tmem + S::kColumnS, a + step / 4 * (kTileRows * 128 / 16) + within, ptx::kUmmaDescHiSw128,
-                                     b + step / 4 * (kKeys * 128 / 16) + within, ptx::kUmmaDescHiSw128, idesc, step != 0);
+                for (uint32_t part = 0; part < kDim / 64; ++part) {
+                    ptx::umma_stage_f16(d, query_lo + part * (kTileRows * 128 / 16), b + part * (kKeys * 128 / 16), ptx::kUmmaDescHiSw128, idesc, part);
                 }
-                ptx::umma_commit(empty + (unit % kSlots) * 8u);
-                ptx::umma_commit(ptx::smem_u32(&control.score_ready));
+                ptx::umma_commit(empty + slot * 8u);
+                ptx::umma_commit(ptx::smem_u32(&control.score_ready[j % kBuffers]));
             }
             __syncwarp();
         };
-        bool ok = true;
-        if (tiles != 0) {
-            ok = wait(control.query_ready, 0) && wait_full(0);
+        bool ok = tiles == 0 || wait(control.query_ready, 0);
+        for (uint32_t j = 0; ok && j < min(tiles, kBuffers); ++j) {
+            ok = wait_full(2 * j);
             ptx::tc_fence_after();
-            if (ok) multiply_scores(0);
+            if (ok) multiply_scores(j);
         }
         for (uint32_t j = 0; ok && j < tiles; ++j) {
-            if (j + 1 < tiles) {
-                ok = wait(control.score_free, j & 1u) && wait_full(2 * (j + 1));
-                if (!ok) break;
-                ptx::tc_fence_after();
-                multiply_scores(j + 1);
-            }
-            const uint32_t unit = 2 * j + 1;
-            ok = wait(control.weight_ready, j & 1u) && wait_full(unit);
+            const uint32_t unit = 2 * j + 1, slot = unit % kSlots, columns = item.tile(item.tile_begin + j).columns;
+            // the weights of tile j come last: they also say that its scores have been read
+            ok = wait_full(unit) && (j + kBuffers >= tiles || wait_full(2 * (j + kBuffers))) &&
+                 wait(control.weight_ready[j % kBuffers], (j / kBuffers) & 1u);
             if (!ok) break;
             ptx::tc_fence_after();
-            const uint32_t columns = item.tile(item.tile_begin + j).columns;
-            // V is the B operand with its head dimension together (MN-major: bit 16); 64 of it to an MMA
-            constexpr uint32_t idesc = ptx::umma_instr_desc(1, 0, 0, kTileRows, 64) | (1u << 16);
-            const bool skip = *reinterpret_cast<volatile uint32_t*>(&control.skip[j & 1u]) != 0;
+            const bool skip = kFormat != KV_INT8 && p.causal && *reinterpret_cast<volatile uint32_t*>(&control.skip[j % 4]) == j + 1;
             if (ptx::elect_one()) {
-                if (!skip) {
-                    const uint32_t b = ptx::umma_desc_lo(slots_base + (unit % kSlots) * S::kTileBytes);
-                    for (uint32_t step = 0; step < columns / 16; ++step) {
+                const uint32_t a = tmem + S::kColumnP + j % kBuffers * (kKeys / 2), d = tmem + S::kColumnO;
+                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
 #pragma unroll
-                        for (uint32_t part = 0; part < kDim / 64; ++part) {
-                            ptx::umma_f16_ts(tmem + S::kColumnO + part * 64, tmem + S::kColumnP + step * 8,
-                                             b + part * (kKeys * 128 / 16) + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, idesc,
-                                             (j | step) != 0);
+                for (uint32_t part = 0; part < kDim / 64; ++part) {
+                    const uint32_t b_part = b + part * (kKeys * 128 / 16);
+                    if (skip) break;
+                    if (columns == kKeys) {
+                        ptx::umma_f16_ts_x4(d + part * 64, a, b_part, ptx::kUmmaDescHiSw128, kValueIdesc, j);
+                    } else {
+                        for (uint32_t step = 0; step < columns / 16; ++step) {
+                            ptx::umma_f16_ts(d + part * 64, a + step * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc, j | step);
                         }
                     }
                 }
-                ptx::umma_commit(empty + (unit % kSlots) * 8u);
-                ptx::umma_commit(ptx::smem_u32(&control.value_done));
+                ptx::umma_commit(empty + slot * 8u);
+                ptx::umma_commit(ptx::smem_u32(&control.value_done[j % kBuffers]));
             }
             __syncwarp();
+            if (j + kBuffers < tiles) multiply_scores(j + kBuffers);
         }
         if (!ok) {
             give_up(DEV_TIMEOUT_MMA);
@@ -393,7 +390,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + min(row, item.rows - 1));
         const uint32_t own_limit = p.causal ? causal_limit(item.own_length, p.q_tokens, at.token) : item.own_length;
         const float kNone = __int_as_float(0xff800000);
-        float reference = kNone, sum = 0.0f;
+        float reference = kNone, fine = 0.0f, sum = 0.0f;
         uint32_t votes = 0;
         bool ok = true;
         for (uint32_t j = 0; j < tiles; ++j) {
@@ -406,59 +403,123 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
             if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
-            ok = ok && wait(control.score_ready, j & 1u);
+            ok = ok && wait(control.score_ready[j % kBuffers], (j / kBuffers) & 1u);
+            const uint32_t column_s = my_tmem + S::kColumnS + j % kBuffers * kKeys, column_p = my_tmem + S::kColumnP + j % kBuffers * (kKeys / 2);
             if (!ok) break;
             ptx::tc_fence_after();
 
             const uint32_t chunks = (t.columns + 31u) / 32u;
-            float grow = 1.0f;
-            if (warp_active) {
+            // 32 columns of S as scores in units of log2, less the reference. The fused multiply-add rounds the difference
+            // alone, so that it is as exact for large scores as for small ones; where the reference's own last bit is
+            // coarser than the weights' room, its rest (`fine`) is taken off too.
+            bool huge = __any_sync(0xffffffffu, fine != 0.0f);
+            const auto scores = [&](uint32_t c, const uint32_t (&s)[32], float shift, float (&x)[32]) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float4 k = make_float4(scale, scale, scale, scale);
+                    if constexpr (kScaled) k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
+                    const float2 lo = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y), make_float2(-shift, -shift));
+                    const float2 hi = __ffma2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w), make_float2(-shift, -shift));
+                    x[i] = lo.x; x[i + 1] = lo.y; x[i + 2] = hi.x; x[i + 3] = hi.y;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = c * 32u + i < visible ? x[i] : kNone;
+                }
+                if (huge) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] -= fine;
+                }
+            };
+            const auto largest_of = [](const float (&x)[32], float largest) {
+                float other = largest;
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    largest = fmaxf(largest, fmaxf(x[i], x[i + 1]));
+                    other = fmaxf(other, fmaxf(x[i + 2], x[i + 3]));
+                }
+                return fmaxf(largest, other);
+            };
+            float value_bits = 0.0f;                                     // log2 of the tile's largest value scale
+            if constexpr (kScaled) {
+                float top = 1e-20f;
+#pragma unroll
+                for (uint32_t i = 0; i < kKeys; i += 32) top = fmaxf(top, value_scales[i + lane]);
+#pragma unroll
+                for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+                value_bits = log2_approx(top);
+            }
+            if (j >= kBuffers) {
+                ok = wait(control.value_done[j % kBuffers], (j / kBuffers - 1) & 1u);           // this buffer of P is free
+                if (!ok) break;
+                ptx::tc_fence_after();
+            }
+            if (j == 0 && warp_active) {
+                // the first tile's maximum; later tiles take the weights for good unless they pass the reference by too much
                 float largest = kNone;
                 for (uint32_t c = 0; c < chunks; ++c) {
                     uint32_t s[32];
-                    ptx::tmem_ld_32x32b_x32(my_tmem + S::kColumnS + c * 32u, s);
+                    float x[32];
+                    ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
                     ptx::tmem_ld_wait(s);
-                    if (masked) {
+                    scores(c, s, 0.0f, x);
+                    largest = largest_of(x, largest);
+                }
+                reference = largest + value_bits - kWeightBits;
+            }
+            for (int attempt = 0; warp_active; ++attempt) {
+                const float shift = reference > kNone ? reference : 0.0f;
+                float largest = kNone;
+                float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                uint32_t s[32];
+                ptx::tmem_ld_32x32b_x32(column_s, s);
+                for (uint32_t c = 0; c < chunks; ++c) {
+                    float x[32];
+                    uint32_t w[16];
+                    ptx::tmem_ld_wait(s);
+                    scores(c, s, shift, x);
+                    if (c + 1 < chunks) ptx::tmem_ld_32x32b_x32(column_s + (c + 1) * 32u, s);
+                    largest = largest_of(x, largest);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float x = __uint_as_float(s[i]);
-                            if constexpr (kScaled) x *= key_scales[c * 32u + i];
-                            if (c * 32u + i < visible) largest = fmaxf(largest, x);
-                        }
-                    } else {
+                    for (int i = 0; i < 32; i += 4) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float x[4];
+                        for (int e = 0; e < 4; ++e) x[i + e] = exp2_approx(x[i + e]);
+                        part[0] = __fadd2_rn(part[0], make_float2(x[i], x[i + 1]));
+                        part[1] = __fadd2_rn(part[1], make_float2(x[i + 2], x[i + 3]));
+                        if constexpr (kScaled) {
+                            const float4 v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
+                            x[i] *= v.x; x[i + 1] *= v.y; x[i + 2] *= v.z; x[i + 3] *= v.w;
+                            if (masked) {                                // a hidden key's scale may be anything
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(s[i + e]);
-                            if constexpr (kScaled) {
-                                const float4 k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
-                                x[0] *= k.x; x[1] *= k.y; x[2] *= k.z; x[3] *= k.w;
+                                for (int e = 0; e < 4; ++e) x[i + e] = c * 32u + i + e < visible ? x[i + e] : 0.0f;
                             }
-                            largest = fmaxf(largest, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
                         }
+                        w[i / 2] = pack_half2(x[i], x[i + 1]);
+                        w[i / 2 + 1] = pack_half2(x[i + 2], x[i + 3]);
                     }
+                    ptx::tmem_st_32x32b_x16(column_p + c * 16u, w);
                 }
-                float wanted = (kScaled ? largest : largest * scale) - kWeightBits;
-                if constexpr (kScaled) {
-                    float top = 1e-20f;
-#pragma unroll
-                    for (uint32_t i = 0; i < kKeys; i += 32) top = fmaxf(top, value_scales[i + lane]);
-#pragma unroll
-                    for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-                    wanted += log2_approx(top);
+                const float over = largest + value_bits - kWeightBits;
+                const bool passed = over > kSlackBits || (largest > kNone && (reference == kNone || (j == 0 && over < -kSlackBits)));
+                if (attempt == 3 || !__any_sync(0xffffffffu, passed)) {
+                    sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                    break;
                 }
-                if (wanted > reference + kSlackBits) {
-                    grow = exp2_approx(reference - wanted);
-                    reference = wanted;
+                // some row's reference moves: what its sums hold is brought to it, and the tile's weights are taken again
+                float grow = 1.0f;
+                if (passed) {
+                    const float step = fine + over, moved = shift + step, back = moved - shift;
+                    const float rest = fabsf(moved) > 4194304.0f ? (shift - (moved - back)) + (step - back) : 0.0f;
+                    grow = exp2_approx((reference - moved) + (fine - rest));
+                    reference = moved;
+                    fine = rest;
                     sum *= grow;
                 }
-            }
-            if (j != 0) {
-                ok = wait(control.value_done, (j - 1) & 1u);             // O is whole, P is free
-                if (!ok) break;
-                ptx::tc_fence_after();
-                if (warp_active && __any_sync(0xffffffffu, grow != 1.0f)) {
+                huge = __any_sync(0xffffffffu, fine != 0.0f);
+                if (j != 0) {
+                    ok = wait(control.value_done[(j - 1) % kBuffers], ((j - 1) / kBuffers) & 1u);      // O is whole
+                    if (!ok) break;
+                    ptx::tc_fence_after();
 #pragma unroll
                     for (uint32_t c = 0; c < kDim; c += 16) {
                         uint32_t o[16];
@@ -470,57 +531,20 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     }
                 }
             }
-            if (warp_active) {
-                const float shift = reference > kNone ? reference : 0.0f;
-                float part[2] = {0.0f, 0.0f};
-                for (uint32_t c = 0; c < chunks; ++c) {
-                    uint32_t s[32], w[16];
-                    ptx::tmem_ld_32x32b_x32(my_tmem + S::kColumnS + c * 32u, s);
-                    ptx::tmem_ld_wait(s);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        float x[4];
-                        float4 k = make_float4(scale, scale, scale, scale), v = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                        if constexpr (kScaled) {
-                            k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
-                            v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
-                        }
-                        x[0] = fmaf(__uint_as_float(s[i]), k.x, -shift);
-                        x[1] = fmaf(__uint_as_float(s[i + 1]), k.y, -shift);
-                        x[2] = fmaf(__uint_as_float(s[i + 2]), k.z, -shift);
-                        x[3] = fmaf(__uint_as_float(s[i + 3]), k.w, -shift);
-                        if (masked) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e]);
-                        part[0] += x[0] + x[1];
-                        part[1] += x[2] + x[3];
-                        if constexpr (kScaled) {
-                            x[0] *= v.x; x[1] *= v.y; x[2] *= v.z; x[3] *= v.w;
-                            if (masked) {                                // a hidden key's scale may be anything
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : 0.0f;
-                            }
-                        }
-                        w[i / 2] = pack_half2(x[0], x[1]);
-                        w[i / 2 + 1] = pack_half2(x[2], x[3]);
-                    }
-                    ptx::tmem_st_32x32b_x16(my_tmem + S::kColumnP + c * 16u, w);
-                }
-                sum += part[0] + part[1];
-            }
-            arrive(control.score_free);
+            if (!ok) break;
             ptx::tmem_st_wait();
 
             // A value that is not finite makes 0 * v a NaN, also in rows that the causal mask hides it from (what lies behind
             // a length was loaded as zeros). Tiles that such a mask divides are looked through, and one that holds such a value
             // is multiplied here, row by row over the keys that the row sees.
-            if (kFormat != KV_INT8 && p.causal && threadIdx.x == 0) control.skip[(j + 1) & 1u] = 0;
             if (kFormat != KV_INT8 && ragged) {
                 const uint32_t unit = 2 * j + 1, base = slots_base + (unit % kSlots) * S::kTileBytes;
-                volatile uint32_t* const skip = &control.skip[j & 1u];
+                if (j != 0) {                                            // O is whole
+                    ok = wait(control.value_done[(j - 1) % kBuffers], ((j - 1) / kBuffers) & 1u);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                }
+                volatile uint32_t* const skip = &control.skip[j % 4];
                 ok = wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
                 if (!ok) break;
                 bool found = false;
@@ -528,12 +552,12 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     const uint4 x = ptx::ld_shared16(base + swizzled(i / (kDim / 8), i % (kDim / 8), kKeys));
                     found = found || half_not_finite(x.x) || half_not_finite(x.y) || half_not_finite(x.z) || half_not_finite(x.w);
                 }
-                if (found) *skip = 1;
+                if (found) *skip = j + 1;
                 arrive(control.vote);
                 ok = wait(control.vote, votes & 1u);
                 if (!ok) break;
                 ++votes;
-                if (*skip != 0 && warp_active) {
+                if (*skip == j + 1 && warp_active) {
                     for (uint32_t c = 0; c < kDim; c += 8) {
                         uint32_t o[8];
                         ptx::tmem_ld_32x32b_x8(my_tmem + S::kColumnO + c, o);
@@ -543,7 +567,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                         for (int i = 0; i < 8; ++i) total[i] = j == 0 ? 0.0f : __uint_as_float(o[i]);
                         for (uint32_t key = 0; key < t.columns; ++key) {
                             uint32_t pair;
-                            ptx::tmem_ld_32x32b_x1(my_tmem + S::kColumnP + key / 2, pair);
+                            ptx::tmem_ld_32x32b_x1(column_p + key / 2, pair);
                             ptx::tmem_ld_wait(pair);
                             const float w = key % 2 == 0 ? half_lo(pair) : half_hi(pair);
                             const uint4 x = ptx::ld_shared16(base + swizzled(key, c / 8, kKeys));
@@ -561,10 +585,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     ptx::tmem_st_wait();
                 }
             }
-            arrive(control.weight_ready);
+            arrive(control.weight_ready[j % kBuffers]);
         }
         // from here on the room of Q is free: the last product has read it, or (no keys) all warps have written theirs
-        if (ok) ok = tiles != 0 ? wait(control.value_done, (tiles - 1) & 1u) : wait(control.query_ready, 0);
+        if (ok) ok = tiles != 0 ? wait(control.value_done[(tiles - 1) % kBuffers], ((tiles - 1) / kBuffers) & 1u) : wait(control.query_ready, 0);
         ptx::tc_fence_after();
         if (!ok) {
             give_up(DEV_TIMEOUT_EPILOGUE);
@@ -613,7 +637,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                         }
                     }
                 }
-                if (row < item.rows) p.part_lse[place] = sum == 0.0f ? kNone : (reference > kNone ? reference : 0.0f) + log2f(sum);
+                if (row < item.rows) p.part_lse[place] = make_float2(sum == 0.0f ? kNone : reference > kNone ? reference : 0.0f, fine + log2f(sum));
             }
         }
     }
@@ -627,8 +651,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
-    constexpr int kLoaderWarps = kFormat == KV_F16 ? 2 : 4;
-    constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 4;
+    constexpr size_t bytes = Shape<kDim>::kQueryBytes + Shape<kDim>::kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (error != cudaSuccess) return error;
@@ -639,9 +663,9 @@ cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool ear
 
 }  // namespace
 
-cudaError_t launch_attention_tiles(const AttentionParams& params, KvFormat format, uint32_t* error_word, long long wait_limit_cycles,
-                                   cudaStream_t stream, bool early_launch) {
-    const TileParams tile_params{params, error_word, wait_limit_cycles};
+cudaError_t launch_attention_tiles(const AttentionParams& params, const AttentionMaps& maps, KvFormat format, uint32_t* error_word,
+                                   long long wait_limit_cycles, cudaStream_t stream, bool early_launch) {
+    const TileParams tile_params{params, maps, error_word, wait_limit_cycles};
     const auto run = [&](auto dim) {
         constexpr int kDim = decltype(dim)::value;
         switch (format) {

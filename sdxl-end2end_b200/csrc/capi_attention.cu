@@ -248,9 +248,34 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
         pass.items = static_cast<uint32_t>(items[i] * pass.splits);
     }
     if (p.slots > 1) {
-        plan.scratch_bytes = static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * (p.dim + 1) * sizeof(float);
+        plan.scratch_bytes = static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * (p.dim + 2) * sizeof(float);
     }
     return SDXLQ_OK;
+}
+
+// FP16 parts get tensor maps where their strides can be described; an entry of extent 1 may have any stride.
+AttentionMaps encode_maps(const sdxlq_context* ctx, const sdxlq_attention_desc& d) {
+    AttentionMaps maps{};
+    for (int i = 0; i < 2; ++i) {
+        const sdxlq_kv_cache& c = i == 0 ? d.prefix : d.own;
+        if (absent(c) || c.dtype != SDXLQ_FP16 || c.capacity < kMapTokens || ctx->encode == nullptr) continue;
+        const cuuint64_t extent[4] = {c.head_dim, c.heads, c.capacity, c.slots};
+        const uint64_t stride[3] = {c.head_stride, c.token_stride, c.slot_stride};
+        cuuint64_t bytes[3];
+        bool describable = true;
+        for (int axis = 0; axis < 3; ++axis) {
+            bytes[axis] = extent[axis + 1] == 1 ? 16 : stride[axis] * 2;
+            describable = describable && bytes[axis] != 0 && bytes[axis] < uint64_t(1) << 40;
+        }
+        const cuuint32_t box[4] = {64, 1, kMapTokens, 1}, step[4] = {1, 1, 1, 1};
+        for (int part = 0; part < 2 && describable; ++part) {
+            describable = ctx->encode(&maps.map[i][part], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, part == 0 ? c.k : c.v, extent, bytes, box, step,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        }
+        maps.usable[i] = describable ? 1u : 0u;
+    }
+    return maps;
 }
 
 int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
@@ -268,16 +293,18 @@ int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
             return fail(ctx, SDXLQ_ERR_WORKSPACE, "attention: needs " + std::to_string(plan.scratch_bytes) + " bytes of 16-byte aligned scratch");
         }
         p.part_o = static_cast<float*>(scratch);
-        p.part_lse = p.part_o + static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * p.dim;
+        p.part_lse = reinterpret_cast<float2*>(p.part_o + static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * p.dim);
     }
     const DeviceScope device(ctx);
     const bool one_launch = p.pass_count == 1 || (plan.format[0] == plan.format[1] && plan.row_tile[0] == plan.row_tile[1]);
     LaunchTimer timer(ctx, SDXLQ_KERNEL_HARNESS, (one_launch ? 1 : 2) + (p.slots > 1 ? 1 : 0));
     cudaError_t error = cudaSuccess;
+    AttentionMaps maps{};
+    if (plan.row_tile[0] == kTensorTile || plan.row_tile[1] == kTensorTile) maps = encode_maps(ctx, d);
     const auto launch = [&](const AttentionParams& params, uint32_t pass) {
         if (error != cudaSuccess) return;
         error = plan.row_tile[pass] == kTensorTile
-                    ? launch_attention_tiles(params, plan.format[pass], ctx->control, ctx->wait_limit_cycles, ctx->stream, early(ctx))
+                    ? launch_attention_tiles(params, maps, plan.format[pass], ctx->control, ctx->wait_limit_cycles, ctx->stream, early(ctx))
                     : launch_attention_rows(params, plan.format[pass], plan.row_tile[pass], ctx->stream, early(ctx));
     };
     if (one_launch) {

@@ -97,6 +97,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const void* tenso
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void* tensor_map, uint32_t bar, int32_t x, int32_t y, int32_t z,
+                                            int32_t w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
 // Orders a tensor map that was written to global memory by the host (cudaMemcpy) before its
 // first use by this CTA's TMA unit.
 __device__ __forceinline__ void fence_tensormap_acquire(const void* tensor_map) {
@@ -304,23 +313,8 @@ __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t tmem_address, const u
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One FP16 MMA (K = 16) with FP32 accumulators: both operands in shared memory, or A in tensor memory (lane = row, two
-// halves to a column). Descriptors as their two words.
-__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        ".reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
-        "}\n"
-        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
+// One FP16 MMA (K = 16) with FP32 accumulators and A in tensor memory (lane = row, two halves to a column). B's descriptor
+// as its two words.
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
                                             uint32_t accumulate) {
     asm volatile(
@@ -332,6 +326,35 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
         "}\n"
         ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Four of the latter: 64 rows of B (K), 16 to an MMA; eight columns of A and 2 KB of B each.
+__device__ __forceinline__ void umma_f16_ts_x4(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                               uint32_t accumulate_first) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        ".reg .b64 db;\n\t"
+        ".reg .b32 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
+        "add.u32 a, %1, 8;\n\t"
+        "add.u32 b, %2, 128;\n\t"
+        "mov.b64 db, {b, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, q;\n\t"
+        "add.u32 a, %1, 16;\n\t"
+        "add.u32 b, %2, 256;\n\t"
+        "mov.b64 db, {b, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, q;\n\t"
+        "add.u32 a, %1, 24;\n\t"
+        "add.u32 b, %2, 384;\n\t"
+        "mov.b64 db, {b, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, q;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate_first), "r"(1u)
         : "memory");
 }
 

@@ -240,6 +240,25 @@ def test_rising_scores_and_value_scales(gpu, queries):
             assert R.off(y, want, bound) <= 1.0
 
 
+@pytest.mark.parametrize("queries,keys", [(1, 700), (150, 700), (150, 6000), (1, 6000), (40, 6000)])
+def test_huge_scores(gpu, queries, keys):
+    """Scores of 10^8, whose neighbours differ by thousands: the largest takes all the weight, wherever it stands."""
+    pkg, context, ops = gpu
+    dim = 64
+    q = torch.full((1, queries, 1, dim), 4096.0, device="cuda").half()
+    v = normal(22, 1, keys, 1, dim)
+    generator = torch.Generator(device="cuda")
+    generator.manual_seed(23)
+    for sign in (1.0, -1.0):
+        k = (2048.0 + 2.0 * (torch.randperm(keys, generator=generator, device="cuda") % 1000)) * sign
+        at = int(k.argmax())
+        k[at] = (k[at] + 4.0)                             # one key stands out, by 10^5
+        k = k[None, :, None, None].expand(1, keys, 1, dim).half().contiguous()
+        y = ops.shared_prefix_attention(q, pkg.KVCache(k, v))
+        context.check()
+        assert torch.equal(y, v[:, at:at + 1].expand(1, queries, 1, dim))
+
+
 @pytest.mark.parametrize("queries", [1, 3, 20, 150])
 @pytest.mark.parametrize("dim", [64, 80])
 def test_hidden_places_hold_anything(gpu, queries, dim):
