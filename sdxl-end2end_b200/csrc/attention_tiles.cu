@@ -73,6 +73,13 @@ __device__ __forceinline__ float log2_approx(float x) {
     return y;
 }
 
+// The largest of three (max.f32 takes three operands on sm_100).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 __device__ __forceinline__ bool half_not_finite(uint32_t pair) {
     return (pair & 0x7C00u) == 0x7C00u || (pair & 0x7C000000u) == 0x7C000000u;
 }
@@ -392,6 +399,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         const float kNone = __int_as_float(0xff800000);
         float reference = kNone, fine = 0.0f, sum = 0.0f;
         uint32_t votes = 0;
+        uint32_t s0[32];                                                 // the first 32 columns of S, where
+        bool fetched = false;                                            // they were fetched under the tile before
         bool ok = true;
         for (uint32_t j = 0; j < tiles; ++j) {
             const typename Item<kDim>::Tile t = item.tile(item.tile_begin + j);
@@ -403,7 +412,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
             if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
-            ok = ok && wait(control.score_ready[j % kBuffers], (j / kBuffers) & 1u);
+            if (!fetched) ok = ok && wait(control.score_ready[j % kBuffers], (j / kBuffers) & 1u);
             const uint32_t column_s = my_tmem + S::kColumnS + j % kBuffers * kKeys, column_p = my_tmem + S::kColumnP + j % kBuffers * (kKeys / 2);
             if (!ok) break;
             ptx::tc_fence_after();
@@ -435,10 +444,34 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 float other = largest;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    largest = fmaxf(largest, fmaxf(x[i], x[i + 1]));
-                    other = fmaxf(other, fmaxf(x[i + 2], x[i + 3]));
+                    largest = max3(largest, x[i], x[i + 1]);
+                    other = max3(other, x[i + 2], x[i + 3]);
                 }
                 return fmaxf(largest, other);
+            };
+            // 32 weights from their scores: into P, and into the row's sums
+            const auto weigh = [&](uint32_t c, float (&x)[32], float2 (&part)[2]) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i + e] = exp2_approx(x[i + e]);
+                    part[0] = __fadd2_rn(part[0], make_float2(x[i], x[i + 1]));
+                    part[1] = __fadd2_rn(part[1], make_float2(x[i + 2], x[i + 3]));
+                    if constexpr (kScaled) {
+                        const float4 v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
+                        const float2 lo = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(v.x, v.y));
+                        const float2 hi = __fmul2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(v.z, v.w));
+                        x[i] = lo.x; x[i + 1] = lo.y; x[i + 2] = hi.x; x[i + 3] = hi.y;
+                        if (masked) {                                    // a hidden key's scale may be anything
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[i + e] = c * 32u + i + e < visible ? x[i + e] : 0.0f;
+                        }
+                    }
+                    w[i / 2] = pack_half2(x[i], x[i + 1]);
+                    w[i / 2 + 1] = pack_half2(x[i + 2], x[i + 3]);
+                }
+                ptx::tmem_st_32x32b_x16(column_p + c * 16u, w);
             };
             float value_bits = 0.0f;                                     // log2 of the tile's largest value scale
             if constexpr (kScaled) {
@@ -471,33 +504,41 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 const float shift = reference > kNone ? reference : 0.0f;
                 float largest = kNone;
                 float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                uint32_t s[32];
-                ptx::tmem_ld_32x32b_x32(column_s, s);
-                for (uint32_t c = 0; c < chunks; ++c) {
+                if (attempt == 0 && !masked && !huge) {
+                    // the ordinary tile: the next 32 columns, also those of the next tile, are on their way under these
                     float x[32];
-                    uint32_t w[16];
-                    ptx::tmem_ld_wait(s);
-                    scores(c, s, shift, x);
-                    if (c + 1 < chunks) ptx::tmem_ld_32x32b_x32(column_s + (c + 1) * 32u, s);
-                    largest = largest_of(x, largest);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[i + e] = exp2_approx(x[i + e]);
-                        part[0] = __fadd2_rn(part[0], make_float2(x[i], x[i + 1]));
-                        part[1] = __fadd2_rn(part[1], make_float2(x[i + 2], x[i + 3]));
-                        if constexpr (kScaled) {
-                            const float4 v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
-                            x[i] *= v.x; x[i + 1] *= v.y; x[i + 2] *= v.z; x[i + 3] *= v.w;
-                            if (masked) {                                // a hidden key's scale may be anything
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) x[i + e] = c * 32u + i + e < visible ? x[i + e] : 0.0f;
-                            }
-                        }
-                        w[i / 2] = pack_half2(x[i], x[i + 1]);
-                        w[i / 2 + 1] = pack_half2(x[i + 2], x[i + 3]);
+                    uint32_t s1[32];
+                    if (!fetched) {
+                        ptx::tmem_ld_32x32b_x32(column_s, s0);
+                        ptx::tmem_ld_wait(s0);
                     }
-                    ptx::tmem_st_32x32b_x16(column_p + c * 16u, w);
+                    ptx::tmem_ld_32x32b_x32(column_s + 32u, s1);
+                    scores(0, s0, shift, x);
+                    largest = largest_of(x, largest);
+                    weigh(0, x, part);
+                    ptx::tmem_ld_wait(s1);
+                    fetched = kBuffers > 1 && j + 1 < tiles;
+                    if (fetched) {
+                        ok = wait(control.score_ready[(j + 1) % kBuffers], ((j + 1) / kBuffers) & 1u);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+                        ptx::tmem_ld_32x32b_x32(my_tmem + S::kColumnS + (j + 1) % kBuffers * kKeys, s0);
+                    }
+                    scores(1, s1, shift, x);
+                    largest = largest_of(x, largest);
+                    weigh(1, x, part);
+                    ptx::tmem_ld_wait(s0);
+                } else {
+                    for (uint32_t c = 0; c < chunks; ++c) {
+                        float x[32];
+                        uint32_t s[32];
+                        ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
+                        ptx::tmem_ld_wait(s);
+                        scores(c, s, shift, x);
+                        largest = largest_of(x, largest);
+                        weigh(c, x, part);
+                    }
+                    if (attempt == 0) fetched = false;
                 }
                 const float over = largest + value_bits - kWeightBits;
                 const bool passed = over > kSlackBits || (largest > kNone && (reference == kNone || (j == 0 && over < -kSlackBits)));
@@ -651,7 +692,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
-    constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 4;
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 2;
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + Shape<kDim>::kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
