@@ -80,13 +80,15 @@ struct AttentionParams {
 cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
                                   bool early_launch);
 
-// Tensor maps of FP16 keys and values, [slot, token, head, d], whose box is a tile of 64 tokens of one head (64 of its
-// dimensions). usable: the part has them (its strides can be described).
+// Tokens of a tile of keys on the tensor memory.
+__host__ __device__ constexpr uint32_t map_tokens(uint32_t dim) { return dim <= 64 ? 128 : 64; }
+
+// Tensor maps of FP16 keys and values, [slot, token, head, d], whose box is a tile of one head (64 of its dimensions).
+// usable: the part has them (its strides can be described).
 struct AttentionMaps {
     CUtensorMap map[2][2];       // prefix, own; keys, values
     uint32_t usable[2];
 };
-constexpr uint32_t kMapTokens = 64;
 
 cudaError_t launch_attention_tiles(const AttentionParams& params, const AttentionMaps& maps, KvFormat format, uint32_t* error_word,
                                    long long wait_limit_cycles, cudaStream_t stream, bool early_launch);

@@ -28,28 +28,26 @@ namespace sdxlq {
 namespace {
 
 constexpr uint32_t kTileRows = 128;
-constexpr uint32_t kKeys = 64;                   // of a tile
-constexpr uint32_t kScaleRing = 8;               // key tiles whose scales are held
+constexpr uint32_t kSlots = 4;                   // K0 V0 K1 V1
+constexpr uint32_t kScaleRing = 4;               // key tiles whose scales are held
 constexpr uint32_t kSoftmaxWarps = 4;
 constexpr uint32_t kColumns = 256;
 constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
 
-// Tensor-memory columns of a CTA: one or two buffers of S (64 columns) and P (32), and O. Shared memory: Q and a ring of slots
-// that take K and V tiles in turn.
+// Tensor-memory columns of a CTA: S, P (two weights to a column) and O. Shared memory: Q and the ring of slots.
 template <int kDim>
 struct Shape {
-    static constexpr uint32_t kBuffers = kDim == 64 ? 2 : 1;
+    static constexpr uint32_t kKeys = map_tokens(kDim);              // of a tile
     static constexpr uint32_t kColumnS = 0;
-    static constexpr uint32_t kColumnP = kBuffers * kKeys;
+    static constexpr uint32_t kColumnP = kKeys;
     static constexpr uint32_t kColumnO = kDim == 64 ? 192 : 128;
-    static constexpr uint32_t kSlots = kDim == 64 ? 8 : 4;
-    static constexpr uint32_t kTileBytes = kKeys * kDim * 2;
+    static constexpr uint32_t kTileBytes = kKeys * kDim * 2;         // 16 KB
     static constexpr uint32_t kQueryBytes = kTileRows * kDim * 2;
 };
 
 struct TileControl {
-    uint64_t query_ready, score_ready[2], weight_ready[2], value_done[2], vote, drained;
-    uint64_t full[8], empty[8], scales_full[kScaleRing];
+    uint64_t query_ready, score_ready, score_free, weight_ready, value_done, vote, drained;
+    uint64_t full[kSlots], empty[kSlots], scales_full[kScaleRing];
     uint32_t tmem_base;
     uint32_t abort;
     uint32_t skip[4];                            // [j % 4] == j + 1: the softmax warps add the values of tile j themselves
@@ -93,6 +91,7 @@ struct Item {
     uint32_t prefix_tiles, tile_begin, tile_end;
 
     __device__ __forceinline__ explicit Item(const AttentionParams& p) {
+        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
         const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
         const AttentionPass& pass = p.pass[second ? 1 : 0];
         uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
@@ -124,6 +123,7 @@ struct Item {
         uint32_t columns;            // keys of the tile, rounded up to the MMA's 16
     };
     __device__ __forceinline__ Tile tile(uint32_t index) const {
+        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
         Tile t;
         t.in_prefix = index < prefix_tiles;
         t.first = (t.in_prefix ? index : index - prefix_tiles) * kKeys;
@@ -136,7 +136,7 @@ struct Item {
 template <int kDim, int kFormat, int kLoaderWarps>
 __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) attention_tiles_kernel(const __grid_constant__ TileParams params) {
     using S = Shape<kDim>;
-    constexpr uint32_t kSlots = S::kSlots, kBuffers = S::kBuffers;
+    constexpr uint32_t kKeys = S::kKeys, kChunks32 = kKeys / 32;
     constexpr bool kScaled = kFormat != KV_F16;
     const AttentionParams& p = params.a;
     extern __shared__ __align__(1024) uint8_t dynamic_smem[];
@@ -149,11 +149,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 
     if (threadIdx.x == 0) {
         ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
-        for (uint32_t b = 0; b < kBuffers; ++b) {
-            ptx::mbar_init(ptx::smem_u32(&control.score_ready[b]), 1);
-            ptx::mbar_init(ptx::smem_u32(&control.weight_ready[b]), kSoftmaxWarps);
-            ptx::mbar_init(ptx::smem_u32(&control.value_done[b]), 1);
-        }
+        ptx::mbar_init(ptx::smem_u32(&control.score_ready), 1);
+        ptx::mbar_init(ptx::smem_u32(&control.score_free), kSoftmaxWarps);
+        ptx::mbar_init(ptx::smem_u32(&control.weight_ready), kSoftmaxWarps);
+        ptx::mbar_init(ptx::smem_u32(&control.value_done), 1);
         ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
         for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kLoaderWarps);
@@ -245,7 +244,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             const bool in_head = chunk * 16u < p.dim;
             const uint32_t target0 = swizzled(first_key, 2u * chunk, kKeys), target1 = swizzled(first_key, 2u * chunk + 1u, kKeys);
             uint4 ahead[kRounds];
-            float ahead_scale[2] = {0.0f, 0.0f};
+            constexpr uint32_t kScales = (kKeys + kThreads - 1) / kThreads;      // of a thread
+            float ahead_scale[kScales][2] = {};
             const auto fetch = [&](uint32_t unit) {
                 typename Item<kDim>::Tile t;
                 const uint8_t* const base = source(unit, t);
@@ -256,16 +256,19 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     const bool inside = in_head && t.first + first_key + i * kStep < t.end;
                     ahead[i] = inside ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
                 }
-                if (unit % 2 == 0 && thread < kKeys) {
+                if (unit % 2 == 0) {
                     const KvView& view = t.in_prefix ? p.prefix : p.own;
                     const int64_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
-                    const int64_t at = (slot * p.kv_heads + item.kv_head) * view.capacity + t.first + thread;
-                    const bool inside = t.first + thread < t.end;
-                    ahead_scale[0] = inside ? __ldg(view.k_scales + at) * fabsf(p.scale_log2) : 0.0f;
-                    ahead_scale[1] = inside ? __ldg(view.v_scales + at) : 0.0f;
+                    const int64_t at = (slot * p.kv_heads + item.kv_head) * view.capacity + t.first;
+#pragma unroll
+                    for (uint32_t i = 0; i < kScales; ++i) {
+                        const uint32_t key = i * kThreads + thread;
+                        const bool inside = key < kKeys && t.first + key < t.end;
+                        ahead_scale[i][0] = inside ? __ldg(view.k_scales + at + key) * fabsf(p.scale_log2) : 0.0f;
+                        ahead_scale[i][1] = inside ? __ldg(view.v_scales + at + key) : 0.0f;
+                    }
                 }
             };
-            static_assert(kThreads >= kKeys && kScaleRing >= kSlots / 2 + kBuffers);
             if (tiles != 0) fetch(0);
             for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
                 if (!slot_free(unit)) {
@@ -281,11 +284,17 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
                 }
                 // The ring of scales is longer than its writer can be ahead of its readers: this tile's slot was freed by the
-                // MMA of the tile that had it before, kSlots / 2 tiles back, and that had waited for the softmax warps to be
-                // through with the tile kBuffers before it.
-                if (unit % 2 == 0 && thread < kKeys) {
-                    scales[unit / 2 % kScaleRing][0][thread] = ahead_scale[0];
-                    scales[unit / 2 % kScaleRing][1][thread] = ahead_scale[1];
+                // MMA of the tile two before it, and that had waited for the softmax warps to be through with the scores
+                // of the one before that.
+                if (unit % 2 == 0) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kScales; ++i) {
+                        const uint32_t key = i * kThreads + thread;
+                        if (key < kKeys) {
+                            scales[unit / 2 % kScaleRing][0][key] = ahead_scale[i][0];
+                            scales[unit / 2 % kScaleRing][1][key] = ahead_scale[i][1];
+                        }
+                    }
                 }
                 if (unit % 2 == 0) {
                     __syncwarp();
@@ -311,39 +320,43 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             const uint32_t slot = 2 * j % kSlots, columns = item.tile(item.tile_begin + j).columns;
             const uint32_t idesc = ptx::umma_instr_desc(1, 0, 0, kTileRows, columns);
             if (ptx::elect_one()) {
-                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16), d = tmem + S::kColumnS + j % kBuffers * kKeys;
+                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
 #pragma unroll
                 for (uint32_t part = 0; part < kDim / 64; ++part) {
-                    ptx::umma_stage_f16(d, query_lo + part * (kTileRows * 128 / 16), b + part * (kKeys * 128 / 16), ptx::kUmmaDescHiSw128, idesc, part);
+                    ptx::umma_stage_f16(tmem + S::kColumnS, query_lo + part * (kTileRows * 128 / 16), b + part * (kKeys * 128 / 16),
+                                        ptx::kUmmaDescHiSw128, idesc, part);
                 }
                 ptx::umma_commit(empty + slot * 8u);
-                ptx::umma_commit(ptx::smem_u32(&control.score_ready[j % kBuffers]));
+                ptx::umma_commit(ptx::smem_u32(&control.score_ready));
             }
             __syncwarp();
         };
-        bool ok = tiles == 0 || wait(control.query_ready, 0);
-        for (uint32_t j = 0; ok && j < min(tiles, kBuffers); ++j) {
-            ok = wait_full(2 * j);
-            ptx::tc_fence_after();
-            if (ok) multiply_scores(j);
-        }
+        bool ok = tiles == 0 || (wait(control.query_ready, 0) && wait_full(0));
+        ptx::tc_fence_after();
+        if (ok && tiles != 0) multiply_scores(0);
         for (uint32_t j = 0; ok && j < tiles; ++j) {
+            if (j + 1 < tiles) {
+                ok = wait_full(2 * j + 2) && wait(control.score_free, j & 1u);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                multiply_scores(j + 1);
+            }
             const uint32_t unit = 2 * j + 1, slot = unit % kSlots, columns = item.tile(item.tile_begin + j).columns;
-            // the weights of tile j come last: they also say that its scores have been read
-            ok = wait_full(unit) && (j + kBuffers >= tiles || wait_full(2 * (j + kBuffers))) &&
-                 wait(control.weight_ready[j % kBuffers], (j / kBuffers) & 1u);
+            ok = wait_full(unit) && wait(control.weight_ready, j & 1u);
             if (!ok) break;
             ptx::tc_fence_after();
             const bool skip = kFormat != KV_INT8 && p.causal && *reinterpret_cast<volatile uint32_t*>(&control.skip[j % 4]) == j + 1;
             if (ptx::elect_one()) {
-                const uint32_t a = tmem + S::kColumnP + j % kBuffers * (kKeys / 2), d = tmem + S::kColumnO;
-                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
+                const uint32_t a = tmem + S::kColumnP, d = tmem + S::kColumnO, b = slots_lo + slot * (S::kTileBytes / 16);
 #pragma unroll
                 for (uint32_t part = 0; part < kDim / 64; ++part) {
                     const uint32_t b_part = b + part * (kKeys * 128 / 16);
                     if (skip) break;
                     if (columns == kKeys) {
-                        ptx::umma_f16_ts_x4(d + part * 64, a, b_part, ptx::kUmmaDescHiSw128, kValueIdesc, j);
+#pragma unroll
+                        for (uint32_t step = 0; step < kKeys / 16; step += 4) {
+                            ptx::umma_f16_ts_x4(d + part * 64, a + step * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc, j | step);
+                        }
                     } else {
                         for (uint32_t step = 0; step < columns / 16; ++step) {
                             ptx::umma_f16_ts(d + part * 64, a + step * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc, j | step);
@@ -351,10 +364,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     }
                 }
                 ptx::umma_commit(empty + slot * 8u);
-                ptx::umma_commit(ptx::smem_u32(&control.value_done[j % kBuffers]));
+                ptx::umma_commit(ptx::smem_u32(&control.value_done));
             }
             __syncwarp();
-            if (j + kBuffers < tiles) multiply_scores(j + kBuffers);
         }
         if (!ok) {
             give_up(DEV_TIMEOUT_MMA);
@@ -367,6 +379,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         // ---------------------------------------- softmax ----------------------------------------
         const uint32_t row = threadIdx.x;                                // of the tile, and lane of tensor memory
         const uint32_t my_tmem = tmem + ((warp * 32u) << 16);
+        const uint32_t column_s = my_tmem + S::kColumnS, column_p = my_tmem + S::kColumnP, column_o = my_tmem + S::kColumnO;
         const bool warp_active = warp * 32u < item.rows;
         const auto wait = [&](const uint64_t& bar, uint32_t parity) {
             return ptx::warp_wait_bounded(ptx::smem_u32(&bar), parity, abort_word, limit);
@@ -398,9 +411,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         const uint32_t own_limit = p.causal ? causal_limit(item.own_length, p.q_tokens, at.token) : item.own_length;
         const float kNone = __int_as_float(0xff800000);
         float reference = kNone, fine = 0.0f, sum = 0.0f;
+        bool huge = false;                                               // some row of the warp has a `fine`
         uint32_t votes = 0;
-        uint32_t s0[32];                                                 // the first 32 columns of S, where
-        bool fetched = false;                                            // they were fetched under the tile before
         bool ok = true;
         for (uint32_t j = 0; j < tiles; ++j) {
             const typename Item<kDim>::Tile t = item.tile(item.tile_begin + j);
@@ -412,8 +424,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
             if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
-            if (!fetched) ok = ok && wait(control.score_ready[j % kBuffers], (j / kBuffers) & 1u);
-            const uint32_t column_s = my_tmem + S::kColumnS + j % kBuffers * kKeys, column_p = my_tmem + S::kColumnP + j % kBuffers * (kKeys / 2);
+            ok = ok && wait(control.score_ready, j & 1u);
             if (!ok) break;
             ptx::tc_fence_after();
 
@@ -421,7 +432,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             // 32 columns of S as scores in units of log2, less the reference. The fused multiply-add rounds the difference
             // alone, so that it is as exact for large scores as for small ones; where the reference's own last bit is
             // coarser than the weights' room, its rest (`fine`) is taken off too.
-            bool huge = __any_sync(0xffffffffu, fine != 0.0f);
             const auto scores = [&](uint32_t c, const uint32_t (&s)[32], float shift, float (&x)[32]) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
@@ -482,11 +492,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
                 value_bits = log2_approx(top);
             }
-            if (j >= kBuffers) {
-                ok = wait(control.value_done[j % kBuffers], (j / kBuffers - 1) & 1u);           // this buffer of P is free
-                if (!ok) break;
-                ptx::tc_fence_after();
-            }
             if (j == 0 && warp_active) {
                 // the first tile's maximum; later tiles take the weights for good unless they pass the reference by too much
                 float largest = kNone;
@@ -500,36 +505,38 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 }
                 reference = largest + value_bits - kWeightBits;
             }
+            // P is free, and O whole, when the products of the tile before are done
+            const auto wait_for_values = [&] {
+                if (j == 0) return true;
+                const bool done = wait(control.value_done, (j - 1) & 1u);
+                ptx::tc_fence_after();
+                return done;
+            };
             for (int attempt = 0; warp_active; ++attempt) {
                 const float shift = reference > kNone ? reference : 0.0f;
                 float largest = kNone;
                 float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 if (attempt == 0 && !masked && !huge) {
-                    // the ordinary tile: the next 32 columns, also those of the next tile, are on their way under these
-                    float x[32];
-                    uint32_t s1[32];
-                    if (!fetched) {
-                        ptx::tmem_ld_32x32b_x32(column_s, s0);
-                        ptx::tmem_ld_wait(s0);
+                    // the ordinary tile: 32 columns are on their way under the 32 before them
+                    uint32_t s[2][32];
+                    ptx::tmem_ld_32x32b_x32(column_s, s[0]);
+                    ptx::tmem_ld_wait(s[0]);
+#pragma unroll
+                    for (uint32_t c = 0; c < kChunks32; ++c) {
+                        float x[32];
+                        if (c + 1 < kChunks32) ptx::tmem_ld_32x32b_x32(column_s + (c + 1) * 32u, s[(c + 1) & 1]);
+                        scores(c, s[c & 1], shift, x);
+                        largest = largest_of(x, largest);
+                        if (c == 0) {
+                            ok = wait_for_values();
+                            if (!ok) break;
+                        }
+                        weigh(c, x, part);
+                        if (c + 1 < kChunks32) ptx::tmem_ld_wait(s[(c + 1) & 1]);
                     }
-                    ptx::tmem_ld_32x32b_x32(column_s + 32u, s1);
-                    scores(0, s0, shift, x);
-                    largest = largest_of(x, largest);
-                    weigh(0, x, part);
-                    ptx::tmem_ld_wait(s1);
-                    fetched = kBuffers > 1 && j + 1 < tiles;
-                    if (fetched) {
-                        ok = wait(control.score_ready[(j + 1) % kBuffers], ((j + 1) / kBuffers) & 1u);
-                        if (!ok) break;
-                        ptx::tc_fence_after();
-                        ptx::tmem_ld_32x32b_x32(my_tmem + S::kColumnS + (j + 1) % kBuffers * kKeys, s0);
-                    }
-                    scores(1, s1, shift, x);
-                    largest = largest_of(x, largest);
-                    weigh(1, x, part);
-                    ptx::tmem_ld_wait(s0);
                 } else {
-                    for (uint32_t c = 0; c < chunks; ++c) {
+                    if (attempt == 0) ok = wait_for_values();
+                    for (uint32_t c = 0; ok && c < chunks; ++c) {
                         float x[32];
                         uint32_t s[32];
                         ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
@@ -538,8 +545,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                         largest = largest_of(x, largest);
                         weigh(c, x, part);
                     }
-                    if (attempt == 0) fetched = false;
                 }
+                if (!ok) break;
                 const float over = largest + value_bits - kWeightBits;
                 const bool passed = over > kSlackBits || (largest > kNone && (reference == kNone || (j == 0 && over < -kSlackBits)));
                 if (attempt == 3 || !__any_sync(0xffffffffu, passed)) {
@@ -558,21 +565,20 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 }
                 huge = __any_sync(0xffffffffu, fine != 0.0f);
                 if (j != 0) {
-                    ok = wait(control.value_done[(j - 1) % kBuffers], ((j - 1) / kBuffers) & 1u);      // O is whole
-                    if (!ok) break;
-                    ptx::tc_fence_after();
 #pragma unroll
                     for (uint32_t c = 0; c < kDim; c += 16) {
                         uint32_t o[16];
-                        ptx::tmem_ld_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                        ptx::tmem_ld_32x32b_x16(column_o + c, o);
                         ptx::tmem_ld_wait(o);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * grow);
-                        ptx::tmem_st_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                        ptx::tmem_st_32x32b_x16(column_o + c, o);
                     }
                 }
             }
+            if (!warp_active) ok = wait_for_values();
             if (!ok) break;
+            arrive(control.score_free);
             ptx::tmem_st_wait();
 
             // A value that is not finite makes 0 * v a NaN, also in rows that the causal mask hides it from (what lies behind
@@ -580,11 +586,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             // is multiplied here, row by row over the keys that the row sees.
             if (kFormat != KV_INT8 && ragged) {
                 const uint32_t unit = 2 * j + 1, base = slots_base + (unit % kSlots) * S::kTileBytes;
-                if (j != 0) {                                            // O is whole
-                    ok = wait(control.value_done[(j - 1) % kBuffers], ((j - 1) / kBuffers) & 1u);
-                    if (!ok) break;
-                    ptx::tc_fence_after();
-                }
                 volatile uint32_t* const skip = &control.skip[j % 4];
                 ok = wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
                 if (!ok) break;
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 if (*skip == j + 1 && warp_active) {
                     for (uint32_t c = 0; c < kDim; c += 8) {
                         uint32_t o[8];
-                        ptx::tmem_ld_32x32b_x8(my_tmem + S::kColumnO + c, o);
+                        ptx::tmem_ld_32x32b_x8(column_o + c, o);
                         ptx::tmem_ld_wait(o);
                         float total[8];
 #pragma unroll
@@ -621,15 +622,15 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                         }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(total[i]);
-                        ptx::tmem_st_32x32b_x8(my_tmem + S::kColumnO + c, o);
+                        ptx::tmem_st_32x32b_x8(column_o + c, o);
                     }
                     ptx::tmem_st_wait();
                 }
             }
-            arrive(control.weight_ready[j % kBuffers]);
+            arrive(control.weight_ready);
         }
         // from here on the room of Q is free: the last product has read it, or (no keys) all warps have written theirs
-        if (ok) ok = tiles != 0 ? wait(control.value_done[(tiles - 1) % kBuffers], ((tiles - 1) / kBuffers) & 1u) : wait(control.query_ready, 0);
+        if (ok) ok = tiles != 0 ? wait(control.value_done, (tiles - 1) & 1u) : wait(control.query_ready, 0);
         ptx::tc_fence_after();
         if (!ok) {
             give_up(DEV_TIMEOUT_EPILOGUE);
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 #pragma unroll
                 for (uint32_t c = 0; c < kDim; c += 16) {
                     uint32_t o[16];
-                    ptx::tmem_ld_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                    ptx::tmem_ld_32x32b_x16(column_o + c, o);
                     ptx::tmem_ld_wait(o);
                     float x[16];
 #pragma unroll
@@ -666,7 +667,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 #pragma unroll
                 for (uint32_t c = 0; c < kDim; c += 16) {
                     uint32_t o[16];
-                    ptx::tmem_ld_32x32b_x16(my_tmem + S::kColumnO + c, o);
+                    ptx::tmem_ld_32x32b_x16(column_o + c, o);
                     ptx::tmem_ld_wait(o);
                     float4* const out = reinterpret_cast<float4*>(p.part_o + place * p.dim + c);
 #pragma unroll
@@ -693,7 +694,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
     constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 2;
-    constexpr size_t bytes = Shape<kDim>::kQueryBytes + Shape<kDim>::kSlots * Shape<kDim>::kTileBytes;
+    constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (error != cudaSuccess) return error;

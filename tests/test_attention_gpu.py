@@ -242,7 +242,9 @@ def test_rising_scores_and_value_scales(gpu, queries):
 
 @pytest.mark.parametrize("queries,keys", [(1, 700), (150, 700), (150, 6000), (1, 6000), (40, 6000)])
 def test_huge_scores(gpu, queries, keys):
-    """Scores of 10^8, whose neighbours differ by thousands: the largest takes all the weight, wherever it stands."""
+    """Scores of 10^8, whose neighbours differ by thousands: the largest takes all the weight, wherever it stands. The weight,
+    2^x with x up to the reference's last bit, is rounded to a half for the product and not in the sum (2^-11), the result is
+    rounded to a half (2^-11, or half its least step), and 2^x and the quotient are a few last bits of 32 off."""
     pkg, context, ops = gpu
     dim = 64
     q = torch.full((1, queries, 1, dim), 4096.0, device="cuda").half()
@@ -256,7 +258,8 @@ def test_huge_scores(gpu, queries, keys):
         k = k[None, :, None, None].expand(1, keys, 1, dim).half().contiguous()
         y = ops.shared_prefix_attention(q, pkg.KVCache(k, v))
         context.check()
-        assert torch.equal(y, v[:, at:at + 1].expand(1, queries, 1, dim))
+        want = v[:, at:at + 1].expand(1, queries, 1, dim).double()
+        assert ((y.double() - want).abs() <= (2 ** -10 + 2 ** -20) * want.abs() + 2 ** -25).all()
 
 
 @pytest.mark.parametrize("queries", [1, 3, 20, 150])
