@@ -80,8 +80,7 @@ struct AttentionParams {
 cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
                                   bool early_launch);
 
-// Tokens of a tile of keys on the tensor memory.
-__host__ __device__ constexpr uint32_t map_tokens(uint32_t dim) { return dim <= 64 ? 128 : 64; }
+constexpr uint32_t kTileKeys = 64;       // of a tile on the tensor memory
 
 // Tensor maps of FP16 keys and values, [slot, token, head, d], whose box is a tile of one head (64 of its dimensions).
 // usable: the part has them (its strides can be described).

@@ -31,22 +31,20 @@ constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kSlots = 4;                   // K0 V0 K1 V1
 constexpr uint32_t kScaleRing = 4;               // key tiles whose scales are held
 constexpr uint32_t kSoftmaxWarps = 4;
-constexpr uint32_t kColumns = 256;
 constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
 
-// Tensor-memory columns of a CTA: S, P (two weights to a column) and O. Shared memory: Q and the ring of slots.
+// Tensor-memory columns of a CTA: S and, in its place, P (the weights of 32 keys in the first 16 columns of their
+// scores), then O. Shared memory: Q and the ring of slots.
 template <int kDim>
 struct Shape {
-    static constexpr uint32_t kKeys = map_tokens(kDim);              // of a tile
-    static constexpr uint32_t kColumnS = 0;
-    static constexpr uint32_t kColumnP = kKeys;
-    static constexpr uint32_t kColumnO = kDim == 64 ? 192 : 128;
-    static constexpr uint32_t kTileBytes = kKeys * kDim * 2;         // 16 KB
+    static constexpr uint32_t kColumns = kDim == 64 ? 128 : 256;
+    static constexpr uint32_t kColumnO = kDim;
+    static constexpr uint32_t kTileBytes = kTileKeys * kDim * 2;
     static constexpr uint32_t kQueryBytes = kTileRows * kDim * 2;
 };
 
 struct TileControl {
-    uint64_t query_ready, score_ready, score_free, weight_ready, value_done, vote, drained;
+    uint64_t query_ready, score_ready, weight_ready, value_done, vote, drained;
     uint64_t full[kSlots], empty[kSlots], scales_full[kScaleRing];
     uint32_t tmem_base;
     uint32_t abort;
@@ -91,7 +89,6 @@ struct Item {
     uint32_t prefix_tiles, tile_begin, tile_end;
 
     __device__ __forceinline__ explicit Item(const AttentionParams& p) {
-        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
         const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
         const AttentionPass& pass = p.pass[second ? 1 : 0];
         uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
@@ -111,8 +108,8 @@ struct Item {
             own_seen = causal_limit(own_length, p.q_tokens, (first_row + rows - 1) / p.repeat);
             least_limit = causal_limit(own_length, p.q_tokens, first_row / p.repeat);
         }
-        prefix_tiles = (prefix_length + kKeys - 1) / kKeys;
-        const uint64_t tiles = static_cast<uint64_t>(prefix_tiles) + (own_seen + kKeys - 1) / kKeys;
+        prefix_tiles = (prefix_length + kTileKeys - 1) / kTileKeys;
+        const uint64_t tiles = static_cast<uint64_t>(prefix_tiles) + (own_seen + kTileKeys - 1) / kTileKeys;
         tile_begin = static_cast<uint32_t>(tiles * split / pass.splits);
         tile_end = static_cast<uint32_t>(tiles * (split + 1) / pass.splits);
     }
@@ -123,25 +120,23 @@ struct Item {
         uint32_t columns;            // keys of the tile, rounded up to the MMA's 16
     };
     __device__ __forceinline__ Tile tile(uint32_t index) const {
-        constexpr uint32_t kKeys = Shape<kDim>::kKeys;
         Tile t;
         t.in_prefix = index < prefix_tiles;
-        t.first = (t.in_prefix ? index : index - prefix_tiles) * kKeys;
+        t.first = (t.in_prefix ? index : index - prefix_tiles) * kTileKeys;
         t.end = t.in_prefix ? prefix_length : own_seen;
-        t.columns = min(kKeys, (t.end - t.first + 15u) & ~15u);
+        t.columns = min(kTileKeys, (t.end - t.first + 15u) & ~15u);
         return t;
     }
 };
 
-template <int kDim, int kFormat, int kLoaderWarps>
-__global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) attention_tiles_kernel(const __grid_constant__ TileParams params) {
+template <int kDim, int kFormat, int kLoaderWarps, int kBlocks>
+__global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBlocks) attention_tiles_kernel(const __grid_constant__ TileParams params) {
     using S = Shape<kDim>;
-    constexpr uint32_t kKeys = S::kKeys, kChunks32 = kKeys / 32;
     constexpr bool kScaled = kFormat != KV_F16;
     const AttentionParams& p = params.a;
     extern __shared__ __align__(1024) uint8_t dynamic_smem[];
     __shared__ TileControl control;
-    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][2][kScaled ? kKeys : 1];       // key scales * softmax scale, value scales
+    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][2][kScaled ? kTileKeys : 1];       // key scales * softmax scale, value scales
     const uint32_t query_base = ptx::smem_u32(dynamic_smem), slots_base = query_base + S::kQueryBytes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     volatile uint32_t* const abort_word = &control.abort;
@@ -150,7 +145,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
     if (threadIdx.x == 0) {
         ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.score_ready), 1);
-        ptx::mbar_init(ptx::smem_u32(&control.score_free), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.weight_ready), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.value_done), 1);
         ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
@@ -165,7 +159,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         ptx::fence_mbar_init();
     }
     if (warp == kSoftmaxWarps) {
-        ptx::tmem_alloc(ptx::smem_u32(&control.tmem_base), kColumns);
+        ptx::tmem_alloc(ptx::smem_u32(&control.tmem_base), S::kColumns);
         ptx::tmem_relinquish();
     }
     ptx::tc_fence_before();
@@ -210,13 +204,13 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 const uint8_t* const base = source(unit, t);
                 const uint32_t to = slots_base + unit % kSlots * S::kTileBytes, bar = full + unit % kSlots * 8u;
                 const uint32_t part = t.in_prefix ? 0u : 1u;
-                if (t.first + kKeys <= t.end && params.maps.usable[part]) {
+                if (t.first + kTileKeys <= t.end && params.maps.usable[part]) {
                     if (ptx::elect_one()) {
                         const uint32_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
                         ptx::mbar_expect_tx(bar, S::kTileBytes);
 #pragma unroll
                         for (uint32_t d = 0; d < kDim; d += 64) {
-                            ptx::tma_load_4d(to + d * (kKeys * 2), &params.maps.map[part][unit % 2], bar, static_cast<int32_t>(d),
+                            ptx::tma_load_4d(to + d * (kTileKeys * 2), &params.maps.map[part][unit % 2], bar, static_cast<int32_t>(d),
                                              static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(slot));
                         }
                     }
@@ -227,7 +221,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     for (uint32_t i = lane; i < t.columns * (kDim / 8); i += 32) {
                         const uint32_t key = i / (kDim / 8), chunk = i % (kDim / 8);
                         const bool inside = chunk * 8u < p.dim && t.first + key < t.end;
-                        ptx::cp_async16(to + swizzled(key, chunk, kKeys), inside ? base + key * stride + chunk * 16u : base, inside);
+                        ptx::cp_async16(to + swizzled(key, chunk, kTileKeys), inside ? base + key * stride + chunk * 16u : base, inside);
                     }
                     ptx::cp_async_commit();
                     ptx::cp_async_wait<0>();
@@ -238,13 +232,13 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         } else {
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
-            constexpr uint32_t kRounds = kKeys / kStep;
-            static_assert(kStep % 8 == 0 && kKeys % kStep == 0);
+            constexpr uint32_t kRounds = kTileKeys / kStep;
+            static_assert(kStep % 8 == 0 && kTileKeys % kStep == 0);
             const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
             const bool in_head = chunk * 16u < p.dim;
-            const uint32_t target0 = swizzled(first_key, 2u * chunk, kKeys), target1 = swizzled(first_key, 2u * chunk + 1u, kKeys);
+            const uint32_t target0 = swizzled(first_key, 2u * chunk, kTileKeys), target1 = swizzled(first_key, 2u * chunk + 1u, kTileKeys);
             uint4 ahead[kRounds];
-            constexpr uint32_t kScales = (kKeys + kThreads - 1) / kThreads;      // of a thread
+            constexpr uint32_t kScales = (kTileKeys + kThreads - 1) / kThreads;      // of a thread
             float ahead_scale[kScales][2] = {};
             const auto fetch = [&](uint32_t unit) {
                 typename Item<kDim>::Tile t;
@@ -263,7 +257,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
 #pragma unroll
                     for (uint32_t i = 0; i < kScales; ++i) {
                         const uint32_t key = i * kThreads + thread;
-                        const bool inside = key < kKeys && t.first + key < t.end;
+                        const bool inside = key < kTileKeys && t.first + key < t.end;
                         ahead_scale[i][0] = inside ? __ldg(view.k_scales + at + key) * fabsf(p.scale_log2) : 0.0f;
                         ahead_scale[i][1] = inside ? __ldg(view.v_scales + at + key) : 0.0f;
                     }
@@ -284,13 +278,12 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                     ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
                 }
                 // The ring of scales is longer than its writer can be ahead of its readers: this tile's slot was freed by the
-                // MMA of the tile two before it, and that had waited for the softmax warps to be through with the scores
-                // of the one before that.
+                // MMA of the tile two before it, and that had waited for the weights of the one before that.
                 if (unit % 2 == 0) {
 #pragma unroll
                     for (uint32_t i = 0; i < kScales; ++i) {
                         const uint32_t key = i * kThreads + thread;
-                        if (key < kKeys) {
+                        if (key < kTileKeys) {
                             scales[unit / 2 % kScaleRing][0][key] = ahead_scale[i][0];
                             scales[unit / 2 % kScaleRing][1][key] = ahead_scale[i][1];
                         }
@@ -323,7 +316,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
 #pragma unroll
                 for (uint32_t part = 0; part < kDim / 64; ++part) {
-                    ptx::umma_stage_f16(tmem + S::kColumnS, query_lo + part * (kTileRows * 128 / 16), b + part * (kKeys * 128 / 16),
+                    ptx::umma_stage_f16(tmem, query_lo + part * (kTileRows * 128 / 16), b + part * (kTileKeys * 128 / 16),
                                         ptx::kUmmaDescHiSw128, idesc, part);
                 }
                 ptx::umma_commit(empty + slot * 8u);
@@ -335,31 +328,23 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         ptx::tc_fence_after();
         if (ok && tiles != 0) multiply_scores(0);
         for (uint32_t j = 0; ok && j < tiles; ++j) {
-            if (j + 1 < tiles) {
-                ok = wait_full(2 * j + 2) && wait(control.score_free, j & 1u);
-                if (!ok) break;
-                ptx::tc_fence_after();
-                multiply_scores(j + 1);
-            }
             const uint32_t unit = 2 * j + 1, slot = unit % kSlots, columns = item.tile(item.tile_begin + j).columns;
-            ok = wait_full(unit) && wait(control.weight_ready, j & 1u);
+            ok = wait_full(unit) && (j + 1 == tiles || wait_full(unit + 1)) && wait(control.weight_ready, j & 1u);
             if (!ok) break;
             ptx::tc_fence_after();
             const bool skip = kFormat != KV_INT8 && p.causal && *reinterpret_cast<volatile uint32_t*>(&control.skip[j % 4]) == j + 1;
             if (ptx::elect_one()) {
-                const uint32_t a = tmem + S::kColumnP, d = tmem + S::kColumnO, b = slots_lo + slot * (S::kTileBytes / 16);
+                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
 #pragma unroll
                 for (uint32_t part = 0; part < kDim / 64; ++part) {
-                    const uint32_t b_part = b + part * (kKeys * 128 / 16);
+                    const uint32_t d = tmem + S::kColumnO + part * 64, b_part = b + part * (kTileKeys * 128 / 16);
                     if (skip) break;
-                    if (columns == kKeys) {
-#pragma unroll
-                        for (uint32_t step = 0; step < kKeys / 16; step += 4) {
-                            ptx::umma_f16_ts_x4(d + part * 64, a + step * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc, j | step);
-                        }
+                    if (columns == kTileKeys) {
+                        ptx::umma_f16_ts_x4(d, tmem, b_part, ptx::kUmmaDescHiSw128, kValueIdesc, j);
                     } else {
                         for (uint32_t step = 0; step < columns / 16; ++step) {
-                            ptx::umma_f16_ts(d + part * 64, a + step * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc, j | step);
+                            ptx::umma_f16_ts(d, tmem + step / 2 * 32 + step % 2 * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc,
+                                             j | step);
                         }
                     }
                 }
@@ -367,6 +352,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 ptx::umma_commit(ptx::smem_u32(&control.value_done));
             }
             __syncwarp();
+            if (j + 1 < tiles) {
+                ok = wait(control.value_done, j & 1u);                   // P has been read: S may take its place
+                ptx::tc_fence_after();
+                if (ok) multiply_scores(j + 1);
+            }
         }
         if (!ok) {
             give_up(DEV_TIMEOUT_MMA);
@@ -379,7 +369,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
         // ---------------------------------------- softmax ----------------------------------------
         const uint32_t row = threadIdx.x;                                // of the tile, and lane of tensor memory
         const uint32_t my_tmem = tmem + ((warp * 32u) << 16);
-        const uint32_t column_s = my_tmem + S::kColumnS, column_p = my_tmem + S::kColumnP, column_o = my_tmem + S::kColumnO;
+        const uint32_t column_o = my_tmem + S::kColumnO;
         const bool warp_active = warp * 32u < item.rows;
         const auto wait = [&](const uint64_t& bar, uint32_t parity) {
             return ptx::warp_wait_bounded(ptx::smem_u32(&bar), parity, abort_word, limit);
@@ -389,38 +379,48 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bar));
         };
+        const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + min(row, item.rows - 1));
+        // Q and the output move by whole lines: a lane takes 16 bytes of the warp's rows in turn
+        constexpr uint32_t kChunks = kDim / 8, kRowsAtOnce = 32 / kChunks;
+        const uint32_t chunk = lane % kChunks, first_of_warp = warp * 32u + lane / kChunks;
+        const bool in_head = chunk * 8u < p.dim;
         {
-            // Q: a negative softmax scale turns the queries' signs, so that scores are multiplied by its magnitude
+            // a negative softmax scale turns the queries' signs, so that scores are multiplied by its magnitude
             const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-            constexpr uint32_t kChunks = kDim / 8;
-            for (uint32_t i = threadIdx.x; i < kTileRows * kChunks; i += 32 * kSoftmaxWarps) {
-                const uint32_t r = i / kChunks, chunk = i % kChunks;
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (r < item.rows && chunk * 8u < p.dim) {
-                    const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + r);
-                    x = __ldg(reinterpret_cast<const uint4*>(p.q + at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head + chunk * 8u));
-                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+            const int64_t offset = at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head;
+            constexpr uint32_t kBatch = 4;
+#pragma unroll
+            for (uint32_t first = 0; first < 32; first += kBatch * kRowsAtOnce) {
+                uint4 x[kBatch];
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t r = first_of_warp + first + i * kRowsAtOnce;
+                    const int64_t from = __shfl_sync(0xffffffffu, offset, r & 31u);
+                    x[i] = r < item.rows && in_head ? __ldg(reinterpret_cast<const uint4*>(p.q + from + chunk * 8u)) : make_uint4(0u, 0u, 0u, 0u);
                 }
-                ptx::st_shared16(query_base + swizzled(r, chunk, kTileRows), x);
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
+                    ptx::st_shared16(query_base + swizzled(first_of_warp + first + i * kRowsAtOnce, chunk, kTileRows), x[i]);
+                }
             }
             ptx::fence_proxy_async();
             arrive(control.query_ready);
         }
         const float scale = fabsf(p.scale_log2);
-        const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + min(row, item.rows - 1));
         const uint32_t own_limit = p.causal ? causal_limit(item.own_length, p.q_tokens, at.token) : item.own_length;
         const float kNone = __int_as_float(0xff800000);
         float reference = kNone, fine = 0.0f, sum = 0.0f;
-        bool huge = false;                                               // some row of the warp has a `fine`
+        bool huge = false;                                               // some row's reference is coarser than the weights' room
         uint32_t votes = 0;
         bool ok = true;
         for (uint32_t j = 0; j < tiles; ++j) {
             const typename Item<kDim>::Tile t = item.tile(item.tile_begin + j);
             const uint32_t seen_by_all = t.in_prefix ? item.prefix_length : item.least_limit;
-            const bool masked = t.first + kKeys > seen_by_all;
+            const bool masked = t.first + kTileKeys > seen_by_all;
             const bool ragged = p.causal && !t.in_prefix && masked;      // rows differ in what they see of the tile
             const uint32_t seen = t.in_prefix ? item.prefix_length : own_limit;
-            const uint32_t visible = seen > t.first ? min(seen - t.first, kKeys) : 0u;       // columns that this row sees
+            const uint32_t visible = seen > t.first ? min(seen - t.first, kTileKeys) : 0u;       // columns that this row sees
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
             if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
@@ -429,156 +429,139 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
             ptx::tc_fence_after();
 
             const uint32_t chunks = (t.columns + 31u) / 32u;
-            // 32 columns of S as scores in units of log2, less the reference. The fused multiply-add rounds the difference
-            // alone, so that it is as exact for large scores as for small ones; where the reference's own last bit is
-            // coarser than the weights' room, its rest (`fine`) is taken off too.
-            const auto scores = [&](uint32_t c, const uint32_t (&s)[32], float shift, float (&x)[32]) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    float4 k = make_float4(scale, scale, scale, scale);
-                    if constexpr (kScaled) k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
-                    const float2 lo = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y), make_float2(-shift, -shift));
-                    const float2 hi = __ffma2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w), make_float2(-shift, -shift));
-                    x[i] = lo.x; x[i + 1] = lo.y; x[i + 2] = hi.x; x[i + 3] = hi.y;
-                }
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = c * 32u + i < visible ? x[i] : kNone;
-                }
-                if (huge) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] -= fine;
-                }
+            // Scores in units of log2, less the reference. The fused multiply-add rounds the difference alone, so that it is as
+            // exact for large scores as for small ones.
+            const auto key_scale = [&](uint32_t column) {
+                return kScaled ? *reinterpret_cast<const float4*>(key_scales + column) : make_float4(scale, scale, scale, scale);
             };
-            const auto largest_of = [](const float (&x)[32], float largest) {
+            const auto load = [&](uint32_t c, uint32_t (&s)[32]) {
+                ptx::tmem_ld_32x32b_x32(my_tmem + c * 32u, s);
+                ptx::tmem_ld_wait(s);
+            };
+            // the largest of 32 columns: of the scores in FP16 without their scale, which is the same for all
+            const auto largest_of = [&](auto careful_case, uint32_t c, const uint32_t (&s)[32], float largest) {
+                constexpr bool careful = decltype(careful_case)::value;
                 float other = largest;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    largest = max3(largest, x[i], x[i + 1]);
-                    other = max3(other, x[i + 2], x[i + 3]);
+                    float x[4] = {__uint_as_float(s[i]), __uint_as_float(s[i + 1]), __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])};
+                    if constexpr (kScaled) {
+                        const float4 k = key_scale(c * 32u + i);
+                        x[0] *= k.x; x[1] *= k.y; x[2] *= k.z; x[3] *= k.w;
+                    }
+                    if (careful) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
+                    }
+                    largest = max3(largest, x[0], x[1]);
+                    other = max3(other, x[2], x[3]);
                 }
                 return fmaxf(largest, other);
             };
-            // 32 weights from their scores: into P, and into the row's sums
-            const auto weigh = [&](uint32_t c, float (&x)[32], float2 (&part)[2]) {
+            // the weights of 32 columns: into P, and into the row's sum
+            const auto weigh = [&](auto careful_case, uint32_t c, const uint32_t (&s)[32], float shift, float2 (&part)[2]) {
+                constexpr bool careful = decltype(careful_case)::value;
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
+                    const float4 k = key_scale(c * 32u + i);
+                    const float2 lo = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y), make_float2(-shift, -shift));
+                    const float2 hi = __ffma2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w), make_float2(-shift, -shift));
+                    float x[4] = {lo.x, lo.y, hi.x, hi.y};
+                    if (careful) {
+                        if (kScaled && huge) {                           // rounded as the maximum was
+                            x[0] = __fmul_rn(__uint_as_float(s[i]), k.x) - shift; x[1] = __fmul_rn(__uint_as_float(s[i + 1]), k.y) - shift;
+                            x[2] = __fmul_rn(__uint_as_float(s[i + 2]), k.z) - shift; x[3] = __fmul_rn(__uint_as_float(s[i + 3]), k.w) - shift;
+                        }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[i + e] = exp2_approx(x[i + e]);
-                    part[0] = __fadd2_rn(part[0], make_float2(x[i], x[i + 1]));
-                    part[1] = __fadd2_rn(part[1], make_float2(x[i + 2], x[i + 3]));
+                        for (int e = 0; e < 4; ++e) x[e] -= fine;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (careful) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
+                        x[e] = exp2_approx(x[e]);
+                    }
+                    part[0] = __fadd2_rn(part[0], make_float2(x[0], x[1]));
+                    part[1] = __fadd2_rn(part[1], make_float2(x[2], x[3]));
                     if constexpr (kScaled) {
                         const float4 v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
-                        const float2 lo = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(v.x, v.y));
-                        const float2 hi = __fmul2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(v.z, v.w));
-                        x[i] = lo.x; x[i + 1] = lo.y; x[i + 2] = hi.x; x[i + 3] = hi.y;
-                        if (masked) {                                    // a hidden key's scale may be anything
+                        x[0] *= v.x; x[1] *= v.y; x[2] *= v.z; x[3] *= v.w;
+                        if (careful) {                                   // a hidden key's scale may be anything
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[i + e] = c * 32u + i + e < visible ? x[i + e] : 0.0f;
+                            for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : 0.0f;
                         }
                     }
-                    w[i / 2] = pack_half2(x[i], x[i + 1]);
-                    w[i / 2 + 1] = pack_half2(x[i + 2], x[i + 3]);
+                    w[i / 2] = pack_half2(x[0], x[1]);
+                    w[i / 2 + 1] = pack_half2(x[2], x[3]);
                 }
-                ptx::tmem_st_32x32b_x16(column_p + c * 16u, w);
+                ptx::tmem_st_32x32b_x16(my_tmem + c * 32u, w);
             };
-            float value_bits = 0.0f;                                     // log2 of the tile's largest value scale
-            if constexpr (kScaled) {
-                float top = 1e-20f;
+            if (warp_active) {
+                float value_bits = 0.0f;                                 // log2 of the tile's largest value scale
+                if constexpr (kScaled) {
+                    float top = 1e-20f;
 #pragma unroll
-                for (uint32_t i = 0; i < kKeys; i += 32) top = fmaxf(top, value_scales[i + lane]);
+                    for (uint32_t i = 0; i < kTileKeys; i += 32) top = fmaxf(top, value_scales[i + lane]);
 #pragma unroll
-                for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-                value_bits = log2_approx(top);
-            }
-            if (j == 0 && warp_active) {
-                // the first tile's maximum; later tiles take the weights for good unless they pass the reference by too much
-                float largest = kNone;
-                for (uint32_t c = 0; c < chunks; ++c) {
-                    uint32_t s[32];
-                    float x[32];
-                    ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
-                    ptx::tmem_ld_wait(s);
-                    scores(c, s, 0.0f, x);
-                    largest = largest_of(x, largest);
+                    for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+                    value_bits = log2_approx(top);
                 }
-                reference = largest + value_bits - kWeightBits;
-            }
-            // P is free, and O whole, when the products of the tile before are done
-            const auto wait_for_values = [&] {
-                if (j == 0) return true;
-                const bool done = wait(control.value_done, (j - 1) & 1u);
-                ptx::tc_fence_after();
-                return done;
-            };
-            for (int attempt = 0; warp_active; ++attempt) {
-                const float shift = reference > kNone ? reference : 0.0f;
+                const bool both = t.columns > 32u;
+                uint32_t s[32];
                 float largest = kNone;
+                const auto find_largest = [&](auto careful) {
+                    load(0, s);
+                    largest = largest_of(careful, 0, s, largest);
+                    if (both) {
+                        load(1, s);
+                        largest = largest_of(careful, 1, s, largest);
+                    }
+                };
+                if (masked) find_largest(std::true_type{});
+                else find_largest(std::false_type{});
+                // the reference moves where the tile's largest weight would be 2^7 past its place, and in the row's first tile
+                const float unit = kScaled ? 1.0f : scale;
+                const bool first = reference == kNone && largest > kNone;
+                const float base = first ? largest * unit : reference;
+                const float over = fmaf(largest, unit, -base) - fine + value_bits - kWeightBits;
+                const bool moves = first || over > kSlackBits;
+                if (__any_sync(0xffffffffu, moves)) {
+                    float grow = 1.0f;
+                    if (moves) {
+                        // the last bit of a reference past 2^22 is coarser than the weights' room: what it rounds off is kept too
+                        const float step = fine + over, moved = base + step, back = moved - base;
+                        const float rest = fabsf(moved) > 4194304.0f ? (base - (moved - back)) + (step - back) : 0.0f;
+                        grow = exp2_approx((reference - moved) + (fine - rest));
+                        reference = moved;
+                        fine = rest;
+                        sum *= grow;
+                    }
+                    huge = __any_sync(0xffffffffu, fabsf(reference) > 4194304.0f && reference != kNone);
+                    if (j != 0) {                                        // the scores' MMA came behind the products of the tile before: O is whole
+#pragma unroll
+                        for (uint32_t c = 0; c < kDim; c += 16) {
+                            uint32_t o[16];
+                            ptx::tmem_ld_32x32b_x16(column_o + c, o);
+                            ptx::tmem_ld_wait(o);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * grow);
+                            ptx::tmem_st_32x32b_x16(column_o + c, o);
+                        }
+                    }
+                }
                 float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                if (attempt == 0 && !masked && !huge) {
-                    // the ordinary tile: 32 columns are on their way under the 32 before them
-                    uint32_t s[2][32];
-                    ptx::tmem_ld_32x32b_x32(column_s, s[0]);
-                    ptx::tmem_ld_wait(s[0]);
-#pragma unroll
-                    for (uint32_t c = 0; c < kChunks32; ++c) {
-                        float x[32];
-                        if (c + 1 < kChunks32) ptx::tmem_ld_32x32b_x32(column_s + (c + 1) * 32u, s[(c + 1) & 1]);
-                        scores(c, s[c & 1], shift, x);
-                        largest = largest_of(x, largest);
-                        if (c == 0) {
-                            ok = wait_for_values();
-                            if (!ok) break;
-                        }
-                        weigh(c, x, part);
-                        if (c + 1 < kChunks32) ptx::tmem_ld_wait(s[(c + 1) & 1]);
+                const float shift = reference == kNone ? 0.0f : reference;       // a row that has seen nothing has no weights at all
+                const auto take_weights = [&](auto careful) {
+                    if (both) {
+                        weigh(careful, 1, s, shift, part);
+                        load(0, s);
                     }
-                } else {
-                    if (attempt == 0) ok = wait_for_values();
-                    for (uint32_t c = 0; ok && c < chunks; ++c) {
-                        float x[32];
-                        uint32_t s[32];
-                        ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
-                        ptx::tmem_ld_wait(s);
-                        scores(c, s, shift, x);
-                        largest = largest_of(x, largest);
-                        weigh(c, x, part);
-                    }
-                }
-                if (!ok) break;
-                const float over = largest + value_bits - kWeightBits;
-                const bool passed = over > kSlackBits || (largest > kNone && (reference == kNone || (j == 0 && over < -kSlackBits)));
-                if (attempt == 3 || !__any_sync(0xffffffffu, passed)) {
-                    sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-                    break;
-                }
-                // some row's reference moves: what its sums hold is brought to it, and the tile's weights are taken again
-                float grow = 1.0f;
-                if (passed) {
-                    const float step = fine + over, moved = shift + step, back = moved - shift;
-                    const float rest = fabsf(moved) > 4194304.0f ? (shift - (moved - back)) + (step - back) : 0.0f;
-                    grow = exp2_approx((reference - moved) + (fine - rest));
-                    reference = moved;
-                    fine = rest;
-                    sum *= grow;
-                }
-                huge = __any_sync(0xffffffffu, fine != 0.0f);
-                if (j != 0) {
-#pragma unroll
-                    for (uint32_t c = 0; c < kDim; c += 16) {
-                        uint32_t o[16];
-                        ptx::tmem_ld_32x32b_x16(column_o + c, o);
-                        ptx::tmem_ld_wait(o);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * grow);
-                        ptx::tmem_st_32x32b_x16(column_o + c, o);
-                    }
-                }
+                    weigh(careful, 0, s, shift, part);
+                };
+                if (masked || huge) take_weights(std::true_type{});
+                else take_weights(std::false_type{});
+                sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
             }
-            if (!warp_active) ok = wait_for_values();
-            if (!ok) break;
-            arrive(control.score_free);
             ptx::tmem_st_wait();
 
             // A value that is not finite makes 0 * v a NaN, also in rows that the causal mask hides it from (what lies behind
@@ -591,7 +574,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                 if (!ok) break;
                 bool found = false;
                 for (uint32_t i = threadIdx.x; i < t.columns * (kDim / 8); i += 32 * kSoftmaxWarps) {
-                    const uint4 x = ptx::ld_shared16(base + swizzled(i / (kDim / 8), i % (kDim / 8), kKeys));
+                    const uint4 x = ptx::ld_shared16(base + swizzled(i / (kDim / 8), i % (kDim / 8), kTileKeys));
                     found = found || half_not_finite(x.x) || half_not_finite(x.y) || half_not_finite(x.z) || half_not_finite(x.w);
                 }
                 if (found) *skip = j + 1;
@@ -609,10 +592,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                         for (int i = 0; i < 8; ++i) total[i] = j == 0 ? 0.0f : __uint_as_float(o[i]);
                         for (uint32_t key = 0; key < t.columns; ++key) {
                             uint32_t pair;
-                            ptx::tmem_ld_32x32b_x1(column_p + key / 2, pair);
+                            ptx::tmem_ld_32x32b_x1(my_tmem + key / 32 * 32 + key % 32 / 2, pair);
                             ptx::tmem_ld_wait(pair);
                             const float w = key % 2 == 0 ? half_lo(pair) : half_hi(pair);
-                            const uint4 x = ptx::ld_shared16(base + swizzled(key, c / 8, kKeys));
+                            const uint4 x = ptx::ld_shared16(base + swizzled(key, c / 8, kTileKeys));
                             if (key < visible) {
                                 total[0] = fmaf(w, half_lo(x.x), total[0]); total[1] = fmaf(w, half_hi(x.x), total[1]);
                                 total[2] = fmaf(w, half_lo(x.y), total[2]); total[3] = fmaf(w, half_hi(x.y), total[3]);
@@ -653,13 +636,12 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
                                      make_uint4(pack_half2(x[8], x[9]), pack_half2(x[10], x[11]), pack_half2(x[12], x[13]), pack_half2(x[14], x[15])));
                 }
                 __syncwarp();
-                constexpr uint32_t kChunks = kDim / 8;
-                for (uint32_t i = lane; i < 32 * kChunks; i += 32) {
-                    const uint32_t r = warp * 32u + i / kChunks, chunk = i % kChunks;
-                    if (r >= item.rows || chunk * 8u >= p.dim) continue;
-                    const QueryRow to = locate_row(p, item.first_member, item.kv_head, item.first_row + r);
-                    *reinterpret_cast<uint4*>(p.y + to.batch * p.y_batch + to.token * p.y_token + to.head * p.y_head + chunk * 8u) =
-                        ptx::ld_shared16(query_base + swizzled(r, chunk, kTileRows));
+                const int64_t offset = at.batch * p.y_batch + at.token * p.y_token + at.head * p.y_head;
+#pragma unroll 4
+                for (uint32_t i = 0; i < 32; i += kRowsAtOnce) {
+                    const uint32_t r = first_of_warp + i;
+                    const int64_t to = __shfl_sync(0xffffffffu, offset, r & 31u);
+                    if (r < item.rows && in_head) *reinterpret_cast<uint4*>(p.y + to + chunk * 8u) = ptx::ld_shared16(query_base + swizzled(r, chunk, kTileRows));
                 }
             } else {
                 const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
@@ -687,15 +669,16 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), 2) at
     __syncthreads();
     if (warp == kSoftmaxWarps) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem, kColumns);
+        ptx::tmem_dealloc(tmem, S::kColumns);
     }
 }
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
     constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 2;
+    constexpr int kBlocks = kDim == 64 ? (kFormat == KV_F16 ? 4 : 3) : 2;
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
-    auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps>;
+    auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps, kBlocks>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (error != cudaSuccess) return error;
     uint32_t blocks = 0;

@@ -258,7 +258,7 @@ AttentionMaps encode_maps(const sdxlq_context* ctx, const sdxlq_attention_desc& 
     AttentionMaps maps{};
     for (int i = 0; i < 2; ++i) {
         const sdxlq_kv_cache& c = i == 0 ? d.prefix : d.own;
-        if (absent(c) || c.dtype != SDXLQ_FP16 || c.capacity < map_tokens(static_cast<uint32_t>(d.head_dim)) || ctx->encode == nullptr) continue;
+        if (absent(c) || c.dtype != SDXLQ_FP16 || c.capacity < kTileKeys || ctx->encode == nullptr) continue;
         const cuuint64_t extent[4] = {c.head_dim, c.heads, c.capacity, c.slots};
         const uint64_t stride[3] = {c.head_stride, c.token_stride, c.slot_stride};
         cuuint64_t bytes[3];
@@ -267,7 +267,7 @@ AttentionMaps encode_maps(const sdxlq_context* ctx, const sdxlq_attention_desc& 
             bytes[axis] = extent[axis + 1] == 1 ? 16 : stride[axis] * 2;
             describable = describable && bytes[axis] != 0 && bytes[axis] < uint64_t(1) << 40;
         }
-        const cuuint32_t box[4] = {64, 1, map_tokens(static_cast<uint32_t>(d.head_dim)), 1}, step[4] = {1, 1, 1, 1};
+        const cuuint32_t box[4] = {64, 1, kTileKeys, 1}, step[4] = {1, 1, 1, 1};
         for (int part = 0; part < 2 && describable; ++part) {
             describable = ctx->encode(&maps.map[i][part], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, part == 0 ? c.k : c.v, extent, bytes, box, step,
                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -329,7 +329,7 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         : "memory");
 }
 
-// Four of the latter: 64 rows of B (K), 16 to an MMA; eight columns of A and 2 KB of B each.
+// Four of the latter over 64 rows of B (K), 2 KB to an MMA; A in columns 0, 8, 32 and 40 from `tmem_a`, eight to an MMA.
 __device__ __forceinline__ void umma_f16_ts_x4(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
                                                uint32_t accumulate_first) {
     asm volatile(
@@ -345,11 +345,11 @@ __device__ __forceinline__ void umma_f16_ts_x4(uint32_t tmem_d, uint32_t tmem_a,
         "add.u32 b, %2, 128;\n\t"
         "mov.b64 db, {b, %3};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, q;\n\t"
-        "add.u32 a, %1, 16;\n\t"
+        "add.u32 a, %1, 32;\n\t"
         "add.u32 b, %2, 256;\n\t"
         "mov.b64 db, {b, %3};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, q;\n\t"
-        "add.u32 a, %1, 24;\n\t"
+        "add.u32 a, %1, 40;\n\t"
         "add.u32 b, %2, 384;\n\t"
         "mov.b64 db, {b, %3};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, q;\n\t"
