@@ -47,17 +47,20 @@ cudaError_t launch_kv_read(const KvCopyLaunch& launch, cudaStream_t stream, bool
 // rows of several batch entries that read the same keys stand behind one another.
 //
 // A launch runs one or two passes. A pass takes `members` batch entries together (all that share a prefix, or one) over
-// the prefix, over the entries' own keys (members == 1), or over the one and then the other. Each of its items is a tile of
-// rows of one key head over one of `splits` shares of the keys. Where a row gets its result from one item alone, the item
-// writes it; else every item leaves its share in a slot of the scratch and the join kernel adds them up.
+// the prefix, over the entries' own keys (members == 1), or over the one and then the other. Its tiles are tiles of rows of
+// one key head, numbered (group, key head, row tile), and each of its blocks takes one of them over one of `splits` shares
+// of the keys. Where a row gets its result from one block alone, that block writes it; else every block leaves its share in
+// the scratch and the join kernel adds them up, either over all rows (the passes are the parts of every row: `by_row`), or
+// over the tiles of one pass.
 struct AttentionPass {
     uint32_t members, groups;    // batch = members * groups
     uint32_t rows;               // members * q_tokens * repeat
     uint32_t row_tiles, splits;
-    uint32_t items;              // row_tiles * splits * kv_heads * groups
-    uint32_t first_slot;         // scratch slot of split 0
+    uint32_t first_tile, tiles;  // of row_tiles * kv_heads * groups
+    uint32_t first_slot;         // by_row: scratch slot of split 0
     uint32_t with_prefix, with_own;
 };
+constexpr uint32_t kMaxPasses = 2;
 
 struct AttentionParams {
     const __half* q;
@@ -70,17 +73,21 @@ struct AttentionParams {
     uint32_t causal;
     float scale_log2;            // softmax scale * log2(e)
     uint32_t pass_count;
-    AttentionPass pass[2];
-    float* part_o;               // [slots, batch * q_tokens * q_heads, dim] shares, each divided by its own sum; null: no join
-    float2* part_lse;            // [slots, batch * q_tokens * q_heads] log2 of the sum of 2^score in two parts, which scores of
+    AttentionPass pass[kMaxPasses];
+    uint32_t by_row;
+    uint32_t slots;              // shares of a row: all passes' splits, or those of the pass that has more than one
+    uint64_t slot_rows;          // rows of a slot: batch * q_tokens * q_heads, or that pass's tiles * tile rows
+    float* part_o;               // [slots, slot_rows, dim] shares, each divided by its own sum
+    float2* part_lse;            // [slots, slot_rows] log2 of the sum of 2^score in two parts, which scores of
                                  // any size leave exact; -inf in the first for an empty share
-    uint32_t slots;
 };
 
 cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format, uint32_t row_tile, cudaStream_t stream,
                                   bool early_launch);
 
 constexpr uint32_t kTileKeys = 64;       // of a tile on the tensor memory
+// Blocks of that kernel on an SM, by their tensor memory, shared memory and registers.
+__host__ __device__ constexpr uint32_t tile_blocks_per_sm(uint32_t dim, KvFormat format) { return dim > 64 ? 2 : format == KV_F16 ? 4 : 3; }
 
 // Tensor maps of FP16 keys and values, [slot, token, head, d], whose box is a tile of one head (64 of its dimensions).
 // usable: the part has them (its strides can be described).
@@ -91,7 +98,39 @@ struct AttentionMaps {
 
 cudaError_t launch_attention_tiles(const AttentionParams& params, const AttentionMaps& maps, KvFormat format, uint32_t* error_word,
                                    long long wait_limit_cycles, cudaStream_t stream, bool early_launch);
-cudaError_t launch_attention_join(const AttentionParams& params, cudaStream_t stream, bool early_launch);
+// tile_rows: of the pass that is joined (by_row: not used).
+cudaError_t launch_attention_join(const AttentionParams& params, uint32_t tile_rows, cudaStream_t stream, bool early_launch);
+
+// A block's place in its pass.
+struct BlockPlace {
+    uint32_t pass, split, tile;  // tile: of the pass's, from 0
+    uint32_t row_tile, kv_head, first_member;
+};
+
+__device__ __forceinline__ BlockPlace place_block(const AttentionParams& p, uint32_t block) {
+    BlockPlace at;
+    const uint32_t first = p.pass[0].tiles * p.pass[0].splits;
+    at.pass = p.pass_count > 1 && block >= first ? 1u : 0u;
+    const AttentionPass& pass = p.pass[at.pass];
+    block -= at.pass ? first : 0u;
+    at.split = block / pass.tiles;
+    at.tile = block % pass.tiles;
+    uint32_t tile = pass.first_tile + at.tile;
+    at.row_tile = tile % pass.row_tiles;
+    tile /= pass.row_tiles;
+    at.kv_head = tile % p.kv_heads;
+    at.first_member = tile / p.kv_heads * pass.members;
+    return at;
+}
+
+// Whether the block's rows are whole, and if not, where in the scratch row `row` of its tile (which is row `global_row` of the
+// output) goes.
+__device__ __forceinline__ bool writes_output(const AttentionParams& p, const BlockPlace& at) { return !p.by_row && p.pass[at.pass].splits == 1; }
+
+__device__ __forceinline__ uint64_t scratch_row(const AttentionParams& p, const BlockPlace& at, uint32_t tile_rows, uint32_t row, uint64_t global_row) {
+    return p.by_row ? (p.pass[at.pass].first_slot + at.split) * p.slot_rows + global_row
+                    : at.split * p.slot_rows + static_cast<uint64_t>(at.tile) * tile_rows + row;
+}
 
 // Where query row r of a pass's group lies.
 struct QueryRow {

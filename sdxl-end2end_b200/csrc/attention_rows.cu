@@ -170,17 +170,11 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
 
     wait_for_prior_kernels_then_release_next();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
-    const AttentionPass& pass = p.pass[second ? 1 : 0];
-    uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
-    const uint32_t row_tile = item % pass.row_tiles;
-    item /= pass.row_tiles;
-    const uint32_t split = item % pass.splits;
-    item /= pass.splits;
-    const uint32_t kv_head = item % p.kv_heads, first_member = item / p.kv_heads * pass.members;
-    const uint32_t first_row = row_tile * kTileRows;
+    const BlockPlace here = place_block(p, blockIdx.x);
+    const AttentionPass& pass = p.pass[here.pass];
+    const uint32_t kv_head = here.kv_head, first_member = here.first_member, first_row = here.row_tile * kTileRows;
 
-    // the keys of the item: blocks of the prefix, then of the entry's own keys
+    // the keys of the block: blocks of the prefix, then of the entry's own keys
     const uint32_t prefix_slot = pass.with_prefix ? first_member / p.rows_per_prefix : 0u;
     const uint32_t prefix_length = pass.with_prefix ? length_of(p.prefix, prefix_slot) : 0u;
     const uint32_t own_length = pass.with_own ? length_of(p.own, first_member) : 0u;
@@ -188,8 +182,8 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
     const uint32_t own_seen = p.causal && pass.with_own ? causal_limit(own_length, p.q_tokens, last_row / p.repeat) : own_length;
     const uint32_t prefix_blocks = (prefix_length + kKeys - 1) / kKeys, own_blocks = (own_seen + kKeys - 1) / kKeys;
     const uint64_t blocks = static_cast<uint64_t>(prefix_blocks) + own_blocks;
-    const uint32_t block_begin = static_cast<uint32_t>(blocks * split / pass.splits);
-    const uint32_t block_end = static_cast<uint32_t>(blocks * (split + 1) / pass.splits);
+    const uint32_t block_begin = static_cast<uint32_t>(blocks * here.split / pass.splits);
+    const uint32_t block_end = static_cast<uint32_t>(blocks * (here.split + 1) / pass.splits);
 
     // Q, and how many own keys each of the lane's rows sees
     uint32_t q[kRowTiles][kSteps][4];
@@ -507,15 +501,14 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
         }
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
         const QueryRow at = locate_row(p, first_member, kv_head, first_row + r);
-        if (p.part_o == nullptr) {
+        if (writes_output(p, here)) {
             __half* const row = p.y + at.batch * p.y_batch + at.token * p.y_token + at.head * p.y_head + d;
             const uint4 packed = make_uint4(pack_half2(sum[0] * inverse, sum[1] * inverse), pack_half2(sum[2] * inverse, sum[3] * inverse),
                                             pack_half2(sum[4] * inverse, sum[5] * inverse), pack_half2(sum[6] * inverse, sum[7] * inverse));
             *reinterpret_cast<uint4*>(row) = packed;
         } else {
-            const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
             const uint64_t row = (static_cast<uint64_t>(at.batch) * p.q_tokens + at.token) * p.q_heads + at.head;
-            const uint64_t place_in_slot = (pass.first_slot + split) * rows + row;
+            const uint64_t place_in_slot = scratch_row(p, here, kTileRows, r, row);
             float4* const out = reinterpret_cast<float4*>(p.part_o + place_in_slot * p.dim + d);
             out[0] = make_float4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
             out[1] = make_float4(sum[4] * inverse, sum[5] * inverse, sum[6] * inverse, sum[7] * inverse);
@@ -529,13 +522,29 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
 
 // y = sum_s 2^lse_s o_s / sum_s 2^lse_s over the shares of each row, in the order of the slots. A lane takes eight
 // dimensions of a row.
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttentionParams p, uint32_t pass_index, uint32_t tile_rows) {
     wait_for_prior_kernels_then_release_next();
     const uint32_t vectors = p.dim / 8;
-    const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
+    const uint64_t rows = p.slot_rows;
     const uint64_t index = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     const uint64_t row = index / vectors;
     if (row >= rows) return;
+    uint64_t b, token;
+    uint32_t head;
+    if (p.by_row) {
+        const uint64_t position = row / p.q_heads;
+        head = static_cast<uint32_t>(row % p.q_heads);
+        b = position / p.q_tokens;
+        token = position % p.q_tokens;
+    } else {
+        const BlockPlace tile = place_block(p, (pass_index ? p.pass[0].tiles * p.pass[0].splits : 0u) + static_cast<uint32_t>(row / tile_rows));
+        const uint32_t r = tile.row_tile * tile_rows + static_cast<uint32_t>(row % tile_rows);
+        if (r >= p.pass[pass_index].rows) return;
+        const QueryRow at = locate_row(p, tile.first_member, tile.kv_head, r);
+        b = at.batch;
+        token = at.token;
+        head = at.head;
+    }
     const uint32_t d = static_cast<uint32_t>(index % vectors) * 8u;
     float2 largest = make_float2(__int_as_float(0xff800000), 0.0f);
     for (uint32_t s = 0; s < p.slots; ++s) {
@@ -554,9 +563,6 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         sum[4] = fmaf(b.x, share, sum[4]); sum[5] = fmaf(b.y, share, sum[5]); sum[6] = fmaf(b.z, share, sum[6]); sum[7] = fmaf(b.w, share, sum[7]);
     }
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-    const uint32_t head = static_cast<uint32_t>(row % p.q_heads);
-    const uint64_t position = row / p.q_heads;
-    const uint64_t b = position / p.q_tokens, token = position % p.q_tokens;
     __half* const out = p.y + b * p.y_batch + token * p.y_token + head * p.y_head + d;
     *reinterpret_cast<uint4*>(out) = make_uint4(pack_half2(sum[0] * inverse, sum[1] * inverse), pack_half2(sum[2] * inverse, sum[3] * inverse),
                                                 pack_half2(sum[4] * inverse, sum[5] * inverse), pack_half2(sum[6] * inverse, sum[7] * inverse));
@@ -571,7 +577,7 @@ cudaError_t launch_tile(const AttentionParams& params, cudaStream_t stream, bool
         if (error != cudaSuccess) return error;
     }
     uint32_t blocks = 0;
-    for (uint32_t i = 0; i < params.pass_count; ++i) blocks += params.pass[i].items;
+    for (uint32_t i = 0; i < params.pass_count; ++i) blocks += params.pass[i].tiles * params.pass[i].splits;
     return launch_behind(kernel, blocks, 32 * kWarps, bytes, stream, early_launch, params);
 }
 
@@ -595,11 +601,12 @@ cudaError_t launch_attention_rows(const AttentionParams& params, KvFormat format
     }
 }
 
-cudaError_t launch_attention_join(const AttentionParams& params, cudaStream_t stream, bool early_launch) {
-    const uint64_t threads = static_cast<uint64_t>(params.batch) * params.q_tokens * params.q_heads * (params.dim / 8);
+cudaError_t launch_attention_join(const AttentionParams& params, uint32_t tile_rows, cudaStream_t stream, bool early_launch) {
+    const uint64_t threads = params.slot_rows * (params.dim / 8);
+    const uint32_t pass = params.pass_count > 1 && params.pass[1].splits > 1 ? 1u : 0u;
     const uint64_t blocks = (threads + 127) / 128;
     if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
-    return launch_behind(attention_join_kernel, static_cast<uint32_t>(blocks), 128, 0, stream, early_launch, params);
+    return launch_behind(attention_join_kernel, static_cast<uint32_t>(blocks), 128, 0, stream, early_launch, params, pass, tile_rows);
 }
 
 }  // namespace sdxlq

@@ -83,24 +83,19 @@ __device__ __forceinline__ bool half_not_finite(uint32_t pair) {
 // The item's place and the tiles of keys that it walks over.
 template <int kDim>
 struct Item {
-    uint32_t kv_head, first_member, first_row, rows, split, slot;
+    BlockPlace here;
+    uint32_t kv_head, first_member, first_row, rows;
     uint32_t prefix_slot, prefix_length, own_length, own_seen;       // own_seen: keys that any row of the tile sees
     uint32_t least_limit;                                            // own keys that all its rows see
     uint32_t prefix_tiles, tile_begin, tile_end;
 
     __device__ __forceinline__ explicit Item(const AttentionParams& p) {
-        const bool second = p.pass_count > 1 && blockIdx.x >= p.pass[0].items;
-        const AttentionPass& pass = p.pass[second ? 1 : 0];
-        uint32_t item = blockIdx.x - (second ? p.pass[0].items : 0u);
-        const uint32_t row_tile = item % pass.row_tiles;
-        item /= pass.row_tiles;
-        split = item % pass.splits;
-        item /= pass.splits;
-        kv_head = item % p.kv_heads;
-        first_member = item / p.kv_heads * pass.members;
-        first_row = row_tile * kTileRows;
+        here = place_block(p, blockIdx.x);
+        const AttentionPass& pass = p.pass[here.pass];
+        kv_head = here.kv_head;
+        first_member = here.first_member;
+        first_row = here.row_tile * kTileRows;
         rows = min(kTileRows, pass.rows - first_row);
-        slot = pass.first_slot + split;
         prefix_slot = pass.with_prefix ? first_member / p.rows_per_prefix : 0u;
         prefix_length = pass.with_prefix ? length_of(p.prefix, prefix_slot) : 0u;
         own_length = own_seen = least_limit = pass.with_own ? length_of(p.own, first_member) : 0u;
@@ -110,8 +105,8 @@ struct Item {
         }
         prefix_tiles = (prefix_length + kTileKeys - 1) / kTileKeys;
         const uint64_t tiles = static_cast<uint64_t>(prefix_tiles) + (own_seen + kTileKeys - 1) / kTileKeys;
-        tile_begin = static_cast<uint32_t>(tiles * split / pass.splits);
-        tile_end = static_cast<uint32_t>(tiles * (split + 1) / pass.splits);
+        tile_begin = static_cast<uint32_t>(tiles * here.split / pass.splits);
+        tile_end = static_cast<uint32_t>(tiles * (here.split + 1) / pass.splits);
     }
 
     struct Tile {
@@ -620,7 +615,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
         } else if (warp_active) {
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
             const bool empty = tiles == 0;                               // O was never written
-            if (p.part_o == nullptr) {
+            if (writes_output(p, item.here)) {
                 // the warp's rows of Q make room for its rows of the output, which leave in whole lines
 #pragma unroll
                 for (uint32_t c = 0; c < kDim; c += 16) {
@@ -644,8 +639,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     if (r < item.rows && in_head) *reinterpret_cast<uint4*>(p.y + to + chunk * 8u) = ptx::ld_shared16(query_base + swizzled(r, chunk, kTileRows));
                 }
             } else {
-                const uint64_t rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
-                const uint64_t place = item.slot * rows + (static_cast<uint64_t>(at.batch) * p.q_tokens + at.token) * p.q_heads + at.head;
+                const uint64_t place = scratch_row(p, item.here, kTileRows, row, (static_cast<uint64_t>(at.batch) * p.q_tokens + at.token) * p.q_heads + at.head);
 #pragma unroll
                 for (uint32_t c = 0; c < kDim; c += 16) {
                     uint32_t o[16];
@@ -676,13 +670,13 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
     constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 2;
-    constexpr int kBlocks = kDim == 64 ? (kFormat == KV_F16 ? 4 : 3) : 2;
+    constexpr int kBlocks = static_cast<int>(tile_blocks_per_sm(kDim, static_cast<KvFormat>(kFormat)));
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps, kBlocks>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (error != cudaSuccess) return error;
     uint32_t blocks = 0;
-    for (uint32_t i = 0; i < params.a.pass_count; ++i) blocks += params.a.pass[i].items;
+    for (uint32_t i = 0; i < params.a.pass_count; ++i) blocks += params.a.pass[i].tiles * params.a.pass[i].splits;
     return launch_behind(kernel, blocks, 32 * (kSoftmaxWarps + 1 + kLoaderWarps), bytes, stream, early_launch, params);
 }
 

@@ -227,29 +227,53 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     } else {
         add_pass(1, with_prefix, with_own);
     }
-    // Each pass's keys are split so that the items of all passes come to about three blocks per SM of like size (two on the
-    // tensor memory), none of less than 256 (512) keys.
-    uint64_t keys[2] = {}, items[2] = {}, work = 0;
+    p.by_row = p.pass_count > 1 ? 1u : 0u;
+    uint64_t keys[2] = {}, work = 0;
     for (uint32_t i = 0; i < p.pass_count; ++i) {
         AttentionPass& pass = p.pass[i];
+        const uint64_t tiles = static_cast<uint64_t>(pass.row_tiles) * p.kv_heads * pass.groups;
+        if (tiles > kMaxExtent / 512) return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: dimensions too large");
         keys[i] = (pass.with_prefix ? p.prefix.capacity : 0ull) + (pass.with_own ? p.own.capacity : 0ull);
-        items[i] = static_cast<uint64_t>(pass.row_tiles) * p.kv_heads * pass.groups;
-        work += items[i] * keys[i];
+        pass.tiles = static_cast<uint32_t>(tiles);
+        pass.splits = 1;
+        work += tiles * keys[i];
+    }
+    const uint32_t tensor_blocks = tile_blocks_per_sm(p.dim, plan.format[0]) * static_cast<uint32_t>(sm_count);
+    if (p.pass_count == 1 && plan.row_tile[0] == kTensorTile) {
+        // Blocks of like length come in waves of `tensor_blocks`. The tiles of the last wave, where it is not full, become a
+        // pass whose keys are split until it is, into shares of no less than 256 keys.
+        const uint32_t tiles = p.pass[0].tiles, rest = tiles % tensor_blocks;
+        const uint32_t splits = rest == 0 ? 1u : static_cast<uint32_t>(std::min<uint64_t>(tensor_blocks / rest, keys[0] / 256));
+        if (splits > 1) {
+            const uint32_t last = rest == tiles ? 0u : 1u;
+            if (last == 1) {
+                p.pass[1] = p.pass[0];
+                plan.format[1] = plan.format[0];
+                plan.row_tile[1] = plan.row_tile[0];
+                p.pass[0].tiles = tiles - rest;
+                p.pass_count = 2;
+            }
+            p.pass[last].first_tile = tiles - rest;
+            p.pass[last].tiles = rest;
+            p.pass[last].splits = splits;
+        }
+    } else {
+        // Each pass's keys are split so that the blocks of all passes come to about three per SM of like size (two on the
+        // tensor memory), none of less than 256 (512) keys.
+        for (uint32_t i = 0; i < p.pass_count; ++i) {
+            const bool tensor = plan.row_tile[i] == kTensorTile;
+            const uint64_t share = std::max<uint64_t>(tensor ? 512 : 256, ceil_div(work, (tensor ? 2ull : 3ull) * sm_count));
+            p.pass[i].splits = static_cast<uint32_t>(std::clamp<uint64_t>(keys[i] / share, 1, 256));
+        }
     }
     p.slots = 0;
     for (uint32_t i = 0; i < p.pass_count; ++i) {
-        AttentionPass& pass = p.pass[i];
-        const bool tensor = plan.row_tile[i] == kTensorTile;
-        const uint64_t share = std::max<uint64_t>(tensor ? 512 : 256, ceil_div(work, (tensor ? 2ull : 3ull) * sm_count));
-        pass.splits = static_cast<uint32_t>(std::clamp<uint64_t>(keys[i] / share, 1, 256));
-        pass.first_slot = p.slots;
-        p.slots += pass.splits;
-        if (items[i] * pass.splits > kMaxExtent / 2) return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: dimensions too large");
-        pass.items = static_cast<uint32_t>(items[i] * pass.splits);
+        p.pass[i].first_slot = p.slots;
+        p.slots = p.by_row ? p.slots + p.pass[i].splits : std::max(p.slots, p.pass[i].splits);
+        if (!p.by_row && p.pass[i].splits > 1) p.slot_rows = static_cast<uint64_t>(p.pass[i].tiles) * plan.row_tile[i];
     }
-    if (p.slots > 1) {
-        plan.scratch_bytes = static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * (p.dim + 2) * sizeof(float);
-    }
+    if (p.by_row) p.slot_rows = static_cast<uint64_t>(p.batch) * p.q_tokens * p.q_heads;
+    if (p.slots > 1) plan.scratch_bytes = p.slots * p.slot_rows * (p.dim + 2) * sizeof(float);
     return SDXLQ_OK;
 }
 
@@ -293,7 +317,7 @@ int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
             return fail(ctx, SDXLQ_ERR_WORKSPACE, "attention: needs " + std::to_string(plan.scratch_bytes) + " bytes of 16-byte aligned scratch");
         }
         p.part_o = static_cast<float*>(scratch);
-        p.part_lse = reinterpret_cast<float2*>(p.part_o + static_cast<uint64_t>(p.slots) * p.batch * p.q_tokens * p.q_heads * p.dim);
+        p.part_lse = reinterpret_cast<float2*>(p.part_o + p.slots * p.slot_rows * p.dim);
     }
     const DeviceScope device(ctx);
     const bool one_launch = p.pass_count == 1 || (plan.format[0] == plan.format[1] && plan.row_tile[0] == plan.row_tile[1]);
@@ -317,7 +341,7 @@ int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
             launch(one, i);
         }
     }
-    if (error == cudaSuccess && p.slots > 1) error = launch_attention_join(p, ctx->stream, early(ctx));
+    if (error == cudaSuccess && p.slots > 1) error = launch_attention_join(p, plan.row_tile[0], ctx->stream, early(ctx));
     if (error != cudaSuccess) return fail_cuda(ctx, error, "attention launch");
     return SDXLQ_OK;
 }
