@@ -90,10 +90,8 @@ constexpr uint32_t kTileKeys = 64;       // of a tile on the tensor memory
 __host__ __device__ constexpr uint32_t tile_blocks_per_sm(uint32_t dim, KvFormat format) { return dim > 64 ? 2 : format == KV_F16 ? 4 : 3; }
 
 // Tensor maps of FP16 keys and values, [slot, token, head, d], whose box is a tile of one head (64 of its dimensions).
-// usable: the part has them (its strides can be described).
 struct AttentionMaps {
     CUtensorMap map[2][2];       // prefix, own; keys, values
-    uint32_t usable[2];
 };
 
 cudaError_t launch_attention_tiles(const AttentionParams& params, const AttentionMaps& maps, KvFormat format, uint32_t* error_word,

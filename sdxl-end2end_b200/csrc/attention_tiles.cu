@@ -2,10 +2,9 @@
 // attention.cuh for rows, passes and items, attention_rows.cu for few rows.
 //
 // A CTA takes 128 rows over its share of the keys, in tiles of 128 keys (heads of up to 64) or 64 (up to 128):
-//   loader warps   K and V tiles into a ring of four slots, as SWIZZLE_128B operands: FP16 by cp.async, which fills what
-//                  lies behind a length or behind the head's size with zeros; 8-bit caches through registers, widened to
-//                  exact halves without their scales
-//   MMA warp       S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V as it lies, MN-major)
+//   MMA warp       S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V as it lies, MN-major);
+//                  FP16 keys and values by TMA into a ring of four slots, as SWIZZLE_128B operands
+//   loader warps   (8-bit caches) the same through registers, widened to exact halves without their scales
 //   softmax warps  a thread per row: S from tensor memory, the weights back into it as halves
 // S, P and O share 256 columns, so that two CTAs work on an SM and the one's MMAs run under the other's exponentials.
 //
@@ -87,7 +86,8 @@ struct Item {
     uint32_t kv_head, first_member, first_row, rows;
     uint32_t prefix_slot, prefix_length, own_length, own_seen;       // own_seen: keys that any row of the tile sees
     uint32_t least_limit;                                            // own keys that all its rows see
-    uint32_t prefix_tiles, tile_begin, tile_end;
+    uint32_t prefix_tiles, odd_prefix_tile, odd_own_tiles;           // the odd tile of the prefix; the first odd one of the rest
+    uint32_t tile_begin, tile_end;
 
     __device__ __forceinline__ explicit Item(const AttentionParams& p) {
         here = place_block(p, blockIdx.x);
@@ -104,10 +104,19 @@ struct Item {
             least_limit = causal_limit(own_length, p.q_tokens, first_row / p.repeat);
         }
         prefix_tiles = (prefix_length + kTileKeys - 1) / kTileKeys;
-        const uint64_t tiles = static_cast<uint64_t>(prefix_tiles) + (own_seen + kTileKeys - 1) / kTileKeys;
-        tile_begin = static_cast<uint32_t>(tiles * here.split / pass.splits);
-        tile_end = static_cast<uint32_t>(tiles * (here.split + 1) / pass.splits);
+        odd_prefix_tile = prefix_length % kTileKeys != 0 ? prefix_tiles - 1 : ~0u;
+        odd_own_tiles = prefix_tiles + least_limit / kTileKeys;
+        tile_begin = 0;
+        tile_end = prefix_tiles + (own_seen + kTileKeys - 1) / kTileKeys;
+        if (pass.splits != 1) {
+            const uint64_t tiles = tile_end;
+            tile_begin = static_cast<uint32_t>(tiles * here.split / pass.splits);
+            tile_end = static_cast<uint32_t>(tiles * (here.split + 1) / pass.splits);
+        }
     }
+
+    // Every row sees every key of the tile.
+    __device__ __forceinline__ bool ordinary(uint32_t index) const { return index != odd_prefix_tile && index < odd_own_tiles; }
 
     struct Tile {
         bool in_prefix;
@@ -144,9 +153,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
         ptx::mbar_init(ptx::smem_u32(&control.value_done), 1);
         ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
-        for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kLoaderWarps);
+        for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kScaled ? kLoaderWarps : 1);
         for (uint32_t s = 0; s < kSlots; ++s) {
-            ptx::mbar_init(ptx::smem_u32(&control.full[s]), kLoaderWarps);
+            ptx::mbar_init(ptx::smem_u32(&control.full[s]), kScaled ? kLoaderWarps : 1);
             ptx::mbar_init(ptx::smem_u32(&control.empty[s]), 1);
         }
         control.abort = 0;
@@ -190,41 +199,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             return (unit % 2 == 0 ? view.k : view.v) + slot * view.slot_stride + item.kv_head * view.head_stride +
                    static_cast<int64_t>(t.first) * view.token_stride;
         };
-        if constexpr (!kScaled) {
-            static_assert(kLoaderWarps == 1);
-            bool ok = true;
-            for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
-                if (!slot_free(unit)) { ok = false; break; }
-                typename Item<kDim>::Tile t;
-                const uint8_t* const base = source(unit, t);
-                const uint32_t to = slots_base + unit % kSlots * S::kTileBytes, bar = full + unit % kSlots * 8u;
-                const uint32_t part = t.in_prefix ? 0u : 1u;
-                if (t.first + kTileKeys <= t.end && params.maps.usable[part]) {
-                    if (ptx::elect_one()) {
-                        const uint32_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
-                        ptx::mbar_expect_tx(bar, S::kTileBytes);
-#pragma unroll
-                        for (uint32_t d = 0; d < kDim; d += 64) {
-                            ptx::tma_load_4d(to + d * (kTileKeys * 2), &params.maps.map[part][unit % 2], bar, static_cast<int32_t>(d),
-                                             static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(slot));
-                        }
-                    }
-                    __syncwarp();
-                } else {
-                    // the end of a part: what lies behind it (and within its memory) has to be zeros
-                    const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
-                    for (uint32_t i = lane; i < t.columns * (kDim / 8); i += 32) {
-                        const uint32_t key = i / (kDim / 8), chunk = i % (kDim / 8);
-                        const bool inside = chunk * 8u < p.dim && t.first + key < t.end;
-                        ptx::cp_async16(to + swizzled(key, chunk, kTileKeys), inside ? base + key * stride + chunk * 16u : base, inside);
-                    }
-                    ptx::cp_async_commit();
-                    ptx::cp_async_wait<0>();
-                    announce(unit);
-                }
-            }
-            if (!ok) give_up(DEV_TIMEOUT_PRODUCER);
-        } else {
+        if constexpr (kScaled) {
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
             constexpr uint32_t kRounds = kTileKeys / kStep;
@@ -293,7 +268,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             }
         }
     } else if (warp == kSoftmaxWarps) {
-        // ---------------------------------------- MMA issuer ----------------------------------------
+        // ------------------------- MMA issuer, and the loads of FP16 keys and values -------------------------
         const uint32_t full = ptx::smem_u32(&control.full[0]), empty = ptx::smem_u32(&control.empty[0]);
         const auto wait = [&](const uint64_t& bar, uint32_t parity) {
             return ptx::warp_wait_bounded(ptx::smem_u32(&bar), parity, abort_word, limit);
@@ -314,11 +289,33 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     ptx::umma_stage_f16(tmem, query_lo + part * (kTileRows * 128 / 16), b + part * (kTileKeys * 128 / 16),
                                         ptx::kUmmaDescHiSw128, idesc, part);
                 }
-                ptx::umma_commit(empty + slot * 8u);
+                if (kScaled) ptx::umma_commit(empty + slot * 8u);
                 ptx::umma_commit(ptx::smem_u32(&control.score_ready));
             }
             __syncwarp();
         };
+        uint32_t loaded = 0;                                             // tiles whose K and V are on their way (FP16)
+        const auto load_tile = [&] {
+            if (kScaled || loaded == tiles) return;
+            const typename Item<kDim>::Tile t = item.tile(item.tile_begin + loaded);
+            if (ptx::elect_one()) {
+                const uint32_t part = t.in_prefix ? 0u : 1u, sequence = t.in_prefix ? item.prefix_slot : item.first_member;
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    const uint32_t slot = (2 * loaded + i) % kSlots, to = slots_base + slot * S::kTileBytes, bar = full + slot * 8u;
+                    ptx::mbar_expect_tx(bar, S::kTileBytes);
+#pragma unroll
+                    for (uint32_t d = 0; d < kDim; d += 64) {
+                        ptx::tma_load_4d(to + d * (kTileKeys * 2), &params.maps.map[part][i], bar, static_cast<int32_t>(d),
+                                         static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(sequence));
+                    }
+                }
+            }
+            __syncwarp();
+            ++loaded;
+        };
+        load_tile();
+        load_tile();
         bool ok = tiles == 0 || (wait(control.query_ready, 0) && wait_full(0));
         ptx::tc_fence_after();
         if (ok && tiles != 0) multiply_scores(0);
@@ -343,14 +340,17 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                         }
                     }
                 }
-                ptx::umma_commit(empty + slot * 8u);
+                if (kScaled) ptx::umma_commit(empty + slot * 8u);
                 ptx::umma_commit(ptx::smem_u32(&control.value_done));
             }
             __syncwarp();
             if (j + 1 < tiles) {
                 ok = wait(control.value_done, j & 1u);                   // P has been read: S may take its place
                 ptx::tc_fence_after();
-                if (ok) multiply_scores(j + 1);
+                if (ok) {
+                    multiply_scores(j + 1);
+                    load_tile();                                         // into the slots of tile j, whose products are done
+                }
             }
         }
         if (!ok) {
@@ -359,6 +359,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             __syncwarp();
             uint32_t never = 0;
             ptx::mbar_wait_bounded(ptx::smem_u32(&control.drained), 0, &never, limit);
+            for (uint32_t unit = 2 * loaded > kSlots ? 2 * loaded - kSlots : 0; unit < 2 * loaded; ++unit) {
+                ptx::mbar_wait_bounded(full + (unit % kSlots) * 8u, (unit / kSlots) & 1u, &never, limit);
+            }
         }
     } else {
         // ---------------------------------------- softmax ----------------------------------------
@@ -410,12 +413,17 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
         uint32_t votes = 0;
         bool ok = true;
         for (uint32_t j = 0; j < tiles; ++j) {
-            const typename Item<kDim>::Tile t = item.tile(item.tile_begin + j);
-            const uint32_t seen_by_all = t.in_prefix ? item.prefix_length : item.least_limit;
-            const bool masked = t.first + kTileKeys > seen_by_all;
-            const bool ragged = p.causal && !t.in_prefix && masked;      // rows differ in what they see of the tile
-            const uint32_t seen = t.in_prefix ? item.prefix_length : own_limit;
-            const uint32_t visible = seen > t.first ? min(seen - t.first, kTileKeys) : 0u;       // columns that this row sees
+            const bool masked = !item.ordinary(item.tile_begin + j);
+            uint32_t columns = kTileKeys, visible = kTileKeys, values = kTileKeys;       // of the tile; that this row sees; that exist
+            bool ragged = false;                                         // rows differ in what they see of the tile
+            if (masked) {
+                const typename Item<kDim>::Tile t = item.tile(item.tile_begin + j);
+                const uint32_t seen = t.in_prefix ? item.prefix_length : own_limit;
+                columns = t.columns;
+                values = min(t.end - t.first, kTileKeys);
+                visible = seen > t.first ? min(seen - t.first, kTileKeys) : 0u;
+                ragged = p.causal && !t.in_prefix;
+            }
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
             if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
@@ -423,7 +431,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             if (!ok) break;
             ptx::tc_fence_after();
 
-            const uint32_t chunks = (t.columns + 31u) / 32u;
             // Scores in units of log2, less the reference. The fused multiply-add rounds the difference alone, so that it is as
             // exact for large scores as for small ones.
             const auto key_scale = [&](uint32_t column) {
@@ -501,7 +508,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
                     value_bits = log2_approx(top);
                 }
-                const bool both = t.columns > 32u;
+                const bool both = columns > 32u;
                 uint32_t s[32];
                 float largest = kNone;
                 const auto find_largest = [&](auto careful) {
@@ -559,8 +566,20 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             }
             ptx::tmem_st_wait();
 
+            // What lies behind the end of a part, within the MMA's last 16 keys, was loaded as it is: zeros take its place, since
+            // 0 * v is not 0 for every v. (Loader warps put zeros there themselves.)
+            if (!kScaled && values < columns) {
+                const uint32_t unit = 2 * j + 1, base = slots_base + (unit % kSlots) * S::kTileBytes;
+                ok = wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
+                if (!ok) break;
+                for (uint32_t i = threadIdx.x; i < (columns - values) * (kDim / 8); i += 32 * kSoftmaxWarps) {
+                    ptx::st_shared16(base + swizzled(values + i / (kDim / 8), i % (kDim / 8), kTileKeys), make_uint4(0u, 0u, 0u, 0u));
+                }
+                ptx::fence_proxy_async();
+            }
+
             // A value that is not finite makes 0 * v a NaN, also in rows that the causal mask hides it from (what lies behind
-            // a length was loaded as zeros). Tiles that such a mask divides are looked through, and one that holds such a value
+            // a length is zeros by now). Tiles that such a mask divides are looked through, and one that holds such a value
             // is multiplied here, row by row over the keys that the row sees.
             if (kFormat != KV_INT8 && ragged) {
                 const uint32_t unit = 2 * j + 1, base = slots_base + (unit % kSlots) * S::kTileBytes;
@@ -568,7 +587,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 ok = wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
                 if (!ok) break;
                 bool found = false;
-                for (uint32_t i = threadIdx.x; i < t.columns * (kDim / 8); i += 32 * kSoftmaxWarps) {
+                for (uint32_t i = threadIdx.x; i < columns * (kDim / 8); i += 32 * kSoftmaxWarps) {
                     const uint4 x = ptx::ld_shared16(base + swizzled(i / (kDim / 8), i % (kDim / 8), kTileKeys));
                     found = found || half_not_finite(x.x) || half_not_finite(x.y) || half_not_finite(x.z) || half_not_finite(x.w);
                 }
@@ -585,7 +604,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                         float total[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) total[i] = j == 0 ? 0.0f : __uint_as_float(o[i]);
-                        for (uint32_t key = 0; key < t.columns; ++key) {
+                        for (uint32_t key = 0; key < columns; ++key) {
                             uint32_t pair;
                             ptx::tmem_ld_32x32b_x1(my_tmem + key / 32 * 32 + key % 32 / 2, pair);
                             ptx::tmem_ld_wait(pair);
@@ -669,7 +688,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
-    constexpr int kLoaderWarps = kFormat == KV_F16 ? 1 : 2;
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : 2;
     constexpr int kBlocks = static_cast<int>(tile_blocks_per_sm(kDim, static_cast<KvFormat>(kFormat)));
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps, kBlocks>;

@@ -128,10 +128,18 @@ uint64_t ceil_div(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
 // Rows of a tile of the kernel that takes passes of so many rows: attention_rows.cu's with 16 or (heads of up to 64) 32, or
 // attention_tiles.cu's with 128.
 constexpr uint32_t kTensorTile = 128;
-uint32_t row_tile_for(uint64_t rows, uint32_t dim) {
-    if (rows <= 16) return 16;
-    if (rows <= 32) return dim <= 64 ? 32 : 16;
-    return kTensorTile;
+uint32_t row_tile_for(uint64_t rows, uint32_t dim, bool tensor) {
+    if (tensor && rows > 32) return kTensorTile;
+    return rows > 16 && dim <= 64 ? 32 : 16;
+}
+
+// Whether tensor maps can describe a part's strides. An extent of 1 may have any.
+bool describable(const sdxlq_kv_cache& c) {
+    const uint64_t extent[3] = {c.heads, c.capacity, c.slots}, stride[3] = {c.head_stride, c.token_stride, c.slot_stride};
+    for (int axis = 0; axis < 3; ++axis) {
+        if (extent[axis] > 1 && (stride[axis] == 0 || stride[axis] * 2 >= uint64_t(1) << 40)) return false;
+    }
+    return true;
 }
 
 // A call's passes, and what its launches need.
@@ -202,11 +210,13 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     // Rows of the entries that share a prefix are taken together over it where that saves more than the join of the two
     // parts costs, which is about the time of four tiles of 128 keys for every tile of rows; a part that is of another
     // type has to be a pass of its own.
+    const bool tensor = (!with_prefix || d.prefix.dtype != SDXLQ_FP16 || describable(d.prefix)) &&
+                        (!with_own || d.own.dtype != SDXLQ_FP16 || describable(d.own));
     bool fold = false;
     if (with_prefix) {
         const uint64_t rows = entry_rows * p.rows_per_prefix;
-        const uint64_t together = ceil_div(rows, row_tile_for(rows, p.dim));
-        const uint64_t apart = p.rows_per_prefix * ceil_div(entry_rows, row_tile_for(entry_rows, p.dim));
+        const uint64_t together = ceil_div(rows, row_tile_for(rows, p.dim, tensor));
+        const uint64_t apart = p.rows_per_prefix * ceil_div(entry_rows, row_tile_for(entry_rows, p.dim, tensor));
         fold = (with_own && d.prefix.dtype != d.own.dtype) ||
                (together < apart && (!with_own || (apart - together) * ceil_div(p.prefix.capacity, 128) > 4 * apart));
     }
@@ -216,7 +226,7 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
         pass.groups = p.batch / members;
         pass.rows = static_cast<uint32_t>(members * entry_rows);
         plan.format[p.pass_count] = static_cast<KvFormat>(prefix ? d.prefix.dtype : d.own.dtype);
-        plan.row_tile[p.pass_count] = row_tile_for(pass.rows, p.dim);
+        plan.row_tile[p.pass_count] = row_tile_for(pass.rows, p.dim, tensor);
         pass.row_tiles = static_cast<uint32_t>(ceil_div(pass.rows, plan.row_tile[p.pass_count++]));
         pass.with_prefix = prefix ? 1u : 0u;
         pass.with_own = own ? 1u : 0u;
@@ -261,8 +271,8 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
         // Each pass's keys are split so that the blocks of all passes come to about three per SM of like size (two on the
         // tensor memory), none of less than 256 (512) keys.
         for (uint32_t i = 0; i < p.pass_count; ++i) {
-            const bool tensor = plan.row_tile[i] == kTensorTile;
-            const uint64_t share = std::max<uint64_t>(tensor ? 512 : 256, ceil_div(work, (tensor ? 2ull : 3ull) * sm_count));
+            const bool on_tensor = plan.row_tile[i] == kTensorTile;
+            const uint64_t share = std::max<uint64_t>(on_tensor ? 512 : 256, ceil_div(work, (on_tensor ? 2ull : 3ull) * sm_count));
             p.pass[i].splits = static_cast<uint32_t>(std::clamp<uint64_t>(keys[i] / share, 1, 256));
         }
     }
@@ -277,29 +287,25 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     return SDXLQ_OK;
 }
 
-// FP16 parts get tensor maps where their strides can be described; an entry of extent 1 may have any stride.
-AttentionMaps encode_maps(const sdxlq_context* ctx, const sdxlq_attention_desc& d) {
-    AttentionMaps maps{};
+// The FP16 parts' tensor maps.
+bool encode_maps(const sdxlq_context* ctx, const sdxlq_attention_desc& d, AttentionMaps& maps) {
     for (int i = 0; i < 2; ++i) {
         const sdxlq_kv_cache& c = i == 0 ? d.prefix : d.own;
-        if (absent(c) || c.dtype != SDXLQ_FP16 || c.capacity < kTileKeys || ctx->encode == nullptr) continue;
+        if (absent(c) || c.dtype != SDXLQ_FP16 || c.capacity == 0) continue;
         const cuuint64_t extent[4] = {c.head_dim, c.heads, c.capacity, c.slots};
         const uint64_t stride[3] = {c.head_stride, c.token_stride, c.slot_stride};
         cuuint64_t bytes[3];
-        bool describable = true;
-        for (int axis = 0; axis < 3; ++axis) {
-            bytes[axis] = extent[axis + 1] == 1 ? 16 : stride[axis] * 2;
-            describable = describable && bytes[axis] != 0 && bytes[axis] < uint64_t(1) << 40;
-        }
+        for (int axis = 0; axis < 3; ++axis) bytes[axis] = extent[axis + 1] == 1 ? 16 : stride[axis] * 2;
         const cuuint32_t box[4] = {64, 1, kTileKeys, 1}, step[4] = {1, 1, 1, 1};
-        for (int part = 0; part < 2 && describable; ++part) {
-            describable = ctx->encode(&maps.map[i][part], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, part == 0 ? c.k : c.v, extent, bytes, box, step,
-                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        for (int part = 0; part < 2; ++part) {
+            if (ctx->encode(&maps.map[i][part], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, part == 0 ? c.k : c.v, extent, bytes, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+                return false;
+            }
         }
-        maps.usable[i] = describable ? 1u : 0u;
     }
-    return maps;
+    return true;
 }
 
 int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
@@ -324,7 +330,9 @@ int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
     LaunchTimer timer(ctx, SDXLQ_KERNEL_HARNESS, (one_launch ? 1 : 2) + (p.slots > 1 ? 1 : 0));
     cudaError_t error = cudaSuccess;
     AttentionMaps maps{};
-    if (plan.row_tile[0] == kTensorTile || plan.row_tile[1] == kTensorTile) maps = encode_maps(ctx, d);
+    if ((plan.row_tile[0] == kTensorTile || plan.row_tile[1] == kTensorTile) && !encode_maps(ctx, d, maps)) {
+        return fail(ctx, SDXLQ_ERR_CUDA, "attention: the driver refused a tensor map");
+    }
     const auto launch = [&](const AttentionParams& params, uint32_t pass) {
         if (error != cudaSuccess) return;
         error = plan.row_tile[pass] == kTensorTile
