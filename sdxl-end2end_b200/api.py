@@ -238,7 +238,8 @@ def load_library() -> ctypes.CDLL:
 
 _front = None
 _FRONT_FUNCTIONS = ("sdxlq_linear", "sdxlq_linear_grouped", "sdxlq_layer_norm", "sdxlq_quantize_act_int8",
-                    "sdxlq_quantize_act_fp8", "sdxlq_pack_weight_int8", "sdxlq_pack_weight_fp8")
+                    "sdxlq_quantize_act_fp8", "sdxlq_pack_weight_int8", "sdxlq_pack_weight_fp8", "sdxlq_kv_cache_write",
+                    "sdxlq_kv_cache_read", "sdxlq_shared_prefix_attention", "sdxlq_shared_prefix_attention_scratch")
 
 
 class _PythonPath:
@@ -248,7 +249,7 @@ class _PythonPath:
     def linear(*arguments):
         return None
 
-    linear_grouped = layer_norm = quantize_int8 = quantize_fp8 = pack_fp8 = linear
+    linear_grouped = layer_norm = quantize_int8 = quantize_fp8 = pack_fp8 = kv_write = kv_read = attention = linear
 
 
 def load_front():
@@ -765,6 +766,9 @@ class Ops:
         own (INT8: max / 127; FP8: a power of two). Row r goes to slot first_slot + r, from token positions[r] on (an int: the
         same for all rows; None: 0); with `counts`, only its first counts[r] tokens. Tokens whose place lies outside the
         slot are not written, and what is not written stays as it was."""
+        done = self._front.kv_write(self.ctx.address, self.ctx.device, cache, key, value, positions, counts, first_slot)
+        if done is not None:
+            return None if done is True else self.ctx.raise_for(done)
         tokens = self._kv_tokens("kv_cache_write", cache, key, value, positions, counts, first_slot)
         if any(cache.k.stride(i) == 0 and cache.k.shape[i] > 1 for i in range(4)):
             raise CudaError("kv_cache_write: the cache's tokens overlap in memory")
@@ -775,6 +779,9 @@ class Ops:
                       rows: Optional[int] = None, first_slot: int = 0) -> tuple:
         """(key, value): FP16 [rows, tokens, heads, head_dim], the inverse of kv_cache_write up to its rounding. Rows default
         to all slots from first_slot on. Tokens that kv_cache_write would not have written are zeros."""
+        pair = self._front.kv_read(self.ctx.address, self.ctx.device, cache, tokens, positions, counts, rows, first_slot, self.poison_outputs)
+        if pair is not None:
+            return pair if pair.__class__ is not int else self.ctx.raise_for(pair)
         rows = cache.slots - first_slot if rows is None else rows
         if rows < 0 or tokens < 0:
             raise CudaError("kv_cache_read: negative extent")
@@ -806,6 +813,10 @@ class Ops:
         q_heads is a multiple of the key heads, and key head h serves the query heads h * n .. h * n + n - 1. The parts may be of
         unlike types. What lies behind a length or is hidden by the causal mask takes no part, whatever it holds, and a query
         that sees no key gives zeros. `out` may be `query`."""
+        y = self._front.attention(self.ctx.address, self.ctx.device, self.ctx.stream_address, query, own, prefix, own_lengths, prefix_lengths,
+                                  causal, scale, out, self.poison_outputs)
+        if y is not None:
+            return y if y.__class__ is not int else self.ctx.raise_for(y)
         if query.dtype != torch.float16 or query.dim() != 4 or (query.shape[3] > 1 and query.stride(3) != 1):
             raise CudaError("attention: expects FP16 queries [batch, tokens, q_heads, head_dim], a head's elements together")
         y = out

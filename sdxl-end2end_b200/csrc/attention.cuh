@@ -43,6 +43,23 @@ cudaError_t launch_kv_write(const KvCopyLaunch& launch, cudaStream_t stream, boo
 cudaError_t launch_kv_read(const KvCopyLaunch& launch, cudaStream_t stream, bool early_launch);
 
 // ---- attention ------------------------------------------------------------------------------------------
+
+// Division of n < 2^31 by a number known at the launch, as a multiplication (Granlund and Montgomery, PLDI 1994).
+struct Divider {
+    uint32_t divisor, magic, shift;
+    void set(uint32_t d) {
+        divisor = d;
+        for (shift = 0; (uint64_t(1) << shift) < d; ++shift) {}
+        magic = static_cast<uint32_t>((((uint64_t(1) << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
+    __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t& rest) const {
+        const uint32_t q = quotient(n);
+        rest = n - q * divisor;
+        return q;
+    }
+};
+
 // Query rows of one key head are numbered r = (member * q_tokens + token) * repeat + head within the key head's group:
 // rows of several batch entries that read the same keys stand behind one another.
 //
@@ -57,6 +74,7 @@ struct AttentionPass {
     uint32_t rows;               // members * q_tokens * repeat
     uint32_t row_tiles, splits;
     uint32_t first_tile, tiles;  // of row_tiles * kv_heads * groups
+    Divider by_tiles, by_row_tiles;
     uint32_t first_slot;         // by_row: scratch slot of split 0
     uint32_t with_prefix, with_own;
 };
@@ -70,6 +88,7 @@ struct AttentionParams {
     KvView prefix, own;
     uint32_t batch, q_tokens, q_heads, kv_heads, repeat, dim;
     uint32_t rows_per_prefix;    // batch entries that share a prefix
+    Divider by_q_tokens, by_repeat, by_kv_heads, by_rows_per_prefix;
     uint32_t causal;
     float scale_log2;            // softmax scale * log2(e)
     uint32_t pass_count;
@@ -111,13 +130,9 @@ __device__ __forceinline__ BlockPlace place_block(const AttentionParams& p, uint
     at.pass = p.pass_count > 1 && block >= first ? 1u : 0u;
     const AttentionPass& pass = p.pass[at.pass];
     block -= at.pass ? first : 0u;
-    at.split = block / pass.tiles;
-    at.tile = block % pass.tiles;
-    uint32_t tile = pass.first_tile + at.tile;
-    at.row_tile = tile % pass.row_tiles;
-    tile /= pass.row_tiles;
-    at.kv_head = tile % p.kv_heads;
-    at.first_member = tile / p.kv_heads * pass.members;
+    at.split = pass.by_tiles.quotient(block, at.tile);
+    const uint32_t tile = pass.by_row_tiles.quotient(pass.first_tile + at.tile, at.row_tile);
+    at.first_member = p.by_kv_heads.quotient(tile, at.kv_head) * pass.members;
     return at;
 }
 
@@ -136,8 +151,9 @@ struct QueryRow {
 };
 
 __device__ __forceinline__ QueryRow locate_row(const AttentionParams& p, uint32_t first_member, uint32_t kv_head, uint32_t r) {
-    const uint32_t head = r % p.repeat, position = r / p.repeat;
-    return {first_member + position / p.q_tokens, position % p.q_tokens, kv_head * p.repeat + head};
+    uint32_t head, token;
+    const uint32_t member = p.by_q_tokens.quotient(p.by_repeat.quotient(r, head), token);
+    return {first_member + member, token, kv_head * p.repeat + head};
 }
 
 __device__ __forceinline__ uint32_t length_of(const KvView& view, uint32_t slot) {

@@ -175,11 +175,11 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
     const uint32_t kv_head = here.kv_head, first_member = here.first_member, first_row = here.row_tile * kTileRows;
 
     // the keys of the block: blocks of the prefix, then of the entry's own keys
-    const uint32_t prefix_slot = pass.with_prefix ? first_member / p.rows_per_prefix : 0u;
+    const uint32_t prefix_slot = pass.with_prefix ? p.by_rows_per_prefix.quotient(first_member) : 0u;
     const uint32_t prefix_length = pass.with_prefix ? length_of(p.prefix, prefix_slot) : 0u;
     const uint32_t own_length = pass.with_own ? length_of(p.own, first_member) : 0u;
     const uint32_t last_row = min(first_row + kTileRows, pass.rows) - 1u;        // sees the most of its entry's own keys
-    const uint32_t own_seen = p.causal && pass.with_own ? causal_limit(own_length, p.q_tokens, last_row / p.repeat) : own_length;
+    const uint32_t own_seen = p.causal && pass.with_own ? causal_limit(own_length, p.q_tokens, p.by_repeat.quotient(last_row)) : own_length;
     const uint32_t prefix_blocks = (prefix_length + kKeys - 1) / kKeys, own_blocks = (own_seen + kKeys - 1) / kKeys;
     const uint64_t blocks = static_cast<uint64_t>(prefix_blocks) + own_blocks;
     const uint32_t block_begin = static_cast<uint32_t>(blocks * here.split / pass.splits);

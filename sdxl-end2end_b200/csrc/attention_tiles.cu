@@ -31,6 +31,7 @@ constexpr uint32_t kSlots = 4;                   // K0 V0 K1 V1
 constexpr uint32_t kScaleRing = 4;               // key tiles whose scales are held
 constexpr uint32_t kSoftmaxWarps = 4;
 constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
+constexpr uint32_t kPolynomialGroups = 0x88;      // of the eight groups of four columns in 32, those whose 2^x is a polynomial
 
 // Tensor-memory columns of a CTA: S and, in its place, P (the weights of 32 keys in the first 16 columns of their
 // scores), then O. Shared memory: Q and the ring of slots.
@@ -68,11 +69,28 @@ __device__ __forceinline__ float log2_approx(float x) {
     return y;
 }
 
-// The largest of three (max.f32 takes three operands on sm_100).
+// The largest of three, NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+
+// 2^x for finite x up to 126 (below -126 it is 2^-126) on the FMA pipe: x = n + f with n the nearest integer, left in the low
+// bits of x + 1.5 * 2^23, and 2^f by the degree-4 polynomial of least relative error on [-1/2, 1/2] (2.7e-6, found by
+// reweighted least squares on Chebyshev nodes), whose exponent n is added to.
+__device__ __forceinline__ float2 exp2_polynomial(float2 x) {
+    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    const float2 shifted = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f));
+    const float2 whole = __fadd2_rn(shifted, make_float2(-12582912.0f, -12582912.0f));
+    const float2 f = __ffma2_rn(whole, make_float2(-1.0f, -1.0f), x);
+    float2 y = make_float2(0.009570101276040077f, 0.009570101276040077f);
+    y = __ffma2_rn(y, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    y = __ffma2_rn(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    y = __ffma2_rn(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    y = __ffma2_rn(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(shifted.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(shifted.y) << 23)));
 }
 
 __device__ __forceinline__ bool half_not_finite(uint32_t pair) {
@@ -96,12 +114,12 @@ struct Item {
         first_member = here.first_member;
         first_row = here.row_tile * kTileRows;
         rows = min(kTileRows, pass.rows - first_row);
-        prefix_slot = pass.with_prefix ? first_member / p.rows_per_prefix : 0u;
+        prefix_slot = pass.with_prefix ? p.by_rows_per_prefix.quotient(first_member) : 0u;
         prefix_length = pass.with_prefix ? length_of(p.prefix, prefix_slot) : 0u;
         own_length = own_seen = least_limit = pass.with_own ? length_of(p.own, first_member) : 0u;
         if (p.causal && pass.with_own) {
-            own_seen = causal_limit(own_length, p.q_tokens, (first_row + rows - 1) / p.repeat);
-            least_limit = causal_limit(own_length, p.q_tokens, first_row / p.repeat);
+            own_seen = causal_limit(own_length, p.q_tokens, p.by_repeat.quotient(first_row + rows - 1));
+            least_limit = causal_limit(own_length, p.q_tokens, p.by_repeat.quotient(first_row));
         }
         prefix_tiles = (prefix_length + kTileKeys - 1) / kTileKeys;
         odd_prefix_tile = prefix_length % kTileKeys != 0 ? prefix_tiles - 1 : ~0u;
@@ -386,7 +404,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             // a negative softmax scale turns the queries' signs, so that scores are multiplied by its magnitude
             const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
             const int64_t offset = at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head;
-            constexpr uint32_t kBatch = 4;
+            constexpr uint32_t kBatch = 8;
 #pragma unroll
             for (uint32_t first = 0; first < 32; first += kBatch * kRowsAtOnce) {
                 uint4 x[kBatch];
@@ -458,7 +476,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     largest = max3(largest, x[0], x[1]);
                     other = max3(other, x[2], x[3]);
                 }
-                return fmaxf(largest, other);
+                return max3(largest, other, other);
             };
             // the weights of 32 columns: into P, and into the row's sum
             const auto weigh = [&](auto careful_case, uint32_t c, const uint32_t (&s)[32], float shift, float2 (&part)[2]) {
@@ -478,10 +496,15 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] -= fine;
                     }
+                    if (!careful && (kPolynomialGroups >> (i / 4) & 1) != 0) {
+                        const float2 a = exp2_polynomial(lo), b = exp2_polynomial(hi);
+                        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (careful) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
-                        x[e] = exp2_approx(x[e]);
+                        for (int e = 0; e < 4; ++e) {
+                            if (careful) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
+                            x[e] = exp2_approx(x[e]);
+                        }
                     }
                     part[0] = __fadd2_rn(part[0], make_float2(x[0], x[1]));
                     part[1] = __fadd2_rn(part[1], make_float2(x[2], x[3]));
@@ -527,7 +550,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 const float base = first ? largest * unit : reference;
                 const float over = fmaf(largest, unit, -base) - fine + value_bits - kWeightBits;
                 const bool moves = first || over > kSlackBits;
-                if (__any_sync(0xffffffffu, moves)) {
+                bool special = false;                                    // a NaN among the tile's scores
+                if (__any_sync(0xffffffffu, moves || largest != largest)) {
+                    special = __any_sync(0xffffffffu, largest != largest);
                     float grow = 1.0f;
                     if (moves) {
                         // the last bit of a reference past 2^22 is coarser than the weights' room: what it rounds off is kept too
@@ -560,7 +585,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     }
                     weigh(careful, 0, s, shift, part);
                 };
-                if (masked || huge) take_weights(std::true_type{});
+                if (masked || huge || special) take_weights(std::true_type{});
                 else take_weights(std::false_type{});
                 sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
             }
@@ -651,7 +676,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 }
                 __syncwarp();
                 const int64_t offset = at.batch * p.y_batch + at.token * p.y_token + at.head * p.y_head;
-#pragma unroll 4
+#pragma unroll 8
                 for (uint32_t i = 0; i < 32; i += kRowsAtOnce) {
                     const uint32_t r = first_of_warp + i;
                     const int64_t to = __shfl_sync(0xffffffffu, offset, r & 31u);

@@ -277,7 +277,13 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
         }
     }
     p.slots = 0;
+    p.by_q_tokens.set(p.q_tokens);
+    p.by_repeat.set(p.repeat);
+    p.by_kv_heads.set(p.kv_heads);
+    p.by_rows_per_prefix.set(p.rows_per_prefix);
     for (uint32_t i = 0; i < p.pass_count; ++i) {
+        p.pass[i].by_tiles.set(p.pass[i].tiles);
+        p.pass[i].by_row_tiles.set(p.pass[i].row_tiles);
         p.pass[i].first_slot = p.slots;
         p.slots = p.by_row ? p.slots + p.pass[i].splits : std::max(p.slots, p.pass[i].splits);
         if (!p.by_row && p.pass[i].splits > 1) p.slot_rows = static_cast<uint64_t>(p.pass[i].tiles) * plan.row_tile[i];

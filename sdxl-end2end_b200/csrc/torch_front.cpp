@@ -22,6 +22,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -38,11 +39,16 @@ int (*g_quantize_int8)(sdxlq_context*, const void*, int32_t, uint64_t, uint64_t,
 int (*g_quantize_fp8)(sdxlq_context*, const void*, uint64_t, int32_t, uint8_t*, float*) = nullptr;
 int (*g_pack_int8)(sdxlq_context*, const void*, int32_t, uint64_t, uint64_t, uint32_t, int8_t*, float*) = nullptr;
 int (*g_pack_fp8)(sdxlq_context*, const void*, int32_t, uint64_t, uint64_t, int32_t, int32_t, int32_t, uint8_t*, float*) = nullptr;
+int (*g_kv_write)(sdxlq_context*, const sdxlq_kv_cache*, const sdxlq_kv_tokens*) = nullptr;
+int (*g_kv_read)(sdxlq_context*, const sdxlq_kv_cache*, const sdxlq_kv_tokens*) = nullptr;
+int (*g_attention)(sdxlq_context*, const sdxlq_attention_desc*) = nullptr;
+size_t (*g_attention_scratch)(const sdxlq_context*, const sdxlq_attention_desc*) = nullptr;
 
-// Attribute names of Weight and LinearCall, interned once.
+// Attribute names of Weight, LinearCall and KVCache, interned once.
 struct Names {
     PyObject *data, *type, *n, *k, *scales, *scale_mode, *layout, *convrot_group_size;
     PyObject *x, *weight, *bias, *activation, *y, *xq, *xq_scales, *acc_out, *residual, *y_amax, *x_amax;
+    PyObject *cache_k, *cache_v, *k_scales, *v_scales;
 } g_names;
 
 sdxlq_context* context_of(PyObject* handle) {
@@ -401,11 +407,232 @@ PyObject* pack_fp8(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return status == SDXLQ_OK ? pair_of(packed, scales) : PyLong_FromLong(status);
 }
 
+// ---- kv cache and attention ---------------------------------------------------------------------------
+
+// A rank-4 tensor on `device` whose last dimension lies together: what keys, values, queries and outputs are.
+bool heads_of(PyObject* object, int64_t device, at::ScalarType type) {
+    if (!ordinary(object)) return false;
+    const at::Tensor& t = THPVariable_Unpack(object);
+    return t.scalar_type() == type && t.dim() == 4 && t.device().index() == device && (t.size(3) <= 1 || t.stride(3) == 1);
+}
+
+// The strides of the first three dimensions; that of a dimension of one is never used. False where one is negative.
+bool strides_of(const at::Tensor& t, uint64_t& a, uint64_t& b, uint64_t& c) {
+    uint64_t* const out[3] = {&a, &b, &c};
+    for (int i = 0; i < 3; ++i) {
+        if (t.stride(i) < 0) return false;
+        *out[i] = t.size(i) == 1 ? 0 : static_cast<uint64_t>(t.stride(i));
+    }
+    return true;
+}
+
+bool overlaps(const at::Tensor& t) {
+    for (int i = 0; i < 4; ++i) {
+        if (t.stride(i) == 0 && t.size(i) > 1) return true;
+    }
+    return false;
+}
+
+at::ScalarType kv_type(uint64_t type) {
+    switch (type) {
+    case SDXLQ_FP8_E4M3: return at::kFloat8_e4m3fn;
+    case SDXLQ_FP8_E5M2: return at::kFloat8_e5m2;
+    case SDXLQ_INT8: return at::kChar;
+    default: return at::kHalf;
+    }
+}
+
+// A KVCache object, whose constructor has made its checks; `write`: its memory is written.
+bool read_cache(PyObject* object, int64_t device, bool write, sdxlq_kv_cache& c) {
+    uint64_t type;
+    if (!Attribute(object, g_names.type).integer(type) || type > SDXLQ_FP16) return false;
+    const Attribute k(object, g_names.cache_k), v(object, g_names.cache_v), k_scales(object, g_names.k_scales), v_scales(object, g_names.v_scales);
+    const at::ScalarType element = kv_type(type);
+    if (!heads_of(k.get(), device, element) || !heads_of(v.get(), device, element)) return false;
+    const at::Tensor& keys = THPVariable_Unpack(k.get());
+    const at::Tensor& values = THPVariable_Unpack(v.get());
+    if (keys.sizes() != values.sizes() || (write && (overlaps(keys) || overlaps(values)))) return false;
+    uint64_t slot, token, head;
+    if (!strides_of(keys, c.slot_stride, c.token_stride, c.head_stride) || !strides_of(values, slot, token, head) || slot != c.slot_stride ||
+        token != c.token_stride || head != c.head_stride) {
+        return false;
+    }
+    void* scale[2] = {};
+    PyObject* const scales[2] = {k_scales.get(), v_scales.get()};
+    for (int i = 0; i < 2; ++i) {
+        if (type == SDXLQ_FP16) {
+            if (scales[i] == nullptr || !is_none(scales[i])) return false;
+            continue;
+        }
+        if (!ordinary(scales[i])) return false;
+        const at::Tensor& t = THPVariable_Unpack(scales[i]);
+        if (t.scalar_type() != at::kFloat || !t.is_contiguous() || t.dim() != 3 || t.device().index() != device || t.size(0) != keys.size(0) ||
+            t.size(1) != keys.size(2) || t.size(2) != keys.size(1)) {
+            return false;
+        }
+        scale[i] = write ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
+    }
+    c.k = write ? keys.mutable_data_ptr() : const_cast<void*>(keys.const_data_ptr());
+    c.v = write ? values.mutable_data_ptr() : const_cast<void*>(values.const_data_ptr());
+    c.k_scales = static_cast<float*>(scale[0]);
+    c.v_scales = static_cast<float*>(scale[1]);
+    c.slots = static_cast<uint64_t>(keys.size(0));
+    c.capacity = static_cast<uint64_t>(keys.size(1));
+    c.heads = static_cast<uint64_t>(keys.size(2));
+    c.head_dim = static_cast<uint64_t>(keys.size(3));
+    c.dtype = static_cast<int32_t>(type);
+    c.reserved = 0;
+    return true;
+}
+
+// None, or a contiguous INT32 vector of `count` on `device`.
+bool int32_vector(PyObject* object, int64_t device, int64_t count, const int32_t*& out) {
+    out = nullptr;
+    if (is_none(object)) return true;
+    if (!ordinary(object)) return false;
+    const at::Tensor& t = THPVariable_Unpack(object);
+    if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != count || !t.is_contiguous() || t.device().index() != device) return false;
+    out = static_cast<const int32_t*>(t.const_data_ptr());
+    return true;
+}
+
+// The tokens' places: `positions` may be an integer.
+bool place_tokens(PyObject* positions, PyObject* counts, PyObject* first_slot, int64_t device, sdxlq_kv_tokens& t) {
+    int64_t number = 0;
+    if (PyLong_Check(positions)) {
+        if (!small_integer(positions, number) || number < 0) return false;
+        t.start = static_cast<uint64_t>(number);
+    } else if (!int32_vector(positions, device, static_cast<int64_t>(t.rows), t.positions)) {
+        return false;
+    }
+    if (!int32_vector(counts, device, static_cast<int64_t>(t.rows), t.counts) || !small_integer(first_slot, number) || number < 0) return false;
+    t.first_slot = static_cast<uint64_t>(number);
+    return true;
+}
+
+// kv_write(handle, device, cache, key, value, positions, counts, first_slot): True
+PyObject* kv_write(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    int64_t device;
+    sdxlq_kv_cache cache;
+    if (count != 8 || !small_integer(args[1], device) || !read_cache(args[2], device, true, cache) ||
+        !heads_of(args[3], device, at::kHalf) || !heads_of(args[4], device, at::kHalf)) {
+        Py_RETURN_NONE;
+    }
+    const at::Tensor& key = THPVariable_Unpack(args[3]);
+    const at::Tensor& value = THPVariable_Unpack(args[4]);
+    sdxlq_kv_tokens t{};
+    uint64_t row, token, head;
+    if (key.sizes() != value.sizes() || static_cast<uint64_t>(key.size(2)) != cache.heads || static_cast<uint64_t>(key.size(3)) != cache.head_dim ||
+        !strides_of(key, t.row_stride, t.token_stride, t.head_stride) || !strides_of(value, row, token, head) || row != t.row_stride ||
+        token != t.token_stride || head != t.head_stride) {
+        Py_RETURN_NONE;
+    }
+    t.rows = static_cast<uint64_t>(key.size(0));
+    t.tokens = static_cast<uint64_t>(key.size(1));
+    t.k = const_cast<void*>(key.const_data_ptr());
+    t.v = const_cast<void*>(value.const_data_ptr());
+    if (!place_tokens(args[5], args[6], args[7], device, t)) Py_RETURN_NONE;
+    const int status = unlocked(g_kv_write, context_of(args[0]), &cache, &t);
+    if (status != SDXLQ_OK) return PyLong_FromLong(status);
+    Py_RETURN_TRUE;
+}
+
+// kv_read(handle, device, cache, tokens, positions, counts, rows, first_slot, poison): (key, value)
+PyObject* kv_read(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    int64_t device, tokens, rows, first_slot;
+    sdxlq_kv_cache cache;
+    if (count != 9 || !small_integer(args[1], device) || !read_cache(args[2], device, false, cache) || !small_integer(args[3], tokens) ||
+        tokens < 0 || !small_integer(args[7], first_slot)) {
+        Py_RETURN_NONE;
+    }
+    if (is_none(args[6])) rows = static_cast<int64_t>(cache.slots) - first_slot;
+    else if (!small_integer(args[6], rows)) Py_RETURN_NONE;
+    if (rows < 0) Py_RETURN_NONE;
+    sdxlq_kv_tokens t{};
+    t.rows = static_cast<uint64_t>(rows);
+    t.tokens = static_cast<uint64_t>(tokens);
+    if (!place_tokens(args[4], args[5], args[7], device, t)) Py_RETURN_NONE;
+    const Attribute k(args[2], g_names.cache_k);
+    const at::Tensor& like = THPVariable_Unpack(k.get());
+    const int64_t sizes[4] = {rows, tokens, static_cast<int64_t>(cache.heads), static_cast<int64_t>(cache.head_dim)};
+    at::Tensor key = empty(sizes, at::kHalf, like), value = empty(sizes, at::kHalf, like);
+    if (args[8] == Py_True) {
+        key.fill_(std::numeric_limits<double>::quiet_NaN());
+        value.fill_(std::numeric_limits<double>::quiet_NaN());
+    }
+    if (!strides_of(key, t.row_stride, t.token_stride, t.head_stride)) Py_RETURN_NONE;
+    t.k = key.mutable_data_ptr();
+    t.v = value.mutable_data_ptr();
+    const int status = unlocked(g_kv_read, context_of(args[0]), &cache, &t);
+    return status == SDXLQ_OK ? pair_of(key, value) : PyLong_FromLong(status);
+}
+
+// attention(handle, device, stream, query, own, prefix, own_lengths, prefix_lengths, causal, scale, out, poison): the output
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    int64_t device;
+    sdxlq_attention_desc d{};
+    if (count != 12 || !small_integer(args[1], device) || !heads_of(args[3], device, at::kHalf)) Py_RETURN_NONE;
+    // the scratch belongs to the stream that the kernels run on, which the Python path sees to where it is not the current one
+    void* const stream = PyLong_AsVoidPtr(args[2]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream() != stream) Py_RETURN_NONE;
+    const at::Tensor& query = THPVariable_Unpack(args[3]);
+    d.batch = static_cast<uint64_t>(query.size(0));
+    d.q_tokens = static_cast<uint64_t>(query.size(1));
+    d.q_heads = static_cast<uint64_t>(query.size(2));
+    d.head_dim = static_cast<uint64_t>(query.size(3));
+    const struct { PyObject *part, *lengths; sdxlq_kv_cache& cache; const int32_t*& out; } parts[2] = {
+        {args[4], args[6], d.own, d.own_lengths}, {args[5], args[7], d.prefix, d.prefix_lengths}};
+    for (const auto& part : parts) {
+        if (is_none(part.part)) {
+            if (!is_none(part.lengths)) Py_RETURN_NONE;
+            continue;
+        }
+        if (!read_cache(part.part, device, false, part.cache) || (part.cache.slots == 0 && d.batch > 0) ||
+            !int32_vector(part.lengths, device, static_cast<int64_t>(part.cache.slots), part.out)) {
+            Py_RETURN_NONE;
+        }
+    }
+    if (!PyBool_Check(args[8])) Py_RETURN_NONE;
+    d.causal = args[8] == Py_True;
+    if (is_none(args[9])) {
+        d.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(d.head_dim == 0 ? 1 : d.head_dim)));
+    } else {
+        const double scale = PyFloat_AsDouble(args[9]);
+        if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+        d.scale = static_cast<float>(scale);
+    }
+    d.q = query.const_data_ptr();
+    if (!strides_of(query, d.q_batch_stride, d.q_token_stride, d.q_head_stride)) Py_RETURN_NONE;
+    at::Tensor allocated;
+    if (is_none(args[10])) {
+        allocated = empty(query.sizes(), at::kHalf, query);
+        if (args[11] == Py_True) allocated.fill_(std::numeric_limits<double>::quiet_NaN());
+        d.y = allocated.mutable_data_ptr();
+        if (!strides_of(allocated, d.y_batch_stride, d.y_token_stride, d.y_head_stride)) Py_RETURN_NONE;
+    } else {
+        if (!heads_of(args[10], device, at::kHalf)) Py_RETURN_NONE;
+        const at::Tensor& out = THPVariable_Unpack(args[10]);
+        if (out.sizes() != query.sizes() || overlaps(out) || !strides_of(out, d.y_batch_stride, d.y_token_stride, d.y_head_stride)) Py_RETURN_NONE;
+        d.y = out.mutable_data_ptr();
+    }
+    sdxlq_context* const context = context_of(args[0]);
+    at::Tensor scratch;
+    const size_t needed = g_attention_scratch(context, &d);
+    if (needed != 0) {
+        scratch = empty({static_cast<int64_t>(needed)}, at::kByte, query);
+        d.scratch = scratch.mutable_data_ptr();
+        d.scratch_bytes = needed;
+    }
+    return answer(unlocked(g_attention, context, &d), tensor_or(args[10], allocated));
+}
+
 // bind(addresses): the C ABI's functions, in the order below.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
-    void* addresses[7];
-    if (count != 7) { PyErr_SetString(PyExc_ValueError, "bind wants seven addresses"); return nullptr; }
-    for (int i = 0; i < 7; ++i) {
+    constexpr int kFunctions = 11;
+    void* addresses[kFunctions];
+    if (count != kFunctions) { PyErr_SetString(PyExc_ValueError, "bind wants eleven addresses"); return nullptr; }
+    for (int i = 0; i < kFunctions; ++i) {
         addresses[i] = PyLong_AsVoidPtr(args[i]);
         if (addresses[i] == nullptr) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null function address");
@@ -419,6 +646,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
     g_quantize_fp8 = reinterpret_cast<decltype(g_quantize_fp8)>(addresses[4]);
     g_pack_int8 = reinterpret_cast<decltype(g_pack_int8)>(addresses[5]);
     g_pack_fp8 = reinterpret_cast<decltype(g_pack_fp8)>(addresses[6]);
+    g_kv_write = reinterpret_cast<decltype(g_kv_write)>(addresses[7]);
+    g_kv_read = reinterpret_cast<decltype(g_kv_read)>(addresses[8]);
+    g_attention = reinterpret_cast<decltype(g_attention)>(addresses[9]);
+    g_attention_scratch = reinterpret_cast<decltype(g_attention_scratch)>(addresses[10]);
     Py_RETURN_NONE;
 }
 
@@ -440,6 +671,9 @@ PyMethodDef g_methods[] = {
     {"quantize_int8", entry<quantize_int8>(), METH_FASTCALL, nullptr},
     {"quantize_fp8", entry<quantize_fp8>(), METH_FASTCALL, nullptr},
     {"pack_fp8", entry<pack_fp8>(), METH_FASTCALL, nullptr},
+    {"kv_write", entry<kv_write>(), METH_FASTCALL, nullptr},
+    {"kv_read", entry<kv_read>(), METH_FASTCALL, nullptr},
+    {"attention", entry<attention>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -454,7 +688,8 @@ PyMODINIT_FUNC PyInit__front() {
         {&g_names.scale_mode, "scale_mode"}, {&g_names.layout, "layout"}, {&g_names.convrot_group_size, "convrot_group_size"},
         {&g_names.x, "x"}, {&g_names.weight, "weight"}, {&g_names.bias, "bias"}, {&g_names.activation, "activation"},
         {&g_names.y, "y"}, {&g_names.xq, "xq"}, {&g_names.xq_scales, "xq_scales"}, {&g_names.acc_out, "acc_out"},
-        {&g_names.residual, "residual"}, {&g_names.y_amax, "y_amax"}, {&g_names.x_amax, "x_amax"}};
+        {&g_names.residual, "residual"}, {&g_names.y_amax, "y_amax"}, {&g_names.x_amax, "x_amax"},
+        {&g_names.cache_k, "k"}, {&g_names.cache_v, "v"}, {&g_names.k_scales, "k_scales"}, {&g_names.v_scales, "v_scales"}};
     for (const auto& name : names) {
         *name.slot = PyUnicode_InternFromString(name.text);
         if (*name.slot == nullptr) return nullptr;

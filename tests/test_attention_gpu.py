@@ -322,11 +322,12 @@ def test_layouts(gpu, queries):
     assert torch.equal(wide[..., :8], normal(41, batch, heads, queries, dim + 24)[..., :8])
     # one prefix seen through a stride of zero is the same as a prefix of its own for each entry
     expanded = pkg.KVCache(prefix.k[:1].expand(4, -1, -1, -1), prefix.v[:1].expand(4, -1, -1, -1))
-    a = ops.shared_prefix_attention(k[:, :7].contiguous(), expanded)
-    b = ops.shared_prefix_attention(k[:, :7].contiguous(), None, pkg.KVCache(prefix.k[:1], prefix.v[:1]))
-    context.check()
-    want, bound = R.attention(k[:, :7], None, (prefix.k[:1].double(), prefix.v[:1].double()))
-    assert R.off(a, want, bound) <= 1.0 and R.off(b, want, bound) <= 1.0
+    for n in (7, 90):
+        a = ops.shared_prefix_attention(k[:, :n].contiguous(), expanded)
+        b = ops.shared_prefix_attention(k[:, :n].contiguous(), None, pkg.KVCache(prefix.k[:1], prefix.v[:1]))
+        context.check()
+        want, bound = R.attention(k[:, :n], None, (prefix.k[:1].double(), prefix.v[:1].double()))
+        assert R.off(a, want, bound) <= 1.0 and R.off(b, want, bound) <= 1.0
 
 
 def test_empty_calls(gpu):
@@ -365,6 +366,43 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(back[0], R.values_of(kq, ks).half()) and torch.equal(back[1], R.values_of(vq, vs).half())
     want, bound = R.attention(q, (R.values_of(kq, ks), R.values_of(vq, vs)), None)
     assert R.off(y, want, bound) <= 1.0
+
+
+class NoFront:
+    """Answers None to everything: the Python path runs."""
+
+    def __getattr__(self, name):
+        return lambda *arguments: None
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("queries", [1, 50])
+def test_front_and_python_path_agree(gpu, dtype, queries):
+    pkg, context, ops = gpu
+    slow = pkg.Ops(context, poison_outputs=True)
+    slow._front = NoFront()
+    k, v, q = normal(95, 3, 40, 2, 64), normal(96, 3, 40, 2, 64), normal(97, 6, queries, 4, 64)
+    own, _ = cache_of(pkg, normal(98, 6, 30, 2, 64), normal(99, 6, 30, 2, 64), dtype)
+    results = []
+    for o in (ops, slow):
+        cache = o.kv_cache(4, 64, 2, 64, scalar_type(pkg, dtype))
+        assert o.kv_cache_write(cache, k, v, positions=int32([0, 5, 40]), counts=int32([40, 3, 40]), first_slot=1) is None
+        prefix = pkg.KVCache(cache.k[1:], cache.v[1:], cache.type, *(None if s is None else s[1:] for s in (cache.k_scales, cache.v_scales)))
+        out = [cache.k.float(), cache.v.float(), *o.kv_cache_read(cache, 20, positions=3), *o.kv_cache_read(cache, 9, int32([1, 60]), int32([9, 2]), 2, 1)]
+        given = torch.empty_like(q)
+        out += [o.shared_prefix_attention(q, own, prefix, own_lengths=int32([30, 0, 1, 7, 30, 2]), prefix_lengths=int32([64, 8, 0]), causal=True),
+                o.shared_prefix_attention(q, None, prefix, scale=0.3), o.shared_prefix_attention(q, own, scale=1, out=given)]
+        assert out[-1] is given
+        results.append(out)
+    context.check()
+    for fast, plain in zip(*results):
+        assert fast.shape == plain.shape and fast.dtype == plain.dtype and torch.equal(fast, plain)
+    with pytest.raises(pkg.CudaError, match="slot per batch entry"):       # found by the library behind the front
+        ops.shared_prefix_attention(q[:4], own)
+    with pytest.raises(pkg.CudaError, match="behind the capacity"):
+        ops.kv_cache_read(own, 31)
+    with pytest.raises(pkg.CudaError, match="more rows than slots"):
+        ops.kv_cache_write(own, normal(1, 7, 3, 2, 64), normal(2, 7, 3, 2, 64))
 
 
 # ---- a run of them, streams and graphs ---------------------------------------------------------------------

@@ -189,7 +189,7 @@ def test_cache_objects_check_their_tensors(pkg):
 
 class NoContext:
     """Stands in for a context: nothing here may reach the library."""
-    device = 0
+    device = address = stream_address = 0
     _lib = None
     _front = None
 
