@@ -9,7 +9,8 @@ package's operator: `Ops.linear`, `Ops.linear_activation`, small grouped calls f
 share an input, a per-generation plan for the cross-attention K/V projections. The operators that
 are not projections (convolution, GroupNorm, LayerNorm, attention, upsample, the CFG combine and
 the Euler update) are plain PyTorch FP16 calls: they are scaffolding around the path, not part of
-it. Weights are random-initialised, seeded per tensor name.
+it. Attention can go through the package too (`attention="shared_prefix"`): images of one prompt then share one
+text context, and its keys and values can be kept in 8 bits for the whole generation. Weights are random-initialised, seeded per tensor name.
 
 Data layout: spatial tensors are NCHW in channels-last memory, so that the token view
 [B, H*W, C] the projections read and write is the same storage (the reference's flatten_spatial /
@@ -26,7 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from .api import (ACT_GEGLU, ACT_NONE, ACT_SILU, CudaError, FP8ScaleMode, FP8WeightLoadOptions,
-                  INT8WeightLoadOptions, LinearCall, Ops, ScalarType, Weight)
+                  INT8WeightLoadOptions, KVCache, LinearCall, Ops, ScalarType, Weight)
 
 
 @dataclass(frozen=True)
@@ -227,6 +228,9 @@ def sinusoidal_embedding(values: torch.Tensor, dimension: int) -> torch.Tensor:
 # --------------------------------------------------------------------------------------------
 # the executor
 # --------------------------------------------------------------------------------------------
+_KV_TYPES = {"f16": ScalarType.Float16, "int8": ScalarType.Int8, "e4m3": ScalarType.Float8E4M3, "e5m2": ScalarType.Float8E5M2}
+
+
 class UNetHarness:
     """UNet::forward of the reference's CUDA executor (src/cuda/unet.cpp:183-310) with this
     package's operator behind every projection.
@@ -240,12 +244,18 @@ class UNetHarness:
     PyTorch layer_norm calls and the projections quantise their input themselves.
     `fuse_group_norm` runs GroupNorm (+ SiLU, + the resnet's time-embedding bias in front of norm2) on the
     channels-last activations through the library's scaffolding kernel instead of PyTorch's group_norm,
-    which copies a channels-last tensor to NCHW and back around the norm."""
+    which copies a channels-last tensor to NCHW and back around the norm.
+    `attention` "library" is PyTorch's; "shared_prefix" is Ops.shared_prefix_attention, with the text context as the prefix:
+    prepare_conditioning then also takes fewer rows than the batch has, one for every batch / rows consecutive entries
+    (all images of a prompt), and `kv_cache` ("int8", "e4m3", "e5m2", or "f16": as projected) is the type in which the context's
+    keys and values are kept from step to step."""
 
     def __init__(self, ops: Ops, config: UNetConfig = BASE_1_0, precision: str = "e4m3", seed: int = 0,
                  parameters: Optional[Dict[str, torch.Tensor]] = None, fuse_residual: bool = True,
                  group_attention_inputs: bool = True, device: Optional[torch.device] = None,
-                 fuse_layer_norm: bool = True, fuse_group_norm: bool = True):
+                 fuse_layer_norm: bool = True, fuse_group_norm: bool = True, attention: str = "library", kv_cache: str = "f16"):
+        if attention not in ("library", "shared_prefix") or kv_cache not in _KV_TYPES or (attention == "library" and kv_cache != "f16"):
+            raise CudaError(f"unknown attention {attention} with a {kv_cache} cache")
         if precision not in ("e4m3", "e5m2", "int8", "f16"):
             raise CudaError(f"unknown precision profile {precision}")
         self.ops = ops
@@ -255,6 +265,8 @@ class UNetHarness:
         self.group_attention_inputs = group_attention_inputs
         self.fuse_layer_norm = fuse_layer_norm
         self.fuse_group_norm = fuse_group_norm
+        self.shared_prefix = attention == "shared_prefix"
+        self.kv_type = _KV_TYPES[kv_cache]
         self.device = device if device is not None else torch.device("cuda", ops.ctx.device)
         source = parameters if parameters is not None else synthetic_parameters(config, self.device, seed)
         self.projections: Dict[str, Weight] = {}
@@ -280,6 +292,7 @@ class UNetHarness:
         self._amax_word = torch.zeros(1, dtype=torch.int32, device=self.device)    # zero between uses: the reader clears it
         self.projection_calls = 0          # projections issued by the last forward (K/V cache included)
         self._kv: Dict[str, torch.Tensor] = {}
+        self._kv_caches: Dict[str, KVCache] = {}       # of the blocks' cross-attention (shared_prefix)
         self._kv_plan = None
         self._kv_source: Optional[torch.Tensor] = None
         self._temb_plan = None
@@ -362,6 +375,33 @@ class UNetHarness:
         out = F.scaled_dot_product_attention(q, k, v)
         return out.transpose(1, 2).reshape(batch, tokens, channels).contiguous()
 
+    def _self_attention(self, query, key, value, heads):
+        if not self.shared_prefix:
+            return self._attention(query, key, value, heads)
+        own = KVCache.of(key, value, heads)
+        return self.ops.shared_prefix_attention(query.unflatten(2, (heads, -1)), own).flatten(2)
+
+    def _cross_attention(self, query, block, heads):
+        if not self.shared_prefix:
+            return self._attention(query, self._kv[f"{block}.attn2.to_k"], self._kv[f"{block}.attn2.to_v"], heads)
+        return self.ops.shared_prefix_attention(query.unflatten(2, (heads, -1)), None, self._kv_caches[block]).flatten(2)
+
+    def _fill_kv_caches(self) -> None:
+        """The context's keys and values as attention reads them: where they were projected (FP16), or quantised."""
+        for name, key in self._kv.items():
+            if not self.shared_prefix or not name.endswith(".attn2.to_k"):
+                continue
+            block = name[: -len(".attn2.to_k")]
+            value = self._kv[f"{block}.attn2.to_v"]
+            heads = self.config.heads[self.config.channels.index(key.shape[2])]
+            projected = KVCache.of(key, value, heads)
+            if self.kv_type == ScalarType.Float16:
+                self._kv_caches[block] = projected
+                continue
+            if block not in self._kv_caches:
+                self._kv_caches[block] = self.ops.kv_cache(key.shape[0], key.shape[1], heads, projected.head_dim, self.kv_type)
+            self.ops.kv_cache_write(self._kv_caches[block], projected.k, projected.v)
+
     # -- per-generation work: cross-attention K/V of every block ----------------------------------------
     def prepare_conditioning(self, encoder_hidden_states: torch.Tensor) -> None:
         """All attn2.to_k / attn2.to_v projections of the UNet in one grouped launch. Their input, the
@@ -374,6 +414,7 @@ class UNetHarness:
         if self._kv_plan is not None and self._kv_source is not None and self._kv_source.shape == source.shape:
             self._kv_source.copy_(source)
             self._kv_plan.run()
+            self._fill_kv_caches()
             return
         if self._kv_plan is not None:
             self._kv_plan.close()
@@ -382,6 +423,8 @@ class UNetHarness:
         calls = [LinearCall(self._kv_source, self.projections[name]) for name in names]
         self._kv_plan = self.ops.plan(calls)
         self._kv = dict(zip(names, self._kv_plan.run()))
+        self._kv_caches = {}
+        self._fill_kv_caches()
 
     # -- UNet::build_time_embedding + the 17 time_emb_proj ---------------------------------------------
     def _time_embedding(self, timestep: torch.Tensor, batch: int, pooled: torch.Tensor, time_ids: torch.Tensor):
@@ -439,13 +482,12 @@ class UNetHarness:
             self.projection_calls += 3
         else:
             query, key, value = (self._linear(normalized, name, bias=False) for name in names)
-        attention = self._attention(query, key, value, heads)
+        attention = self._self_attention(query, key, value, heads)
         hidden = self._linear(attention, f"{prefix}.attn1.to_out.0", residual=hidden, out=hidden)
 
         normalized = self._layer_norm(hidden, f"{prefix}.norm2", f"{prefix}.attn2.to_q")
         query = self._linear(normalized, f"{prefix}.attn2.to_q", bias=False)
-        key, value = self._kv[f"{prefix}.attn2.to_k"], self._kv[f"{prefix}.attn2.to_v"]
-        attention = self._attention(query, key, value, heads)
+        attention = self._cross_attention(query, prefix, heads)
         hidden = self._linear(attention, f"{prefix}.attn2.to_out.0", residual=hidden, out=hidden)
 
         normalized = self._layer_norm(hidden, f"{prefix}.norm3", f"{prefix}.ff.net.0.proj")
@@ -470,6 +512,10 @@ class UNetHarness:
         hidden = self._linear(hidden, f"{prefix}.proj_out", residual=skip)                     # + add_in_place(hidden, input)
         return hidden.view(batch, height, width, channels).permute(0, 3, 1, 2)                 # unflatten_spatial
 
+    def _conditions(self, rows: int, batch: int) -> bool:
+        """Whether so many rows of text states serve the batch: one for each entry, or for as many consecutive ones."""
+        return rows == batch or (self.shared_prefix and 0 < rows and batch % rows == 0)
+
     # -- UNet::forward --------------------------------------------------------------------------------
     def forward(self, latent_sample: torch.Tensor, timestep, pooled_text_embeds: torch.Tensor,
                 time_ids: torch.Tensor) -> torch.Tensor:
@@ -482,7 +528,7 @@ class UNetHarness:
             raise CudaError("CUDA UNet input shape mismatch")
         batch = latent_sample.shape[0]
         if pooled_text_embeds.shape[0] != batch or time_ids.shape[0] != batch or \
-                self._kv_source is None or self._kv_source.shape[0] != batch:
+                self._kv_source is None or not self._conditions(self._kv_source.shape[0], batch):
             raise CudaError("CUDA UNet conditioning batch mismatch")
         self._follow_current_stream()
         self.projection_calls = len(self._kv)          # the cached K/V projections belong to the forward
@@ -571,7 +617,8 @@ class EulerDenoiser:
         self.step_index = 0
 
     def set_conditioning(self, prompt_embeds: torch.Tensor, pooled: torch.Tensor, time_ids: torch.Tensor) -> None:
-        """prompt_embeds FP16 [2 * images, 77, cross_dim] laid out [uncond x images | cond x images]."""
+        """prompt_embeds FP16 [2 * images, 77, cross_dim] laid out [uncond x images | cond x images]; with shared-prefix
+        attention also [2 * prompts, ..]: each row serves images / prompts consecutive images."""
         self.unet._follow_current_stream()
         self.unet.prepare_conditioning(prompt_embeds)
         self.pooled.copy_(pooled)
