@@ -21,6 +21,7 @@
 #include "ptx.cuh"
 
 #include <type_traits>
+#include <utility>
 
 namespace sdxlq {
 
@@ -221,14 +222,17 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
             constexpr uint32_t kRounds = kTileKeys / kStep;
+            constexpr uint32_t kAhead = kDim == 64 ? 2 : 4;
             static_assert(kStep % 8 == 0 && kTileKeys % kStep == 0);
             const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
             const bool in_head = chunk * 16u < p.dim;
             const uint32_t target0 = swizzled(first_key, 2u * chunk, kTileKeys), target1 = swizzled(first_key, 2u * chunk + 1u, kTileKeys);
-            uint4 ahead[kRounds];
+            // kAhead tiles of K or V are on their way to the registers at a time
+            uint4 ahead[kAhead][kRounds];
             constexpr uint32_t kScales = (kTileKeys + kThreads - 1) / kThreads;      // of a thread
-            float ahead_scale[kScales][2] = {};
-            const auto fetch = [&](uint32_t unit) {
+            float ahead_scale[kAhead / 2][kScales][2] = {};
+            const auto fetch = [&](uint32_t unit, auto buffer) {
+                constexpr uint32_t kBuffer = decltype(buffer)::value;
                 typename Item<kDim>::Tile t;
                 const uint8_t* const base = source(unit, t);
                 const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
@@ -236,9 +240,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 #pragma unroll
                 for (uint32_t i = 0; i < kRounds; ++i, from += kStep * stride) {
                     const bool inside = in_head && t.first + first_key + i * kStep < t.end;
-                    ahead[i] = inside ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+                    ahead[kBuffer][i] = inside ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
                 }
-                if (unit % 2 == 0) {
+                if constexpr (kBuffer % 2 == 0) {
                     const KvView& view = t.in_prefix ? p.prefix : p.own;
                     const int64_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
                     const int64_t at = (slot * p.kv_heads + item.kv_head) * view.capacity + t.first;
@@ -246,44 +250,58 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     for (uint32_t i = 0; i < kScales; ++i) {
                         const uint32_t key = i * kThreads + thread;
                         const bool inside = key < kTileKeys && t.first + key < t.end;
-                        ahead_scale[i][0] = inside ? __ldg(view.k_scales + at + key) * fabsf(p.scale_log2) : 0.0f;
-                        ahead_scale[i][1] = inside ? __ldg(view.v_scales + at + key) : 0.0f;
+                        ahead_scale[kBuffer / 2][i][0] = inside ? __ldg(view.k_scales + at + key) * fabsf(p.scale_log2) : 0.0f;
+                        ahead_scale[kBuffer / 2][i][1] = inside ? __ldg(view.v_scales + at + key) : 0.0f;
                     }
                 }
             };
-            if (tiles != 0) fetch(0);
-            for (uint32_t unit = 0; unit < 2 * tiles; ++unit) {
-                if (!slot_free(unit)) {
-                    give_up(DEV_TIMEOUT_PRODUCER);
-                    break;
-                }
+            const auto put = [&](uint32_t unit, auto buffer) {
+                constexpr uint32_t kBuffer = decltype(buffer)::value;
+                if (!slot_free(unit)) return false;
                 uint32_t to = slots_base + (unit % kSlots) * S::kTileBytes;
 #pragma unroll
                 for (uint32_t i = 0; i < kRounds; ++i, to += kStep * 128u) {
-                    const uint2 a = widen4<kFormat>(ahead[i].x), b = widen4<kFormat>(ahead[i].y), c = widen4<kFormat>(ahead[i].z),
-                                d = widen4<kFormat>(ahead[i].w);
+                    const uint4 x = ahead[kBuffer][i];
+                    const uint2 a = widen4<kFormat>(x.x), b = widen4<kFormat>(x.y), c = widen4<kFormat>(x.z), d = widen4<kFormat>(x.w);
                     ptx::st_shared16(to + target0, make_uint4(a.x, a.y, b.x, b.y));
                     ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
                 }
                 // The ring of scales is longer than its writer can be ahead of its readers: this tile's slot was freed by the
                 // MMA of the tile two before it, and that had waited for the weights of the one before that.
-                if (unit % 2 == 0) {
+                if constexpr (kBuffer % 2 == 0) {
 #pragma unroll
                     for (uint32_t i = 0; i < kScales; ++i) {
                         const uint32_t key = i * kThreads + thread;
                         if (key < kTileKeys) {
-                            scales[unit / 2 % kScaleRing][0][key] = ahead_scale[i][0];
-                            scales[unit / 2 % kScaleRing][1][key] = ahead_scale[i][1];
+                            scales[unit / 2 % kScaleRing][0][key] = ahead_scale[kBuffer / 2][i][0];
+                            scales[unit / 2 % kScaleRing][1][key] = ahead_scale[kBuffer / 2][i][1];
                         }
                     }
-                }
-                if (unit % 2 == 0) {
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&control.scales_full[unit / 2 % kScaleRing]));
                 }
-                if (unit + 1 < 2 * tiles) fetch(unit + 1);
+                if (unit + kAhead < 2 * tiles) fetch(unit + kAhead, buffer);
                 announce(unit);
+                return true;
+            };
+            // buffer by buffer, each known at compile time
+            const auto each_buffer = [&](auto action) {
+                [&]<uint32_t... kBuffer>(std::integer_sequence<uint32_t, kBuffer...>) {
+                    return (action(std::integral_constant<uint32_t, kBuffer>{}) && ...);
+                }(std::make_integer_sequence<uint32_t, kAhead>{});
+            };
+            each_buffer([&](auto buffer) {
+                if (buffer.value < 2 * tiles) fetch(buffer.value, buffer);
+                return true;
+            });
+            bool ok = true;
+            for (uint32_t first = 0; ok && first < 2 * tiles; first += kAhead) {
+                each_buffer([&](auto buffer) {
+                    if (first + buffer.value < 2 * tiles) ok = put(first + buffer.value, buffer);
+                    return ok;
+                });
             }
+            if (!ok) give_up(DEV_TIMEOUT_PRODUCER);
         }
     } else if (warp == kSoftmaxWarps) {
         // ------------------------- MMA issuer, and the loads of FP16 keys and values -------------------------
@@ -713,7 +731,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
-    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : 2;
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : kDim == 64 ? 2 : 4;
     constexpr int kBlocks = static_cast<int>(tile_blocks_per_sm(kDim, static_cast<KvFormat>(kFormat)));
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps, kBlocks>;

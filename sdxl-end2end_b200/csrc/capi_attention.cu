@@ -238,7 +238,7 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
         add_pass(1, with_prefix, with_own);
     }
     p.by_row = p.pass_count > 1 ? 1u : 0u;
-    uint64_t keys[2] = {}, work = 0;
+    uint64_t keys[2] = {}, work[2] = {};
     for (uint32_t i = 0; i < p.pass_count; ++i) {
         AttentionPass& pass = p.pass[i];
         const uint64_t tiles = static_cast<uint64_t>(pass.row_tiles) * p.kv_heads * pass.groups;
@@ -246,8 +246,9 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
         keys[i] = (pass.with_prefix ? p.prefix.capacity : 0ull) + (pass.with_own ? p.own.capacity : 0ull);
         pass.tiles = static_cast<uint32_t>(tiles);
         pass.splits = 1;
-        work += tiles * keys[i];
+        work[i] = tiles * keys[i];
     }
+    const bool one_launch = p.pass_count > 1 && plan.format[0] == plan.format[1] && plan.row_tile[0] == plan.row_tile[1];
     const uint32_t tensor_blocks = tile_blocks_per_sm(p.dim, plan.format[0]) * static_cast<uint32_t>(sm_count);
     if (p.pass_count == 1 && plan.row_tile[0] == kTensorTile) {
         // Blocks of like length come in waves of `tensor_blocks`. The tiles of the last wave, where it is not full, become a
@@ -268,11 +269,12 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
             p.pass[last].splits = splits;
         }
     } else {
-        // Each pass's keys are split so that the blocks of all passes come to about three per SM of like size (two on the
-        // tensor memory), none of less than 256 (512) keys.
+        // The keys are split so that the blocks of a launch are of like size and fill the SMs once (tensor memory) or come to
+        // about three per SM, none of less than 256 keys.
         for (uint32_t i = 0; i < p.pass_count; ++i) {
-            const bool on_tensor = plan.row_tile[i] == kTensorTile;
-            const uint64_t share = std::max<uint64_t>(on_tensor ? 512 : 256, ceil_div(work, (on_tensor ? 2ull : 3ull) * sm_count));
+            const uint64_t blocks = plan.row_tile[i] == kTensorTile ? tile_blocks_per_sm(p.dim, plan.format[i]) * static_cast<uint64_t>(sm_count)
+                                                                    : 3ull * sm_count;
+            const uint64_t share = std::max<uint64_t>(256, ceil_div(one_launch ? work[0] + work[1] : work[i], blocks));
             p.pass[i].splits = static_cast<uint32_t>(std::clamp<uint64_t>(keys[i] / share, 1, 256));
         }
     }
