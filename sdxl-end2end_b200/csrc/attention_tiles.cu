@@ -35,9 +35,11 @@ constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
 constexpr uint32_t kPolynomialGroups = 0x88;      // of the eight groups of four columns in 32, those whose 2^x is a polynomial
 
 // Tensor-memory columns of a CTA: S and, in its place, P (the weights of 32 keys in the first 16 columns of their
-// scores), then O. Shared memory: Q and the ring of slots.
+// scores), for heads of 128 in two buffers (scores of the next tile under the softmax of this one), then O. Shared memory: Q
+// and the ring of slots.
 template <int kDim>
 struct Shape {
+    static constexpr uint32_t kBuffers = kDim == 64 ? 1 : 2;
     static constexpr uint32_t kColumns = kDim == 64 ? 128 : 256;
     static constexpr uint32_t kColumnO = kDim;
     static constexpr uint32_t kTileBytes = kTileKeys * kDim * 2;
@@ -45,7 +47,8 @@ struct Shape {
 };
 
 struct TileControl {
-    uint64_t query_ready, score_ready, weight_ready, value_done, vote, drained;
+    uint64_t query_ready, score_ready[2], weight_ready[2], value_done[2], vote, drained;       // [j % buffers]: a barrier's parity tells
+                                                                                             // one phase from the next only
     uint64_t full[kSlots], empty[kSlots], scales_full[kScaleRing];
     uint32_t tmem_base;
     uint32_t abort;
@@ -155,6 +158,7 @@ struct Item {
 template <int kDim, int kFormat, int kLoaderWarps, int kBlocks>
 __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBlocks) attention_tiles_kernel(const __grid_constant__ TileParams params) {
     using S = Shape<kDim>;
+    constexpr uint32_t kBuffers = S::kBuffers;
     constexpr bool kScaled = kFormat != KV_F16;
     const AttentionParams& p = params.a;
     extern __shared__ __align__(1024) uint8_t dynamic_smem[];
@@ -167,9 +171,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 
     if (threadIdx.x == 0) {
         ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&control.score_ready), 1);
-        ptx::mbar_init(ptx::smem_u32(&control.weight_ready), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&control.value_done), 1);
+        for (uint32_t b = 0; b < S::kBuffers; ++b) {
+            ptx::mbar_init(ptx::smem_u32(&control.score_ready[b]), 1);
+            ptx::mbar_init(ptx::smem_u32(&control.weight_ready[b]), kSoftmaxWarps);
+            ptx::mbar_init(ptx::smem_u32(&control.value_done[b]), 1);
+        }
         ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
         for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kScaled ? kLoaderWarps : 1);
@@ -266,8 +272,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     ptx::st_shared16(to + target0, make_uint4(a.x, a.y, b.x, b.y));
                     ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
                 }
-                // The ring of scales is longer than its writer can be ahead of its readers: this tile's slot was freed by the
-                // MMA of the tile two before it, and that had waited for the weights of the one before that.
+                // The ring of scales is as long as its writer can be ahead of its readers: this tile's slot was freed by the MMA
+                // of the tile two before it, and that had waited for the weights of the tile kBuffers before it.
+                static_assert(kScaleRing >= kSlots / 2 + kBuffers);
                 if constexpr (kBuffer % 2 == 0) {
 #pragma unroll
                     for (uint32_t i = 0; i < kScales; ++i) {
@@ -322,71 +329,73 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
 #pragma unroll
                 for (uint32_t part = 0; part < kDim / 64; ++part) {
-                    ptx::umma_stage_f16(tmem, query_lo + part * (kTileRows * 128 / 16), b + part * (kTileKeys * 128 / 16),
+                    ptx::umma_stage_f16(tmem + j % kBuffers * kTileKeys, query_lo + part * (kTileRows * 128 / 16), b + part * (kTileKeys * 128 / 16),
                                         ptx::kUmmaDescHiSw128, idesc, part);
                 }
                 if (kScaled) ptx::umma_commit(empty + slot * 8u);
-                ptx::umma_commit(ptx::smem_u32(&control.score_ready));
+                ptx::umma_commit(ptx::smem_u32(&control.score_ready[j % kBuffers]));
             }
             __syncwarp();
         };
-        uint32_t loaded = 0;                                             // tiles whose K and V are on their way (FP16)
-        const auto load_tile = [&] {
-            if (kScaled || loaded == tiles) return;
-            const typename Item<kDim>::Tile t = item.tile(item.tile_begin + loaded);
+        uint32_t loaded[2] = {0, 0};                                     // tiles of K and of V that were sent for (FP16)
+        const auto load_tile = [&](uint32_t which) {
+            if (kScaled || loaded[which] == tiles) return;
+            const uint32_t index = loaded[which]++, slot = (2 * index + which) % kSlots, bar = full + slot * 8u;
+            const typename Item<kDim>::Tile t = item.tile(item.tile_begin + index);
             if (ptx::elect_one()) {
                 const uint32_t part = t.in_prefix ? 0u : 1u, sequence = t.in_prefix ? item.prefix_slot : item.first_member;
+                ptx::mbar_expect_tx(bar, S::kTileBytes);
 #pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    const uint32_t slot = (2 * loaded + i) % kSlots, to = slots_base + slot * S::kTileBytes, bar = full + slot * 8u;
-                    ptx::mbar_expect_tx(bar, S::kTileBytes);
-#pragma unroll
-                    for (uint32_t d = 0; d < kDim; d += 64) {
-                        ptx::tma_load_4d(to + d * (kTileKeys * 2), &params.maps.map[part][i], bar, static_cast<int32_t>(d),
-                                         static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(sequence));
-                    }
+                for (uint32_t d = 0; d < kDim; d += 64) {
+                    ptx::tma_load_4d(slots_base + slot * S::kTileBytes + d * (kTileKeys * 2), &params.maps.map[part][which], bar, static_cast<int32_t>(d),
+                                     static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(sequence));
                 }
             }
             __syncwarp();
-            ++loaded;
         };
-        load_tile();
-        load_tile();
-        bool ok = tiles == 0 || (wait(control.query_ready, 0) && wait_full(0));
-        ptx::tc_fence_after();
-        if (ok && tiles != 0) multiply_scores(0);
+        for (uint32_t i = 0; i < 4; ++i) load_tile(i % 2);
+        bool ok = tiles == 0 || wait(control.query_ready, 0);
+        for (uint32_t j = 0; ok && j < min(tiles, kBuffers); ++j) {
+            ok = wait_full(2 * j);
+            ptx::tc_fence_after();
+            if (ok) multiply_scores(j);
+        }
         for (uint32_t j = 0; ok && j < tiles; ++j) {
             const uint32_t unit = 2 * j + 1, slot = unit % kSlots, columns = item.tile(item.tile_begin + j).columns;
-            ok = wait_full(unit) && (j + 1 == tiles || wait_full(unit + 1)) && wait(control.weight_ready, j & 1u);
+            const uint32_t buffer = j % kBuffers, phase = (j / kBuffers) & 1u, next = j + kBuffers;
+            if (!kScaled) {
+                ok = wait(control.score_ready[buffer], phase);           // the keys of tile j have been read: the next but one take their slot
+                if (!ok) break;
+                load_tile(0);
+            }
+            ok = wait_full(unit) && (next >= tiles || wait_full(2 * next)) && wait(control.weight_ready[buffer], phase);
             if (!ok) break;
             ptx::tc_fence_after();
             const bool skip = kFormat != KV_INT8 && p.causal && *reinterpret_cast<volatile uint32_t*>(&control.skip[j % 4]) == j + 1;
             if (ptx::elect_one()) {
-                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16);
+                const uint32_t b = slots_lo + slot * (S::kTileBytes / 16), a = tmem + buffer * kTileKeys;
 #pragma unroll
                 for (uint32_t part = 0; part < kDim / 64; ++part) {
                     const uint32_t d = tmem + S::kColumnO + part * 64, b_part = b + part * (kTileKeys * 128 / 16);
                     if (skip) break;
                     if (columns == kTileKeys) {
-                        ptx::umma_f16_ts_x4(d, tmem, b_part, ptx::kUmmaDescHiSw128, kValueIdesc, j);
+                        ptx::umma_f16_ts_x4(d, a, b_part, ptx::kUmmaDescHiSw128, kValueIdesc, j);
                     } else {
                         for (uint32_t step = 0; step < columns / 16; ++step) {
-                            ptx::umma_f16_ts(d, tmem + step / 2 * 32 + step % 2 * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc,
+                            ptx::umma_f16_ts(d, a + step / 2 * 32 + step % 2 * 8, b_part + step * (16 * 128 / 16), ptx::kUmmaDescHiSw128, kValueIdesc,
                                              j | step);
                         }
                     }
                 }
                 if (kScaled) ptx::umma_commit(empty + slot * 8u);
-                ptx::umma_commit(ptx::smem_u32(&control.value_done));
+                ptx::umma_commit(ptx::smem_u32(&control.value_done[buffer]));
             }
             __syncwarp();
-            if (j + 1 < tiles) {
-                ok = wait(control.value_done, j & 1u);                   // P has been read: S may take its place
+            if (next < tiles || loaded[1] < tiles) {
+                ok = wait(control.value_done[buffer], phase);            // P has been read: S may take its place, and values the slot
                 ptx::tc_fence_after();
-                if (ok) {
-                    multiply_scores(j + 1);
-                    load_tile();                                         // into the slots of tile j, whose products are done
-                }
+                if (ok && next < tiles) multiply_scores(next);
+                if (ok) load_tile(1);
             }
         }
         if (!ok) {
@@ -395,8 +404,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             __syncwarp();
             uint32_t never = 0;
             ptx::mbar_wait_bounded(ptx::smem_u32(&control.drained), 0, &never, limit);
-            for (uint32_t unit = 2 * loaded > kSlots ? 2 * loaded - kSlots : 0; unit < 2 * loaded; ++unit) {
-                ptx::mbar_wait_bounded(full + (unit % kSlots) * 8u, (unit / kSlots) & 1u, &never, limit);
+            for (uint32_t which = 0; which < 2; ++which) {               // and so do the copies
+                for (uint32_t index = loaded[which] > 2 ? loaded[which] - 2 : 0; index < loaded[which]; ++index) {
+                    const uint32_t unit = 2 * index + which;
+                    ptx::mbar_wait_bounded(full + (unit % kSlots) * 8u, (unit / kSlots) & 1u, &never, limit);
+                }
             }
         }
     } else {
@@ -463,7 +475,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
             if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
-            ok = ok && wait(control.score_ready, j & 1u);
+            ok = ok && wait(control.score_ready[j % kBuffers], (j / kBuffers) & 1u);
+            const uint32_t column_s = my_tmem + j % kBuffers * kTileKeys;
             if (!ok) break;
             ptx::tc_fence_after();
 
@@ -473,7 +486,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 return kScaled ? *reinterpret_cast<const float4*>(key_scales + column) : make_float4(scale, scale, scale, scale);
             };
             const auto load = [&](uint32_t c, uint32_t (&s)[32]) {
-                ptx::tmem_ld_32x32b_x32(my_tmem + c * 32u, s);
+                ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
                 ptx::tmem_ld_wait(s);
             };
             // the largest of 32 columns: of the scores in FP16 without their scale, which is the same for all
@@ -537,7 +550,14 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     w[i / 2] = pack_half2(x[0], x[1]);
                     w[i / 2 + 1] = pack_half2(x[2], x[3]);
                 }
-                ptx::tmem_st_32x32b_x16(my_tmem + c * 32u, w);
+                ptx::tmem_st_32x32b_x16(column_s + c * 32u, w);
+            };
+            // O is whole when the products of the tile before are done; with one buffer the scores' MMA has come behind them.
+            const auto values_done = [&] {
+                if (kBuffers == 1 || j == 0) return true;
+                const bool done = wait(control.value_done[(j - 1) % kBuffers], ((j - 1) / kBuffers) & 1u);
+                ptx::tc_fence_after();
+                return done;
             };
             if (warp_active) {
                 float value_bits = 0.0f;                                 // log2 of the tile's largest value scale
@@ -582,7 +602,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                         sum *= grow;
                     }
                     huge = __any_sync(0xffffffffu, fabsf(reference) > 4194304.0f && reference != kNone);
-                    if (j != 0) {                                        // the scores' MMA came behind the products of the tile before: O is whole
+                    if (j != 0) {
+                        ok = values_done();
+                        if (!ok) break;
 #pragma unroll
                         for (uint32_t c = 0; c < kDim; c += 16) {
                             uint32_t o[16];
@@ -627,7 +649,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             if (kFormat != KV_INT8 && ragged) {
                 const uint32_t unit = 2 * j + 1, base = slots_base + (unit % kSlots) * S::kTileBytes;
                 volatile uint32_t* const skip = &control.skip[j % 4];
-                ok = wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
+                ok = values_done() && wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
                 if (!ok) break;
                 bool found = false;
                 for (uint32_t i = threadIdx.x; i < columns * (kDim / 8); i += 32 * kSoftmaxWarps) {
@@ -649,7 +671,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                         for (int i = 0; i < 8; ++i) total[i] = j == 0 ? 0.0f : __uint_as_float(o[i]);
                         for (uint32_t key = 0; key < columns; ++key) {
                             uint32_t pair;
-                            ptx::tmem_ld_32x32b_x1(my_tmem + key / 32 * 32 + key % 32 / 2, pair);
+                            ptx::tmem_ld_32x32b_x1(column_s + key / 32 * 32 + key % 32 / 2, pair);
                             ptx::tmem_ld_wait(pair);
                             const float w = key % 2 == 0 ? half_lo(pair) : half_hi(pair);
                             const uint4 x = ptx::ld_shared16(base + swizzled(key, c / 8, kTileKeys));
@@ -667,10 +689,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     ptx::tmem_st_wait();
                 }
             }
-            arrive(control.weight_ready);
+            arrive(control.weight_ready[j % kBuffers]);
         }
         // from here on the room of Q is free: the last product has read it, or (no keys) all warps have written theirs
-        if (ok) ok = tiles != 0 ? wait(control.value_done, (tiles - 1) & 1u) : wait(control.query_ready, 0);
+        if (ok && tiles == 0) ok = wait(control.query_ready, 0);
+        if (ok && tiles != 0) ok = wait(control.value_done[(tiles - 1) % kBuffers], ((tiles - 1) / kBuffers) & 1u);
         ptx::tc_fence_after();
         if (!ok) {
             give_up(DEV_TIMEOUT_EPILOGUE);
