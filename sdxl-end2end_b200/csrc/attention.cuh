@@ -116,7 +116,7 @@ struct AttentionMaps {
 cudaError_t launch_attention_tiles(const AttentionParams& params, const AttentionMaps& maps, KvFormat format, uint32_t* error_word,
                                    long long wait_limit_cycles, cudaStream_t stream, bool early_launch);
 // tile_rows: of the pass that is joined (by_row: not used).
-cudaError_t launch_attention_join(const AttentionParams& params, uint32_t tile_rows, cudaStream_t stream, bool early_launch);
+cudaError_t launch_attention_join(const AttentionParams& params, uint32_t tile_rows, cudaStream_t stream);
 
 // A block's place in its pass.
 struct BlockPlace {

@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
             constexpr uint32_t kRounds = kTileKeys / kStep;
-            constexpr uint32_t kAhead = kDim == 64 ? 2 : 4;
+            constexpr uint32_t kAhead = 2;
             static_assert(kStep % 8 == 0 && kTileKeys % kStep == 0);
             const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
             const bool in_head = chunk * 16u < p.dim;
@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
-    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : kDim == 64 ? 2 : 4;
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : 2;
     constexpr int kBlocks = static_cast<int>(tile_blocks_per_sm(kDim, static_cast<KvFormat>(kFormat)));
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps, kBlocks>;

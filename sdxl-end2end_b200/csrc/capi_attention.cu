@@ -357,7 +357,7 @@ int run_attention(sdxlq_context* ctx, const sdxlq_attention_desc* desc) {
             launch(one, i);
         }
     }
-    if (error == cudaSuccess && p.slots > 1) error = launch_attention_join(p, plan.row_tile[0], ctx->stream, false);
+    if (error == cudaSuccess && p.slots > 1) error = launch_attention_join(p, plan.row_tile[0], ctx->stream);
     if (error != cudaSuccess) return fail_cuda(ctx, error, "attention launch");
     return SDXLQ_OK;
 }
