@@ -217,13 +217,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(full + (unit % kSlots) * 8u);
         };
-        const auto source = [&](uint32_t unit, typename Item<kDim>::Tile& t) -> const uint8_t* {
-            t = item.tile(item.tile_begin + unit / 2);
-            const KvView& view = t.in_prefix ? p.prefix : p.own;
-            const int64_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
-            return (unit % 2 == 0 ? view.k : view.v) + slot * view.slot_stride + item.kv_head * view.head_stride +
-                   static_cast<int64_t>(t.first) * view.token_stride;
-        };
         if constexpr (kScaled) {
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
@@ -237,27 +230,47 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             uint4 ahead[kAhead][kRounds];
             constexpr uint32_t kScales = (kTileKeys + kThreads - 1) / kThreads;      // of a thread
             float ahead_scale[kAhead / 2][kScales][2] = {};
-            const auto fetch = [&](uint32_t unit, auto buffer) {
-                constexpr uint32_t kBuffer = decltype(buffer)::value;
-                typename Item<kDim>::Tile t;
-                const uint8_t* const base = source(unit, t);
-                const int64_t stride = t.in_prefix ? p.prefix.token_stride : p.own.token_stride;
-                const uint8_t* from = base + first_key * stride + chunk * 16u;
-#pragma unroll
-                for (uint32_t i = 0; i < kRounds; ++i, from += kStep * stride) {
-                    const bool inside = in_head && t.first + first_key + i * kStep < t.end;
-                    ahead[kBuffer][i] = inside ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+            // where the thread's first 16 bytes of the next tile to fetch are, in K and V, and its scales; tiles come in order
+            const uint8_t* from[2] = {};
+            const float* scale_from[2] = {};
+            int64_t step = 0, to_next = 0;                               // bytes between rounds, and from tile to tile
+            typename Item<kDim>::Tile t{};
+            const auto seek = [&](uint32_t index) {
+                const bool was_in_prefix = t.in_prefix;
+                t = item.tile(item.tile_begin + index);
+                if (index != 0 && was_in_prefix == t.in_prefix) {
+                    from[0] += to_next; from[1] += to_next;
+                    scale_from[0] += kTileKeys; scale_from[1] += kTileKeys;
+                    return;
                 }
-                if constexpr (kBuffer % 2 == 0) {
-                    const KvView& view = t.in_prefix ? p.prefix : p.own;
-                    const int64_t slot = t.in_prefix ? item.prefix_slot : item.first_member;
-                    const int64_t at = (slot * p.kv_heads + item.kv_head) * view.capacity + t.first;
+                const KvView& view = t.in_prefix ? p.prefix : p.own;
+                const int64_t sequence = t.in_prefix ? item.prefix_slot : item.first_member;
+                const int64_t at = sequence * view.slot_stride + item.kv_head * view.head_stride + static_cast<int64_t>(t.first + first_key) * view.token_stride + chunk * 16u;
+                const int64_t scales_at = (sequence * p.kv_heads + item.kv_head) * view.capacity + t.first;
+                from[0] = view.k + at;
+                from[1] = view.v + at;
+                scale_from[0] = view.k_scales + scales_at;
+                scale_from[1] = view.v_scales + scales_at;
+                step = kStep * view.token_stride;
+                to_next = kTileKeys * view.token_stride;
+            };
+            const auto fetch = [&](uint32_t unit, auto buffer) {
+                constexpr uint32_t kBuffer = decltype(buffer)::value, kWhich = kBuffer % 2;
+                if constexpr (kWhich == 0) seek(unit / 2);
+                const uint8_t* at = from[kWhich];
+                const uint32_t left = t.end - t.first;
+#pragma unroll
+                for (uint32_t i = 0; i < kRounds; ++i, at += step) {
+                    const bool inside = in_head && first_key + i * kStep < left;
+                    ahead[kBuffer][i] = inside ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                if constexpr (kWhich == 0) {
 #pragma unroll
                     for (uint32_t i = 0; i < kScales; ++i) {
                         const uint32_t key = i * kThreads + thread;
-                        const bool inside = key < kTileKeys && t.first + key < t.end;
-                        ahead_scale[kBuffer / 2][i][0] = inside ? __ldg(view.k_scales + at + key) * fabsf(p.scale_log2) : 0.0f;
-                        ahead_scale[kBuffer / 2][i][1] = inside ? __ldg(view.v_scales + at + key) : 0.0f;
+                        const bool inside = key < kTileKeys && key < left;
+                        ahead_scale[kBuffer / 2][i][0] = inside ? __ldg(scale_from[0] + key) * fabsf(p.scale_log2) : 0.0f;
+                        ahead_scale[kBuffer / 2][i][1] = inside ? __ldg(scale_from[1] + key) : 0.0f;
                     }
                 }
             };
@@ -480,14 +493,19 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             if (!ok) break;
             ptx::tc_fence_after();
 
-            // Scores in units of log2, less the reference. The fused multiply-add rounds the difference alone, so that it is as
-            // exact for large scores as for small ones.
-            const auto key_scale = [&](uint32_t column) {
-                return kScaled ? *reinterpret_cast<const float4*>(key_scales + column) : make_float4(scale, scale, scale, scale);
-            };
+            // 32 columns of S; those of an 8-bit cache times their key's scale
             const auto load = [&](uint32_t c, uint32_t (&s)[32]) {
                 ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
                 ptx::tmem_ld_wait(s);
+                if constexpr (kScaled) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
+                        const float2 lo = __fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y));
+                        const float2 hi = __fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w));
+                        s[i] = __float_as_uint(lo.x); s[i + 1] = __float_as_uint(lo.y); s[i + 2] = __float_as_uint(hi.x); s[i + 3] = __float_as_uint(hi.y);
+                    }
+                }
             };
             // the largest of 32 columns: of the scores in FP16 without their scale, which is the same for all
             const auto largest_of = [&](auto careful_case, uint32_t c, const uint32_t (&s)[32], float largest) {
@@ -496,10 +514,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                     float x[4] = {__uint_as_float(s[i]), __uint_as_float(s[i + 1]), __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])};
-                    if constexpr (kScaled) {
-                        const float4 k = key_scale(c * 32u + i);
-                        x[0] *= k.x; x[1] *= k.y; x[2] *= k.z; x[3] *= k.w;
-                    }
                     if (careful) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
@@ -515,15 +529,14 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    const float4 k = key_scale(c * 32u + i);
-                    const float2 lo = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y), make_float2(-shift, -shift));
-                    const float2 hi = __ffma2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w), make_float2(-shift, -shift));
+                    // Scores in units of log2, less the reference. The fused multiply-add rounds the difference alone, so that
+                    // it is as exact for large scores as for small ones.
+                    float2 lo = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), hi = make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                    const float2 back = make_float2(-shift, -shift);
+                    lo = kScaled ? __fadd2_rn(lo, back) : __ffma2_rn(lo, make_float2(scale, scale), back);
+                    hi = kScaled ? __fadd2_rn(hi, back) : __ffma2_rn(hi, make_float2(scale, scale), back);
                     float x[4] = {lo.x, lo.y, hi.x, hi.y};
                     if (careful) {
-                        if (kScaled && huge) {                           // rounded as the maximum was
-                            x[0] = __fmul_rn(__uint_as_float(s[i]), k.x) - shift; x[1] = __fmul_rn(__uint_as_float(s[i + 1]), k.y) - shift;
-                            x[2] = __fmul_rn(__uint_as_float(s[i + 2]), k.z) - shift; x[3] = __fmul_rn(__uint_as_float(s[i + 3]), k.w) - shift;
-                        }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] -= fine;
                     }
@@ -570,14 +583,17 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     value_bits = log2_approx(top);
                 }
                 const bool both = columns > 32u;
-                uint32_t s[32];
+                // Columns 32 to 63 stay in registers until they are weighed; the first 32 too, where there is room for them.
+                constexpr bool kHold = kDim > 64;
+                uint32_t s[kHold ? 2 : 1][32];
+                uint32_t (&s0)[32] = s[0], (&s1)[32] = s[kHold ? 1 : 0];
                 float largest = kNone;
                 const auto find_largest = [&](auto careful) {
-                    load(0, s);
-                    largest = largest_of(careful, 0, s, largest);
+                    load(0, s0);
+                    largest = largest_of(careful, 0, s0, largest);
                     if (both) {
-                        load(1, s);
-                        largest = largest_of(careful, 1, s, largest);
+                        load(1, s1);
+                        largest = largest_of(careful, 1, s1, largest);
                     }
                 };
                 if (masked) find_largest(std::true_type{});
@@ -620,10 +636,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 const float shift = reference == kNone ? 0.0f : reference;       // a row that has seen nothing has no weights at all
                 const auto take_weights = [&](auto careful) {
                     if (both) {
-                        weigh(careful, 1, s, shift, part);
-                        load(0, s);
+                        weigh(careful, 1, s1, shift, part);
+                        if (!kHold) load(0, s0);
                     }
-                    weigh(careful, 0, s, shift, part);
+                    weigh(careful, 0, s0, shift, part);
                 };
                 if (masked || huge || special) take_weights(std::true_type{});
                 else take_weights(std::false_type{});
