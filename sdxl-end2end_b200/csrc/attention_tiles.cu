@@ -169,25 +169,73 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
     volatile uint32_t* const abort_word = &control.abort;
     const long long limit = params.wait_limit_cycles;
 
-    if (threadIdx.x == 0) {
-        ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
-        for (uint32_t b = 0; b < S::kBuffers; ++b) {
-            ptx::mbar_init(ptx::smem_u32(&control.score_ready[b]), 1);
-            ptx::mbar_init(ptx::smem_u32(&control.weight_ready[b]), kSoftmaxWarps);
-            ptx::mbar_init(ptx::smem_u32(&control.value_done[b]), 1);
+    wait_for_prior_kernels_then_release_next();
+    const Item<kDim> item(p);
+    const uint32_t tiles = item.tile_end - item.tile_begin;
+    const uint32_t full = ptx::smem_u32(&control.full[0]), empty = ptx::smem_u32(&control.empty[0]);
+    const auto give_up = [&](uint32_t code) {
+        *abort_word = 1;
+        atomicCAS(params.error_word, 0u, code);
+    };
+
+    // FP16 keys (0) and values (1), a tile at a time, by the MMA warp
+    uint32_t loaded[2] = {0, 0};
+    const auto load_tile = [&](uint32_t which) {
+        if (kScaled || loaded[which] == tiles) return;
+        const uint32_t index = loaded[which]++, slot = (2 * index + which) % kSlots, bar = full + slot * 8u;
+        const typename Item<kDim>::Tile t = item.tile(item.tile_begin + index);
+        if (ptx::elect_one()) {
+            const uint32_t part = t.in_prefix ? 0u : 1u, sequence = t.in_prefix ? item.prefix_slot : item.first_member;
+            ptx::mbar_expect_tx(bar, S::kTileBytes);
+#pragma unroll
+            for (uint32_t d = 0; d < kDim; d += 64) {
+                ptx::tma_load_4d(slots_base + slot * S::kTileBytes + d * (kTileKeys * 2), &params.maps.map[part][which], bar, static_cast<int32_t>(d),
+                                 static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(sequence));
+            }
         }
-        ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
-        for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kScaled ? kLoaderWarps : 1);
-        for (uint32_t s = 0; s < kSlots; ++s) {
-            ptx::mbar_init(ptx::smem_u32(&control.full[s]), kScaled ? kLoaderWarps : 1);
-            ptx::mbar_init(ptx::smem_u32(&control.empty[s]), 1);
+        __syncwarp();
+    };
+
+    // Q and the output move by whole lines: a lane takes 16 bytes of the warp's rows in turn, eight at a time. The first eight
+    // are on their way while the barriers and the tensor memory are set up.
+    constexpr uint32_t kChunksOfRow = kDim / 8, kRowsAtOnce = 32 / kChunksOfRow, kBatch = 8;
+    const uint32_t row = threadIdx.x;                                    // of the tile, and lane of tensor memory (softmax)
+    const uint32_t chunk_of_row = lane % kChunksOfRow, first_of_warp = warp * 32u + lane / kChunksOfRow;
+    const bool in_head = chunk_of_row * 8u < p.dim;
+    QueryRow at{};
+    int64_t query_offset = 0;
+    uint4 query[kBatch];
+    const auto load_queries = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t r = first_of_warp + first + i * kRowsAtOnce;
+            const int64_t from = __shfl_sync(0xffffffffu, query_offset, r & 31u);
+            query[i] = r < item.rows && in_head ? __ldg(reinterpret_cast<const uint4*>(p.q + from + chunk_of_row * 8u)) : make_uint4(0u, 0u, 0u, 0u);
         }
-        control.abort = 0;
-        for (uint32_t i = 0; i < 4; ++i) control.skip[i] = 0;
-        ptx::fence_mbar_init();
-    }
-    if (warp == kSoftmaxWarps) {
+    };
+    if (warp < kSoftmaxWarps) {
+        at = locate_row(p, item.first_member, item.kv_head, item.first_row + min(row, item.rows - 1));
+        query_offset = at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head;
+        load_queries(0);
+        if (threadIdx.x == 0) {
+            ptx::mbar_init(ptx::smem_u32(&control.query_ready), kSoftmaxWarps);
+            for (uint32_t b = 0; b < kBuffers; ++b) {
+                ptx::mbar_init(ptx::smem_u32(&control.score_ready[b]), 1);
+                ptx::mbar_init(ptx::smem_u32(&control.weight_ready[b]), kSoftmaxWarps);
+                ptx::mbar_init(ptx::smem_u32(&control.value_done[b]), 1);
+            }
+            ptx::mbar_init(ptx::smem_u32(&control.vote), kSoftmaxWarps);
+            ptx::mbar_init(ptx::smem_u32(&control.drained), 1);
+            for (uint32_t s = 0; s < kScaleRing; ++s) ptx::mbar_init(ptx::smem_u32(&control.scales_full[s]), kScaled ? kLoaderWarps : 1);
+            for (uint32_t s = 0; s < kSlots; ++s) {
+                ptx::mbar_init(full + s * 8u, kScaled ? kLoaderWarps : 1);
+                ptx::mbar_init(empty + s * 8u, 1);
+            }
+            control.abort = 0;
+            for (uint32_t i = 0; i < 4; ++i) control.skip[i] = 0;
+            ptx::fence_mbar_init();
+        }
+    } else if (warp == kSoftmaxWarps) {
         ptx::tmem_alloc(ptx::smem_u32(&control.tmem_base), S::kColumns);
         ptx::tmem_relinquish();
     }
@@ -195,20 +243,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&control.tmem_base);
-    wait_for_prior_kernels_then_release_next();
-
-    const Item<kDim> item(p);
-    const uint32_t tiles = item.tile_end - item.tile_begin;
-    const auto give_up = [&](uint32_t code) {
-        *abort_word = 1;
-        atomicCAS(params.error_word, 0u, code);
-    };
 
     if (warp > kSoftmaxWarps) {
         // ---------------------------------------- loaders ----------------------------------------
         const uint32_t thread = threadIdx.x - 32u * (kSoftmaxWarps + 1);
         constexpr uint32_t kThreads = 32u * kLoaderWarps;
-        const uint32_t full = ptx::smem_u32(&control.full[0]), empty = ptx::smem_u32(&control.empty[0]);
         const auto slot_free = [&](uint32_t unit) {
             return ptx::warp_wait_bounded(empty + (unit % kSlots) * 8u, ((unit / kSlots) & 1u) ^ 1u, abort_word, limit);
         };
@@ -325,7 +364,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
         }
     } else if (warp == kSoftmaxWarps) {
         // ------------------------- MMA issuer, and the loads of FP16 keys and values -------------------------
-        const uint32_t full = ptx::smem_u32(&control.full[0]), empty = ptx::smem_u32(&control.empty[0]);
         const auto wait = [&](const uint64_t& bar, uint32_t parity) {
             return ptx::warp_wait_bounded(ptx::smem_u32(&bar), parity, abort_word, limit);
         };
@@ -347,22 +385,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 }
                 if (kScaled) ptx::umma_commit(empty + slot * 8u);
                 ptx::umma_commit(ptx::smem_u32(&control.score_ready[j % kBuffers]));
-            }
-            __syncwarp();
-        };
-        uint32_t loaded[2] = {0, 0};                                     // tiles of K and of V that were sent for (FP16)
-        const auto load_tile = [&](uint32_t which) {
-            if (kScaled || loaded[which] == tiles) return;
-            const uint32_t index = loaded[which]++, slot = (2 * index + which) % kSlots, bar = full + slot * 8u;
-            const typename Item<kDim>::Tile t = item.tile(item.tile_begin + index);
-            if (ptx::elect_one()) {
-                const uint32_t part = t.in_prefix ? 0u : 1u, sequence = t.in_prefix ? item.prefix_slot : item.first_member;
-                ptx::mbar_expect_tx(bar, S::kTileBytes);
-#pragma unroll
-                for (uint32_t d = 0; d < kDim; d += 64) {
-                    ptx::tma_load_4d(slots_base + slot * S::kTileBytes + d * (kTileKeys * 2), &params.maps.map[part][which], bar, static_cast<int32_t>(d),
-                                     static_cast<int32_t>(item.kv_head), static_cast<int32_t>(t.first), static_cast<int32_t>(sequence));
-                }
             }
             __syncwarp();
         };
@@ -426,7 +448,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
         }
     } else {
         // ---------------------------------------- softmax ----------------------------------------
-        const uint32_t row = threadIdx.x;                                // of the tile, and lane of tensor memory
         const uint32_t my_tmem = tmem + ((warp * 32u) << 16);
         const uint32_t column_o = my_tmem + S::kColumnO;
         const bool warp_active = warp * 32u < item.rows;
@@ -438,29 +459,17 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bar));
         };
-        const QueryRow at = locate_row(p, item.first_member, item.kv_head, item.first_row + min(row, item.rows - 1));
-        // Q and the output move by whole lines: a lane takes 16 bytes of the warp's rows in turn
-        constexpr uint32_t kChunks = kDim / 8, kRowsAtOnce = 32 / kChunks;
-        const uint32_t chunk = lane % kChunks, first_of_warp = warp * 32u + lane / kChunks;
-        const bool in_head = chunk * 8u < p.dim;
         {
             // a negative softmax scale turns the queries' signs, so that scores are multiplied by its magnitude
             const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-            const int64_t offset = at.batch * p.q_batch + at.token * p.q_token + at.head * p.q_head;
-            constexpr uint32_t kBatch = 8;
 #pragma unroll
             for (uint32_t first = 0; first < 32; first += kBatch * kRowsAtOnce) {
-                uint4 x[kBatch];
+                if (first != 0) load_queries(first);
 #pragma unroll
                 for (uint32_t i = 0; i < kBatch; ++i) {
-                    const uint32_t r = first_of_warp + first + i * kRowsAtOnce;
-                    const int64_t from = __shfl_sync(0xffffffffu, offset, r & 31u);
-                    x[i] = r < item.rows && in_head ? __ldg(reinterpret_cast<const uint4*>(p.q + from + chunk * 8u)) : make_uint4(0u, 0u, 0u, 0u);
-                }
-#pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i) {
-                    x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
-                    ptx::st_shared16(query_base + swizzled(first_of_warp + first + i * kRowsAtOnce, chunk, kTileRows), x[i]);
+                    uint4 x = query[i];
+                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                    ptx::st_shared16(query_base + swizzled(first_of_warp + first + i * kRowsAtOnce, chunk_of_row, kTileRows), x);
                 }
             }
             ptx::fence_proxy_async();
@@ -715,7 +724,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             give_up(DEV_TIMEOUT_EPILOGUE);
         } else if (warp_active) {
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const bool empty = tiles == 0;                               // O was never written
+            const bool nothing = tiles == 0 || sum == 0.0f;              // O was never written, or holds no weight
             if (writes_output(p, item.here)) {
                 // the warp's rows of Q make room for its rows of the output, which leave in whole lines
 #pragma unroll
@@ -725,7 +734,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     ptx::tmem_ld_wait(o);
                     float x[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = empty || sum == 0.0f ? 0.0f : __uint_as_float(o[i]) * inverse;
+                    for (int i = 0; i < 16; ++i) x[i] = nothing ? 0.0f : __uint_as_float(o[i]) * inverse;
                     ptx::st_shared16(query_base + swizzled(row, c / 8, kTileRows),
                                      make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7])));
                     ptx::st_shared16(query_base + swizzled(row, c / 8 + 1, kTileRows),
@@ -737,24 +746,32 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 for (uint32_t i = 0; i < 32; i += kRowsAtOnce) {
                     const uint32_t r = first_of_warp + i;
                     const int64_t to = __shfl_sync(0xffffffffu, offset, r & 31u);
-                    if (r < item.rows && in_head) *reinterpret_cast<uint4*>(p.y + to + chunk * 8u) = ptx::ld_shared16(query_base + swizzled(r, chunk, kTileRows));
+                    if (r < item.rows && in_head) *reinterpret_cast<uint4*>(p.y + to + chunk_of_row * 8u) = ptx::ld_shared16(query_base + swizzled(r, chunk_of_row, kTileRows));
                 }
             } else {
+                // in 32 bits through the warp's share of the slots, which are free by now, and out in whole lines
                 const uint64_t place = scratch_row(p, item.here, kTileRows, row, (static_cast<uint64_t>(at.batch) * p.q_tokens + at.token) * p.q_heads + at.head);
+                constexpr uint32_t kQuads = kDim / 4, kRowsOut = 32 / kQuads;
+                const uint32_t room = slots_base + warp * (32 * kDim * 4);
 #pragma unroll
                 for (uint32_t c = 0; c < kDim; c += 16) {
                     uint32_t o[16];
                     ptx::tmem_ld_32x32b_x16(column_o + c, o);
                     ptx::tmem_ld_wait(o);
-                    float4* const out = reinterpret_cast<float4*>(p.part_o + place * p.dim + c);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = nothing ? 0u : __float_as_uint(__uint_as_float(o[i]) * inverse);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (row < item.rows && c + 4u * i < p.dim) {
-                            out[i] = empty || sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                                          : make_float4(__uint_as_float(o[4 * i]) * inverse, __uint_as_float(o[4 * i + 1]) * inverse,
-                                                                        __uint_as_float(o[4 * i + 2]) * inverse, __uint_as_float(o[4 * i + 3]) * inverse);
-                        }
+                        ptx::st_shared16(room + lane * (kDim * 4) + (((c / 4 + i) ^ (lane & 7u)) << 4), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
                     }
+                }
+                __syncwarp();
+                const uint32_t quad = lane % kQuads;
+#pragma unroll 8
+                for (uint32_t r = lane / kQuads; r < 32; r += kRowsOut) {
+                    const uint64_t to = __shfl_sync(0xffffffffu, place, r);
+                    const uint4 x = ptx::ld_shared16(room + r * (kDim * 4) + ((quad ^ (r & 7u)) << 4));
+                    if (warp * 32u + r < item.rows && quad * 4u < p.dim) *reinterpret_cast<uint4*>(p.part_o + to * p.dim + quad * 4u) = x;
                 }
                 if (row < item.rows) p.part_lse[place] = make_float2(sum == 0.0f ? kNone : reference > kNone ? reference : 0.0f, fine + log2f(sum));
             }

@@ -252,9 +252,20 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     const uint32_t tensor_blocks = tile_blocks_per_sm(p.dim, plan.format[0]) * static_cast<uint32_t>(sm_count);
     if (p.pass_count == 1 && plan.row_tile[0] == kTensorTile) {
         // Blocks of like length come in waves of `tensor_blocks`. The tiles of the last wave, where it is not full, become a
-        // pass whose keys are split until it is, into shares of no less than 256 keys.
+        // pass of their own whose keys are split: `splits` shares of no less than 256 keys make ceil(rest * splits / tensor_blocks)
+        // waves of 1 / splits the length. A wave also has about four key tiles' time of setting up and storing, and the join
+        // as much again.
         const uint32_t tiles = p.pass[0].tiles, rest = tiles % tensor_blocks;
-        const uint32_t splits = rest == 0 ? 1u : static_cast<uint32_t>(std::min<uint64_t>(tensor_blocks / rest, keys[0] / 256));
+        const double key_tiles = static_cast<double>(keys[0]) / kTileKeys;
+        uint32_t splits = 1;
+        double least = key_tiles + 4.0;
+        for (uint32_t s = 2; rest != 0 && s <= 64 && keys[0] / s >= 256; ++s) {
+            const double time = static_cast<double>(ceil_div(static_cast<uint64_t>(rest) * s, tensor_blocks)) * (key_tiles / s + 4.0) + 4.0;
+            if (time < least) {
+                least = time;
+                splits = s;
+            }
+        }
         if (splits > 1) {
             const uint32_t last = rest == tiles ? 0u : 1u;
             if (last == 1) {
