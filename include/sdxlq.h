@@ -254,7 +254,7 @@ int sdxlq_layer_norm(sdxlq_context* ctx, const sdxlq_layer_norm_desc* desc);
 /* Keys and values of `slots` sequences of up to `capacity` tokens: a cache in one of the library's types, or FP16 tensors as
  * the to_k / to_v projections write them. Element d of head h of token t of slot s is at
  * s * slot_stride + t * token_stride + h * head_stride + d, in k and in v alike (strides in elements).
- * 8-bit types hold a scale for each vector of a head: value = element * scales[s, h, t].
+ * 8-bit types hold a finite scale for each vector of a head: value = element * scales[s, h, t].
  * head_dim is a multiple of 8 (FP16) or 16 (8-bit types) and at most 128; k, v and the strides are multiples of 16 bytes
  * (SDXLQ_ERR_UNSUPPORTED_SHAPE otherwise). */
 typedef struct sdxlq_kv_cache {

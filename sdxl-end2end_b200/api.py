@@ -1,6 +1,7 @@
 """ctypes binding of include/sdxlq.h plus the host-side mirror of the reference interface."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import enum
 import importlib.machinery
@@ -476,14 +477,17 @@ class Context:
         if status != STATUS_OK:
             raise CudaError(self._lib.sdxlq_last_error(self._handle).decode(), status)
 
-    def scratch(self, size: int) -> torch.Tensor:
-        """Memory for the kernels of one call: in the pool of the stream that they run on, whichever stream is current, so that
-        its next owner comes behind them."""
+    def on_stream(self):
+        """Makes the context's stream PyTorch's current one: memory allocated here is handed out again behind its kernels."""
         device = torch.device("cuda", self.device)
         if torch.cuda.current_stream(device).cuda_stream == self.stream_address:
-            return torch.empty(size, dtype=torch.uint8, device=device)
-        with torch.cuda.stream(torch.cuda.ExternalStream(self.stream_address, device=device)):
-            return torch.empty(size, dtype=torch.uint8, device=device)
+            return contextlib.nullcontext()
+        return torch.cuda.stream(torch.cuda.ExternalStream(self.stream_address, device=device))
+
+    def scratch(self, size: int) -> torch.Tensor:
+        """Memory for the kernels of one call."""
+        with self.on_stream():
+            return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", self.device))
 
     def set_stream(self, stream: torch.cuda.Stream) -> None:
         self.stream = stream
@@ -737,10 +741,11 @@ class Ops:
         if type not in _KV_TORCH:
             raise CudaError("kv cache: expects FP16, INT8 or FP8 elements of the stated type")
         device = torch.device("cuda", self.ctx.device)
-        k, v = (torch.zeros((slots, heads, capacity, head_dim), dtype=_KV_TORCH[type], device=device).transpose(1, 2) for _ in "kv")
-        scales = (None, None)
-        if type != ScalarType.Float16:
-            scales = tuple(torch.ones((slots, heads, capacity), dtype=torch.float32, device=device) for _ in "kv")
+        with self.ctx.on_stream():                                   # cleared where it will be written and read
+            k, v = (torch.zeros((slots, heads, capacity, head_dim), dtype=_KV_TORCH[type], device=device).transpose(1, 2) for _ in "kv")
+            scales = (None, None)
+            if type != ScalarType.Float16:
+                scales = tuple(torch.ones((slots, heads, capacity), dtype=torch.float32, device=device) for _ in "kv")
         return KVCache(k, v, type, *scales)
 
     def _kv_tokens(self, what: str, cache: KVCache, key: torch.Tensor, value: torch.Tensor, positions, counts, first_slot: int) -> _CKvTokens:

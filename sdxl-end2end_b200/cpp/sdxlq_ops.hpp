@@ -219,6 +219,19 @@ public:
         return output;
     }
 
+    // Keys and values into a cache in the library's types and back, and attention over a prefix that several batch entries
+    // share and over keys of their own: the C ABI's descriptors, with CudaError where it refuses one. Attention's scratch is the
+    // context's workspace unless the descriptor brings its own.
+    void kv_cache_write(const sdxlq_kv_cache& cache, const sdxlq_kv_tokens& tokens) const {
+        runtime_->check(sdxlq_kv_cache_write(runtime_->context(), &cache, &tokens));
+    }
+    void kv_cache_read(const sdxlq_kv_cache& cache, const sdxlq_kv_tokens& tokens) const {
+        runtime_->check(sdxlq_kv_cache_read(runtime_->context(), &cache, &tokens));
+    }
+    void shared_prefix_attention(const sdxlq_attention_desc& desc) const {
+        runtime_->check(sdxlq_shared_prefix_attention(runtime_->context(), &desc));
+    }
+
     // Ops::quantize_fp8 / quantize_e4m3 / quantize_e5m2 (src/cuda/ops_blas.cpp:231-242).
     [[nodiscard]] TensorRef quantize_fp8(const TensorRef& input, ScalarType fp8_type) const {
         if (input.type != ScalarType::Float16 || !is_fp8(fp8_type)) {

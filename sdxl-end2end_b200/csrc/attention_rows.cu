@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
         if constexpr (kScaled) {
             float largest = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kKeys / 4; ++i) largest = fmaxf(largest, values.scale[i]);
+            for (int i = 0; i < kKeys / 4; ++i) largest = fmaxf(largest, fabsf(values.scale[i]));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
             if (largest > kScaleSlack * scale_reference) {

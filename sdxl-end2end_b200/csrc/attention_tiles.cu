@@ -1,20 +1,25 @@
 // Attention of many query rows per key head (image tokens, long questions): tiles of 128 rows on the tensor memory. See
 // attention.cuh for rows, passes and items, attention_rows.cu for few rows.
 //
-// A CTA takes 128 rows over its share of the keys, in tiles of 128 keys (heads of up to 64) or 64 (up to 128):
+// A CTA takes 128 rows over its share of the keys, in tiles of 64 keys:
 //   MMA warp       S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V as it lies, MN-major);
 //                  FP16 keys and values by TMA into a ring of four slots, as SWIZZLE_128B operands
 //   loader warps   (8-bit caches) the same through registers, widened to exact halves without their scales
-//   softmax warps  a thread per row: S from tensor memory, the weights back into it as halves
-// S, P and O share 256 columns, so that two CTAs work on an SM and the one's MMAs run under the other's exponentials.
+//   softmax warps  a thread per row: S from tensor memory, the weights back into it as halves, in the place of their scores
+// Everything that one tile needs of the one before it is a round trip between the warps (softmax, product, scores: 2.2
+// thousand clocks, of which the SM's exponentials take 512), so what counts is how many tiles an SM has in flight. Heads of
+// 64 take 128 columns of tensor memory and 48 KB, so four CTAs share an SM; heads of up to 128 take 256 columns, two CTAs,
+// each with the scores of two tiles. Measured on the self-attention of 2 x 4096 tokens, 10 heads of 64: tiles of 128
+// keys with two CTAs per SM 226 us, these 139 us (620 TFLOP/s). Taking every fourth exponential as a polynomial on the FMA
+// pipe gave nothing (141 us): the pipe of the exponentials is busy 60 % of the time.
 //
 // With M the row's running reference, a weight is 2^(s_j log2 e - M); M is the running maximum minus 6, and only moves when a
 // tile's maximum passes it by more than 2^7: then O, in tensor memory, and the sum are multiplied by 2^(M_old - M). Weights
 // of an 8-bit cache are multiplied by their value's scale, and M contains the logarithm of the tile's largest value scale,
 // so that they stay within the halves; O / l is the same for any M.
 //
-// What bounds it: for heads of 64 the exponentials, 1024 clocks of the SM's 16 lanes a clock for a tile of 128 x 128, whose
-// MMAs take 512; for short keys the bytes of Q and of the output.
+// What bounds it: those round trips; for keys of one or two tiles setting up and storing (5 of 7 us of a CTA's life over 77
+// keys: 80 us for 16 x 4096 queries of 10 heads, 2.1 TB/s); for 8-bit caches and heads of 128 the loaders' conversions.
 
 #include "attention.cuh"
 #include "internal.cuh"
@@ -32,7 +37,6 @@ constexpr uint32_t kSlots = 4;                   // K0 V0 K1 V1
 constexpr uint32_t kScaleRing = 4;               // key tiles whose scales are held
 constexpr uint32_t kSoftmaxWarps = 4;
 constexpr float kWeightBits = 6.0f, kSlackBits = 7.0f;
-constexpr uint32_t kPolynomialGroups = 0x88;      // of the eight groups of four columns in 32, those whose 2^x is a polynomial
 
 // Tensor-memory columns of a CTA: S and, in its place, P (the weights of 32 keys in the first 16 columns of their
 // scores), for heads of 128 in two buffers (scores of the next tile under the softmax of this one), then O. Shared memory: Q
@@ -73,28 +77,11 @@ __device__ __forceinline__ float log2_approx(float x) {
     return y;
 }
 
-// The largest of three, NaN if one of them is.
+// The largest of three (max.f32 takes three operands on sm_100); NaN never wins.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
-}
-
-// 2^x for finite x up to 126 (below -126 it is 2^-126) on the FMA pipe: x = n + f with n the nearest integer, left in the low
-// bits of x + 1.5 * 2^23, and 2^f by the degree-4 polynomial of least relative error on [-1/2, 1/2] (2.7e-6, found by
-// reweighted least squares on Chebyshev nodes), whose exponent n is added to.
-__device__ __forceinline__ float2 exp2_polynomial(float2 x) {
-    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
-    const float2 shifted = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f));
-    const float2 whole = __fadd2_rn(shifted, make_float2(-12582912.0f, -12582912.0f));
-    const float2 f = __ffma2_rn(whole, make_float2(-1.0f, -1.0f), x);
-    float2 y = make_float2(0.009570101276040077f, 0.009570101276040077f);
-    y = __ffma2_rn(y, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
-    y = __ffma2_rn(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    y = __ffma2_rn(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    y = __ffma2_rn(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(shifted.x) << 23)),
-                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(shifted.y) << 23)));
 }
 
 __device__ __forceinline__ bool half_not_finite(uint32_t pair) {
@@ -259,12 +246,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
         if constexpr (kScaled) {
             constexpr uint32_t kChunks = kDim / 16;                      // 16-byte loads of a key
             constexpr uint32_t kStep = kThreads / kChunks;
-            constexpr uint32_t kRounds = kTileKeys / kStep;
+            constexpr uint32_t kRounds = (kTileKeys + kStep - 1) / kStep;
             constexpr uint32_t kAhead = 2;
-            static_assert(kStep % 8 == 0 && kTileKeys % kStep == 0);
+            static_assert(kThreads % kChunks == 0);
             const uint32_t chunk = thread % kChunks, first_key = thread / kChunks;
             const bool in_head = chunk * 16u < p.dim;
-            const uint32_t target0 = swizzled(first_key, 2u * chunk, kTileKeys), target1 = swizzled(first_key, 2u * chunk + 1u, kTileKeys);
             // kAhead tiles of K or V are on their way to the registers at a time
             uint4 ahead[kAhead][kRounds];
             constexpr uint32_t kScales = (kTileKeys + kThreads - 1) / kThreads;      // of a thread
@@ -297,7 +283,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 constexpr uint32_t kBuffer = decltype(buffer)::value, kWhich = kBuffer % 2;
                 if constexpr (kWhich == 0) seek(unit / 2);
                 const uint8_t* at = from[kWhich];
-                const uint32_t left = t.end - t.first;
+                const uint32_t left = min(t.end - t.first, kTileKeys);
 #pragma unroll
                 for (uint32_t i = 0; i < kRounds; ++i, at += step) {
                     const bool inside = in_head && first_key + i * kStep < left;
@@ -307,7 +293,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 #pragma unroll
                     for (uint32_t i = 0; i < kScales; ++i) {
                         const uint32_t key = i * kThreads + thread;
-                        const bool inside = key < kTileKeys && key < left;
+                        const bool inside = key < left;
                         ahead_scale[kBuffer / 2][i][0] = inside ? __ldg(scale_from[0] + key) * fabsf(p.scale_log2) : 0.0f;
                         ahead_scale[kBuffer / 2][i][1] = inside ? __ldg(scale_from[1] + key) : 0.0f;
                     }
@@ -316,13 +302,15 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             const auto put = [&](uint32_t unit, auto buffer) {
                 constexpr uint32_t kBuffer = decltype(buffer)::value;
                 if (!slot_free(unit)) return false;
-                uint32_t to = slots_base + (unit % kSlots) * S::kTileBytes;
+                const uint32_t to = slots_base + (unit % kSlots) * S::kTileBytes;
 #pragma unroll
-                for (uint32_t i = 0; i < kRounds; ++i, to += kStep * 128u) {
+                for (uint32_t i = 0; i < kRounds; ++i) {
+                    const uint32_t key = first_key + i * kStep;
+                    if (key >= kTileKeys) break;
                     const uint4 x = ahead[kBuffer][i];
                     const uint2 a = widen4<kFormat>(x.x), b = widen4<kFormat>(x.y), c = widen4<kFormat>(x.z), d = widen4<kFormat>(x.w);
-                    ptx::st_shared16(to + target0, make_uint4(a.x, a.y, b.x, b.y));
-                    ptx::st_shared16(to + target1, make_uint4(c.x, c.y, d.x, d.y));
+                    ptx::st_shared16(to + swizzled(key, 2u * chunk, kTileKeys), make_uint4(a.x, a.y, b.x, b.y));
+                    ptx::st_shared16(to + swizzled(key, 2u * chunk + 1u, kTileKeys), make_uint4(c.x, c.y, d.x, d.y));
                 }
                 // The ring of scales is as long as its writer can be ahead of its readers: this tile's slot was freed by the MMA
                 // of the tile two before it, and that had waited for the weights of the tile kBuffers before it.
@@ -549,15 +537,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] -= fine;
                     }
-                    if (!careful && (kPolynomialGroups >> (i / 4) & 1) != 0) {
-                        const float2 a = exp2_polynomial(lo), b = exp2_polynomial(hi);
-                        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
-                    } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (careful) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
-                            x[e] = exp2_approx(x[e]);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        if (careful) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
+                        x[e] = exp2_approx(x[e]);
                     }
                     part[0] = __fadd2_rn(part[0], make_float2(x[0], x[1]));
                     part[1] = __fadd2_rn(part[1], make_float2(x[2], x[3]));
@@ -586,7 +569,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 if constexpr (kScaled) {
                     float top = 1e-20f;
 #pragma unroll
-                    for (uint32_t i = 0; i < kTileKeys; i += 32) top = fmaxf(top, value_scales[i + lane]);
+                    for (uint32_t i = 0; i < kTileKeys; i += 32) top = fmaxf(top, fabsf(value_scales[i + lane]));
 #pragma unroll
                     for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
                     value_bits = log2_approx(top);
@@ -613,9 +596,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 const float base = first ? largest * unit : reference;
                 const float over = fmaf(largest, unit, -base) - fine + value_bits - kWeightBits;
                 const bool moves = first || over > kSlackBits;
-                bool special = false;                                    // a NaN among the tile's scores
-                if (__any_sync(0xffffffffu, moves || largest != largest)) {
-                    special = __any_sync(0xffffffffu, largest != largest);
+                if (__any_sync(0xffffffffu, moves)) {
                     float grow = 1.0f;
                     if (moves) {
                         // the last bit of a reference past 2^22 is coarser than the weights' room: what it rounds off is kept too
@@ -650,7 +631,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     }
                     weigh(careful, 0, s0, shift, part);
                 };
-                if (masked || huge || special) take_weights(std::true_type{});
+                if (masked || huge) take_weights(std::true_type{});
                 else take_weights(std::false_type{});
                 sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
             }
@@ -787,7 +768,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
 
 template <int kDim, int kFormat>
 cudaError_t launch_tiles(const TileParams& params, cudaStream_t stream, bool early_launch) {
-    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : 2;
+    constexpr int kLoaderWarps = kFormat == KV_F16 ? 0 : kDim == 64 ? 2 : 3;
     constexpr int kBlocks = static_cast<int>(tile_blocks_per_sm(kDim, static_cast<KvFormat>(kFormat)));
     constexpr size_t bytes = Shape<kDim>::kQueryBytes + kSlots * Shape<kDim>::kTileBytes;
     auto* const kernel = attention_tiles_kernel<kDim, kFormat, kLoaderWarps, kBlocks>;
