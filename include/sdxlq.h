@@ -294,7 +294,8 @@ typedef struct sdxlq_kv_tokens {
  *   FP8   scale = the smallest power of two with a / scale <= the format's largest value, element = FP8_satfinite(x / scale)
  *   FP16  copied
  * Tokens behind counts[r], and those whose place lies outside the slot, are not written; the rest of the cache stays as it
- * was. `tokens->k` and `v` must not overlap the cache. */
+ * was. `tokens->k` and `v` must not overlap the cache. Strides that let what is written (here, by sdxlq_kv_cache_read or as
+ * attention's y) overlap itself are refused. */
 int sdxlq_kv_cache_write(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens);
 
 /* Reads tokens back: half_rn(element * scale), saturating. Tokens that sdxlq_kv_cache_write would not write read as zeros. */

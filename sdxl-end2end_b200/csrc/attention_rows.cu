@@ -1,5 +1,5 @@
 // Attention of few query rows per key head over long keys: tokens of sequences that share a prefix (see attention.cuh for
-// rows, passes and items), and the kernel that joins the shares of the keys.
+// rows, passes and blocks), and the kernel that joins the shares of the keys.
 //
 //   s_j = scale * q . k_j,  y = sum_j 2^(s_j log2 e - m) v_j / sum_j 2^(s_j log2 e - m)
 // in one pass over the keys with a running m. The sums stay as they are when m grows by less than 2^7: weights are kept
@@ -604,7 +604,7 @@ cudaError_t launch_format(const AttentionParams& params, uint32_t row_tile, cuda
     if (params.dim <= 64) {
         return row_tile == 16 ? launch_tile<64, kFormat, 1>(params, stream, early_launch) : launch_tile<64, kFormat, 2>(params, stream, early_launch);
     }
-    return row_tile == 16 ? launch_tile<128, kFormat, 1>(params, stream, early_launch) : launch_tile<128, kFormat, 2>(params, stream, early_launch);
+    return launch_tile<128, kFormat, 1>(params, stream, early_launch);       // two tiles of 128 dimensions are more than the registers hold
 }
 
 }  // namespace

@@ -1,5 +1,5 @@
 // Attention of many query rows per key head (image tokens, long questions): tiles of 128 rows on the tensor memory. See
-// attention.cuh for rows, passes and items, attention_rows.cu for few rows.
+// attention.cuh for rows, passes and blocks, attention_rows.cu for few rows.
 //
 // A CTA takes 128 rows over its share of the keys, in tiles of 64 keys:
 //   MMA warp       S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V as it lies, MN-major);

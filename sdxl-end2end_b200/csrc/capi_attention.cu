@@ -39,6 +39,15 @@ bool strides_ok(uint64_t bytes, uint64_t a, uint64_t b, uint64_t c) {
     return a <= kMaxStride && b <= kMaxStride && c <= kMaxStride && a * bytes % 16 == 0 && b * bytes % 16 == 0 && c * bytes % 16 == 0;
 }
 
+// Whether heads of `dim` elements lie beside one another in some dimension with these strides, so that writing one writes
+// another.
+bool overlapping(uint64_t dim, const uint64_t (&extent)[3], const uint64_t (&stride)[3]) {
+    for (int axis = 0; axis < 3; ++axis) {
+        if (extent[axis] > 1 && stride[axis] < dim) return true;
+    }
+    return false;
+}
+
 bool absent(const sdxlq_kv_cache& c) { return c.slots == 0; }
 
 // The checks that every reader and writer of a cache makes.
@@ -98,6 +107,10 @@ int copy_tokens(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_
     }
     if (!aligned16(t.k) || !aligned16(t.v) || !strides_ok(2, t.row_stride, t.token_stride, t.head_stride)) {
         return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "kv cache: tokens and their strides must be multiples of 16 bytes");
+    }
+    if (write ? overlapping(cache->head_dim, {t.rows, cache->capacity, cache->heads}, {cache->slot_stride, cache->token_stride, cache->head_stride})
+              : overlapping(cache->head_dim, {t.rows, t.tokens, cache->heads}, {t.row_stride, t.token_stride, t.head_stride})) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "kv cache: what is written overlaps in memory");
     }
     KvCopyLaunch launch{};
     launch.cache = view_of(*cache, nullptr);
@@ -163,6 +176,9 @@ int plan_attention(sdxlq_context* ctx, int sm_count, const sdxlq_attention_desc&
     if (!aligned16(d.q) || !aligned16(d.y) || !strides_ok(2, d.q_batch_stride, d.q_token_stride, d.q_head_stride) ||
         !strides_ok(2, d.y_batch_stride, d.y_token_stride, d.y_head_stride)) {
         return fail(ctx, SDXLQ_ERR_UNSUPPORTED_SHAPE, "attention: queries, outputs and their strides must be multiples of 16 bytes");
+    }
+    if (overlapping(d.head_dim, {d.batch, d.q_tokens, d.q_heads}, {d.y_batch_stride, d.y_token_stride, d.y_head_stride})) {
+        return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: the output's rows overlap in memory");
     }
     if (!std::isfinite(d.scale)) return fail(ctx, SDXLQ_ERR_INVALID_ARGUMENT, "attention: the scale must be finite");
     const bool with_prefix = !absent(d.prefix), with_own = !absent(d.own);

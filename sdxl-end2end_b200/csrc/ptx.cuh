@@ -358,14 +358,6 @@ __device__ __forceinline__ void umma_f16_ts_x4(uint32_t tmem_d, uint32_t tmem_a,
         : "memory");
 }
 
-// Asynchronous copy of 16 bytes to shared memory; zeros where `inside` is false (nothing is read then).
-__device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* source, bool inside) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(source), "r"(inside ? 16u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int Pending>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Pending) : "memory"); }
-
 // Makes this thread's writes to shared memory visible to the asynchronous proxy (MMA operands).
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

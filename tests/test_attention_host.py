@@ -77,6 +77,9 @@ int main() {
     copy("head size 20 f16", [](C c, T) { c.dtype = SDXLQ_FP16; c.head_dim = 20; });
     copy("stride", [](C c, T) { c.token_stride = 264; });
     copy("huge stride", [](C c, T) { c.slot_stride = uint64_t(1) << 50; });
+    copy("one place for all slots", [](C c, T t) { c.slot_stride = 0; t.row_stride = 0; });
+    copy("one place for all tokens", [](C c, T t) { c.token_stride = 0; t.token_stride = 32; });
+    copy("one place for all heads", [](C c, T t) { c.head_stride = 48; t.head_stride = 0; });
     copy("alignment", [](C c, T) { c.k = reinterpret_cast<void*>(0x10008); });
     copy("null tokens", [](C, T t) { t.v = nullptr; });
     copy("token stride", [](C, T t) { t.token_stride = 252; });
@@ -106,6 +109,8 @@ int main() {
     attend("wide query", [](D d) { d.head_dim = 136; });
     attend("query alignment", [](D d) { d.q = reinterpret_cast<void*>(0x60002); });
     attend("output stride", [](D d) { d.y_token_stride = 508; });
+    attend("one output for all entries", [](D d) { d.y_batch_stride = 0; });
+    attend("one output for all heads", [](D d) { d.y_head_stride = 0; });
     attend("many rows", [](D d) { d.q_tokens = 1u << 30; });
     attend("scale", [](D d) { d.scale = NAN; });
     attend("no keys", [](D d) { d.prefix.slots = 0; d.own.slots = 0; });
@@ -145,7 +150,9 @@ INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 5
     ("huge stride", UNSUPPORTED, "16 bytes"), ("alignment", UNSUPPORTED, "16 bytes"), ("null tokens", INVALID, "null tokens"),
     ("token stride", UNSUPPORTED, "tokens and their strides"), ("token alignment", UNSUPPORTED, "tokens and their strides"),
     ("rows", INVALID, "more rows than slots"), ("first slot", INVALID, "more rows than slots"), ("start", INVALID, "behind the capacity"),
-    ("huge capacity", UNSUPPORTED, "too large"),
+    ("huge capacity", UNSUPPORTED, "too large"), ("one place for all slots", INVALID, "overlaps"),
+    ("one place for all tokens", INVALID, "overlaps"), ("one place for all heads", INVALID, "overlaps"),
+    ("one output for all entries", INVALID, "overlap"), ("one output for all heads", INVALID, "overlap"),
     ("empty batch", 0, ""), ("no queries", 0, ""), ("null query", INVALID, "null query"), ("null output", INVALID, "null query or output"),
     ("no query heads", INVALID, "no heads"), ("query size", UNSUPPORTED, "multiple of 8"), ("wide query", UNSUPPORTED, "at most 128"),
     ("query alignment", UNSUPPORTED, "16 bytes"), ("output stride", UNSUPPORTED, "16 bytes"), ("many rows", UNSUPPORTED, "too large"),
