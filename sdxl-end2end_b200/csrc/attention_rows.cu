@@ -5,7 +5,9 @@
 // in one pass over the keys with a running m. The sums stay as they are when m grows by less than 2^7: weights are kept
 // as halves, up to 2^6 at m and 2^13 above it, so that the smallest that a half resolves is 2^-31 of the weight at m.
 //
-// What bounds it: the bytes of the cache. Every warp of a block takes every fourth group of 16 (FP16) or 32 (8-bit) keys
+// What bounds it: the bytes of the cache for long keys; for short ones latency, the start of a block and the first round trip to
+// memory (256 keys for each of 64 sequences, 20 heads of 64 in FP16: 84 MB of cache room, of which 36 MB come from memory, in 19 us,
+// caches cold). Every warp of a block takes every fourth group of 16 (FP16) or 32 (8-bit) keys
 // and keeps its own sums, so that no warp waits for another before the end; keys and values go from global memory to the
 // registers of the warp's MMAs, 4 KB (heads of 64) or 8 KB (128) of them in flight per warp, and through no shared
 // memory. That works because the products do not care about the order of what they sum over:
