@@ -313,7 +313,8 @@ int sdxlq_kv_cache_read(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const s
  * The two parts may differ in type. Rows of several entries that share a prefix are multiplied with it together where that
  * reads it fewer times, and long keys are split over the GPU's SMs; both leave shares of the result in `scratch`
  * (sdxlq_shared_prefix_attention_scratch bytes; NULL: the context's workspace, which calls on other streams and captured
- * graphs of the same context share). Results do not depend on the schedule. q, y and their strides are multiples of 16 bytes,
+ * graphs of the same context share). Results do not depend on the schedule. Weights are halves that resolve 2^-31 of the row's
+ * largest weight, in an 8-bit cache of the largest weight times the largest value scale met so far. q, y and their strides are multiples of 16 bytes,
  * as above; y may not overlap the inputs, except that it may be q itself. */
 typedef struct sdxlq_attention_desc {
     const void* q;               /* FP16 [batch, q_tokens, q_heads, head_dim] */
