@@ -191,6 +191,10 @@ __device__ __forceinline__ uint2 widen4(uint32_t bytes) {
     return r;
 }
 
+// The bits of four bytes of a cache that are not all clear where one of them is not zero.
+template <int kFormat>
+__device__ __forceinline__ constexpr uint32_t magnitude_bits() { return kFormat == KV_INT8 ? 0xFFFFFFFFu : 0x7F7F7F7Fu; }
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

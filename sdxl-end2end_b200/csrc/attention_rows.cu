@@ -16,8 +16,8 @@
 //   O = P V: the lane holds for keys 2t, 2t + 1, 2t + 8, 2t + 9 eight consecutive dimensions 8g .. 8g + 7, and MMA j takes
 //   the j-th of them, so its column g is dimension 8g + j.
 // An 8-bit cache enters the MMAs as exact halves without its scales. A key's scale multiplies its column of S; a value's
-// multiplies its weight, relative to the largest value scale so far (else weights of small-scaled values would fall
-// below the halves), which the sums are divided by.
+// multiplies its weight, relative to the largest value scale so far of a vector that is not all zeros (else weights of
+// small-scaled values would fall below the halves), which the sums are divided by.
 
 #include "attention.cuh"
 
@@ -117,6 +117,26 @@ struct ValueBlock {
                 else word8[i][v] = load_vector8(row + d, key < end && d < dim);
             }
             if constexpr (!kHalf) scale[i] = key < end ? __ldg(scales + key) : 0.0f;
+        }
+    }
+
+    // A vector of zeros adds nothing whatever its scale is (1, where the cache was written from zeros), and must not be what the
+    // other weights are placed by: its scale becomes 0. Every eight lanes of a key have a part of it; the groups' 32 keys make
+    // the bits of one word.
+    __device__ __forceinline__ void drop_zero_vectors(uint32_t t) {
+        static_assert(kKeys == 32);
+        uint32_t lives = 0;
+#pragma unroll
+        for (int i = 0; i < kKeys / 4; ++i) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) bits |= word8[i][v].x | word8[i][v].y;
+            if ((bits & magnitude_bits<kFormat>()) != 0) lives |= 1u << i;
+        }
+        lives = __reduce_or_sync(0xffffffffu, lives << (8u * t)) >> (8u * t);
+#pragma unroll
+        for (int i = 0; i < kKeys / 4; ++i) {
+            if ((lives >> i & 1u) == 0) scale[i] = 0.0f;
         }
     }
 
@@ -296,6 +316,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
         const bool masked = first + kKeys > seen_by_all;
         float value_factor = 1.0f;
         if constexpr (kScaled) {
+            values.drop_zero_vectors(t);
             float largest = 0.0f;
 #pragma unroll
             for (int i = 0; i < kKeys / 4; ++i) largest = fmaxf(largest, fabsf(values.scale[i]));

@@ -15,8 +15,8 @@
 //
 // With M the row's running reference, a weight is 2^(s_j log2 e - M); M is the running maximum minus 6, and only moves when a
 // tile's maximum passes it by more than 2^7: then O, in tensor memory, and the sum are multiplied by 2^(M_old - M). Weights
-// of an 8-bit cache are multiplied by their value's scale, and M contains the logarithm of the tile's largest value scale,
-// so that they stay within the halves; O / l is the same for any M.
+// of an 8-bit cache are multiplied by their value's scale, and M contains the logarithm of the tile's largest value scale
+// (of a vector that is not all zeros), so that they stay within the halves; O / l is the same for any M.
 //
 // What bounds it: those round trips; for keys of one or two tiles setting up and storing (5 of 7 us of a CTA's life over 77
 // keys: 80 us for 16 x 4096 queries of 10 heads, 2.1 TB/s); for 8-bit caches and heads of 128 the loaders' conversions.
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
     const AttentionParams& p = params.a;
     extern __shared__ __align__(1024) uint8_t dynamic_smem[];
     __shared__ TileControl control;
-    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][2][kScaled ? kTileKeys : 1];       // key scales * softmax scale, value scales
+    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][2][kScaled ? kTileKeys : 1];       // key scales * softmax scale, value scales (0: a vector of zeros)
     const uint32_t query_base = ptx::smem_u32(dynamic_smem), slots_base = query_base + S::kQueryBytes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     volatile uint32_t* const abort_word = &control.abort;
@@ -253,8 +253,12 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             const bool in_head = chunk * 16u < p.dim;
             // kAhead tiles of K or V are on their way to the registers at a time
             uint4 ahead[kAhead][kRounds];
-            constexpr uint32_t kScales = (kTileKeys + kThreads - 1) / kThreads;      // of a thread
-            float ahead_scale[kAhead / 2][kScales][2] = {};
+            // a lane has the scales of one of the keys that its warp loads in a tile
+            constexpr uint32_t kKeysOfRound = 32 / kChunks;
+            static_assert(kAhead == 2 && kRounds * kKeysOfRound <= 32);
+            const uint32_t scale_round = lane / kKeysOfRound, scale_key = scale_round * kStep + thread / 32u * kKeysOfRound + lane % kKeysOfRound;
+            const bool has_scale = scale_round < kRounds && scale_key < kTileKeys;
+            float ahead_scale[kAhead] = {};
             // where the thread's first 16 bytes of the next tile to fetch are, in K and V, and its scales; tiles come in order
             const uint8_t* from[2] = {};
             const float* scale_from[2] = {};
@@ -289,15 +293,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     const bool inside = in_head && first_key + i * kStep < left;
                     ahead[kBuffer][i] = inside ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0u, 0u, 0u, 0u);
                 }
-                if constexpr (kWhich == 0) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kScales; ++i) {
-                        const uint32_t key = i * kThreads + thread;
-                        const bool inside = key < left;
-                        ahead_scale[kBuffer / 2][i][0] = inside ? __ldg(scale_from[0] + key) * fabsf(p.scale_log2) : 0.0f;
-                        ahead_scale[kBuffer / 2][i][1] = inside ? __ldg(scale_from[1] + key) : 0.0f;
-                    }
-                }
+                const float scale = has_scale && scale_key < left ? __ldg(scale_from[kWhich] + scale_key) : 0.0f;
+                ahead_scale[kWhich] = kWhich == 0 ? scale * fabsf(p.scale_log2) : scale;
             };
             const auto put = [&](uint32_t unit, auto buffer) {
                 constexpr uint32_t kBuffer = decltype(buffer)::value;
@@ -315,17 +312,23 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 // The ring of scales is as long as its writer can be ahead of its readers: this tile's slot was freed by the MMA
                 // of the tile two before it, and that had waited for the weights of the tile kBuffers before it.
                 static_assert(kScaleRing >= kSlots / 2 + kBuffers);
+                float* const ring = scales[unit / 2 % kScaleRing][kBuffer % 2];
                 if constexpr (kBuffer % 2 == 0) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kScales; ++i) {
-                        const uint32_t key = i * kThreads + thread;
-                        if (key < kTileKeys) {
-                            scales[unit / 2 % kScaleRing][0][key] = ahead_scale[kBuffer / 2][i][0];
-                            scales[unit / 2 % kScaleRing][1][key] = ahead_scale[kBuffer / 2][i][1];
-                        }
-                    }
+                    if (has_scale) ring[scale_key] = ahead_scale[0];
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&control.scales_full[unit / 2 % kScaleRing]));
+                } else {
+                    // A vector of zeros adds nothing whatever its scale is (1, where the cache was written from zeros), and must
+                    // not be what the other weights are placed by: its scale becomes 0.
+                    uint32_t lives = 0;
+#pragma unroll
+                    for (uint32_t i = 0; i < kRounds; ++i) {
+                        const uint4 x = ahead[kBuffer][i];
+                        const uint32_t some = __ballot_sync(0xffffffffu, ((x.x | x.y | x.z | x.w) & magnitude_bits<kFormat>()) != 0);
+                        if (scale_round == i) lives = some;
+                    }
+                    lives = lives >> (lane % kKeysOfRound * kChunks) & ((1u << kChunks) - 1u);
+                    if (has_scale) ring[scale_key] = lives != 0 ? ahead_scale[1] : 0.0f;
                 }
                 if (unit + kAhead < 2 * tiles) fetch(unit + kAhead, buffer);
                 announce(unit);
@@ -484,7 +487,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             }
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
-            if (kScaled) ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u);
+            if (kScaled) {                                               // the values' scales come with the values
+                ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u) &&
+                     wait(control.full[(2 * j + 1) % kSlots], ((2 * j + 1) / kSlots) & 1u);
+            }
             ok = ok && wait(control.score_ready[j % kBuffers], (j / kBuffers) & 1u);
             const uint32_t column_s = my_tmem + j % kBuffers * kTileKeys;
             if (!ok) break;
