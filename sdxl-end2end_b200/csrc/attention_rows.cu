@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                     }
                 }
             }
-            float shift[2];
+            // Differences of scores, not sums with the reference, decide and make the weights: they are exact for neighbours of any size.
+            float reference[2];
             float grow[2];
             bool grown = false;
 #pragma unroll
@@ -356,12 +357,13 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
                 grow[half] = 1.0f;
-                if (largest > row_max[rt][half] + kSlackBits) {
-                    grow[half] = exp2_approx(row_max[rt][half] - largest);
+                const float over = largest - row_max[rt][half];          // NaN where neither is there
+                if (over > kSlackBits) {
+                    grow[half] = exp2_approx(-over);
                     row_max[rt][half] = largest;
                     grown = true;
                 }
-                shift[half] = row_max[rt][half] > __int_as_float(0xff800000) ? kWeightBits - row_max[rt][half] : 0.0f;
+                reference[half] = row_max[rt][half] > __int_as_float(0xff800000) ? row_max[rt][half] : 0.0f;
             }
             if (__any_sync(0xffffffffu, grown)) {
                 row_sum[rt][0] *= grow[0];
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 float w[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    w[c] = exp2_approx(s[rt][tile][c] + shift[c >> 1]);
+                    w[c] = exp2_approx((s[rt][tile][c] - reference[c >> 1]) + kWeightBits);
                     row_sum[rt][c >> 1] += w[c];
                     if constexpr (kScaled) {
                         const float factor = values.scale[tile / 2 * 4 + tile % 2 * 2 + (c & 1)] * value_factor;
