@@ -195,6 +195,13 @@ __device__ __forceinline__ uint2 widen4(uint32_t bytes) {
 template <int kFormat>
 __device__ __forceinline__ constexpr uint32_t magnitude_bits() { return kFormat == KV_INT8 ? 0xFFFFFFFFu : 0x7F7F7F7Fu; }
 
+// log2 of a value scale, rounded down, as far as it places weights: from 2^-66 on, which also stands for a vector of zeros (what lies
+// further down is nothing in a half, whatever the element).
+__device__ __forceinline__ float place_bits(float scale) {
+    const int exponent = static_cast<int>(__float_as_uint(scale) >> 23 & 0xFFu) - 127;
+    return static_cast<float>(max(exponent, -66));
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -16,8 +16,8 @@
 //   O = P V: the lane holds for keys 2t, 2t + 1, 2t + 8, 2t + 9 eight consecutive dimensions 8g .. 8g + 7, and MMA j takes
 //   the j-th of them, so its column g is dimension 8g + j.
 // An 8-bit cache enters the MMAs as exact halves without its scales. A key's scale multiplies its column of S; a value's
-// multiplies its weight, relative to the largest value scale so far of a vector that is not all zeros (else weights of
-// small-scaled values would fall below the halves), which the sums are divided by.
+// multiplies its weight, and the halves hold that product relative to the largest so far of the keys that the row sees: O is kept
+// divided by 2^lift, lift the largest of s_j log2 e - m + log2(value scale), which like m moves by more than 2^7 only.
 
 #include "attention.cuh"
 
@@ -28,7 +28,6 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr float kWeightBits = 6.0f;      // a weight at the running maximum is 2^6
 constexpr float kSlackBits = 7.0f;       // the maximum may be passed by this much before the sums are rescaled
-constexpr float kScaleSlack = 4.0f;      // the same for the largest value scale
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -239,7 +238,9 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
         row_max[rt][0] = row_max[rt][1] = __int_as_float(0xff800000);
         row_sum[rt][0] = row_sum[rt][1] = 0.0f;
     }
-    float scale_reference = 0.0f;        // the value scale that the sums are relative to (8-bit caches)
+    float lift[kScaled ? kRowTiles : 1][2];       // 8-bit caches: O is relative to 2^lift; nothing seen yet is far below any
+#pragma unroll
+    for (int rt = 0; rt < (kScaled ? kRowTiles : 1); ++rt) lift[rt][0] = lift[rt][1] = -1000.0f;
 
     const auto rescale = [&](int rt, float factor0, float factor1) {
 #pragma unroll
@@ -314,21 +315,11 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
 
         const uint32_t seen_by_all = in_prefix ? prefix_length : least_limit;
         const bool masked = first + kKeys > seen_by_all;
-        float value_factor = 1.0f;
+        float bits[kScaled ? kKeys / 4 : 1];
         if constexpr (kScaled) {
             values.drop_zero_vectors(t);
-            float largest = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kKeys / 4; ++i) largest = fmaxf(largest, fabsf(values.scale[i]));
-            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-            if (largest > kScaleSlack * scale_reference) {
-                const float factor = scale_reference / largest;
-                scale_reference = largest;
-#pragma unroll
-                for (int rt = 0; rt < kRowTiles; ++rt) rescale(rt, factor, factor);
-            }
-            value_factor = scale_reference > 0.0f ? 1.0f / scale_reference : 0.0f;
+            for (int i = 0; i < kKeys / 4; ++i) bits[i] = place_bits(values.scale[i]);
         }
 
         uint32_t weights[kRowTiles][kTiles / 2][4];
@@ -346,8 +337,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 }
             }
             // Differences of scores, not sums with the reference, decide and make the weights: they are exact for neighbours of any size.
-            float reference[2];
-            float grow[2];
+            float grow[2], lower[2];                                     // of the row's sum, and of O
             bool grown = false;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -356,29 +346,51 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 for (int tile = 0; tile < kTiles; ++tile) largest = fmaxf(largest, fmaxf(s[rt][tile][2 * half], s[rt][tile][2 * half + 1]));
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                grow[half] = 1.0f;
                 const float over = largest - row_max[rt][half];          // NaN where neither is there
-                if (over > kSlackBits) {
-                    grow[half] = exp2_approx(-over);
-                    row_max[rt][half] = largest;
-                    grown = true;
+                const bool moves = over > kSlackBits;
+                if (moves) row_max[rt][half] = largest;
+                grown = grown || moves;
+                grow[half] = lower[half] = moves ? exp2_approx(-over) : 1.0f;
+                const float reference = row_max[rt][half] > __int_as_float(0xff800000) ? row_max[rt][half] : 0.0f;
+                float above = __int_as_float(0xff800000);
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) {
+#pragma unroll
+                    for (int c = 2 * half; c < 2 * half + 2; ++c) {
+                        s[rt][tile][c] -= reference;
+                        if constexpr (kScaled) above = fmaxf(above, s[rt][tile][c] + bits[tile / 2 * 4 + tile % 2 * 2 + (c & 1)]);
+                    }
                 }
-                reference[half] = row_max[rt][half] > __int_as_float(0xff800000) ? row_max[rt][half] : 0.0f;
+                if constexpr (kScaled) {
+                    above = fmaxf(above, __shfl_xor_sync(0xffffffffu, above, 1));
+                    above = fmaxf(above, __shfl_xor_sync(0xffffffffu, above, 2));
+                    const float kept = moves ? lift[rt][half] - over : lift[rt][half];
+                    if (moves || above > kept + kSlackBits) {
+                        lift[rt][half] = fmaxf(kept, above);
+                        lower[half] = exp2_approx(kept - lift[rt][half]);
+                        grown = true;
+                    }
+                }
             }
             if (__any_sync(0xffffffffu, grown)) {
                 row_sum[rt][0] *= grow[0];
                 row_sum[rt][1] *= grow[1];
-                rescale(rt, grow[0], grow[1]);
+                rescale(rt, lower[0], lower[1]);
+            }
+            float unit[2] = {1.0f, 1.0f};
+            if constexpr (kScaled) {
+                unit[0] = exp2_approx(-lift[rt][0]);
+                unit[1] = exp2_approx(-lift[rt][1]);
             }
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
                 float w[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    w[c] = exp2_approx((s[rt][tile][c] - reference[c >> 1]) + kWeightBits);
+                    w[c] = exp2_approx(s[rt][tile][c] + kWeightBits);
                     row_sum[rt][c >> 1] += w[c];
                     if constexpr (kScaled) {
-                        const float factor = values.scale[tile / 2 * 4 + tile % 2 * 2 + (c & 1)] * value_factor;
+                        const float factor = values.scale[tile / 2 * 4 + tile % 2 * 2 + (c & 1)] * unit[c >> 1];
                         w[c] = s[rt][tile][c] == __int_as_float(0xff800000) ? 0.0f : w[c] * factor;
                     }
                 }
@@ -488,11 +500,11 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 shared_l[warp * kTileRows + r] = sum;
             }
             float* const row = shared_o + (warp * kTileRows + r) * kPitch;
+            const float unit = kScaled ? exp2_approx(lift[kScaled ? rt : 0][half]) : 1.0f;
 #pragma unroll
             for (int v = 0; v < kDim / 64; ++v) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float unit = kScaled ? scale_reference : 1.0f;
                     row[v * 64 + 16u * t + j] = o[rt][v * 8 + j][2 * half] * unit;
                     row[v * 64 + 16u * t + 8 + j] = o[rt][v * 8 + j][2 * half + 1] * unit;
                 }

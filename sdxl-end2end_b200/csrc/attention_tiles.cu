@@ -15,8 +15,8 @@
 //
 // With M the row's running reference, a weight is 2^(s_j log2 e - M); M is the running maximum minus 6, and only moves when a
 // tile's maximum passes it by more than 2^7: then O, in tensor memory, and the sum are multiplied by 2^(M_old - M). Weights
-// of an 8-bit cache are multiplied by their value's scale, and M contains the logarithm of the tile's largest value scale
-// (of a vector that is not all zeros), so that they stay within the halves; O / l is the same for any M.
+// of an 8-bit cache are multiplied by their value's scale, and the maximum is that of s_j log2 e + log2(value scale) over the keys
+// that the row sees, so that the products are what the halves resolve; O / l is the same for any M.
 //
 // What bounds it: those round trips; for keys of one or two tiles setting up and storing (5 of 7 us of a CTA's life over 77
 // keys: 80 us for 16 x 4096 queries of 10 heads, 2.1 TB/s); for 8-bit caches and heads of 128 the loaders' conversions.
@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
     const AttentionParams& p = params.a;
     extern __shared__ __align__(1024) uint8_t dynamic_smem[];
     __shared__ TileControl control;
-    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][2][kScaled ? kTileKeys : 1];       // key scales * softmax scale, value scales (0: a vector of zeros)
+    // key scales * softmax scale, value scales (0: a vector of zeros), and log2 of the latter as place_bits has it
+    __shared__ __align__(16) float scales[kScaled ? kScaleRing : 1][3][kScaled ? kTileKeys : 1];
     const uint32_t query_base = ptx::smem_u32(dynamic_smem), slots_base = query_base + S::kQueryBytes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     volatile uint32_t* const abort_word = &control.abort;
@@ -312,9 +313,9 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 // The ring of scales is as long as its writer can be ahead of its readers: this tile's slot was freed by the MMA
                 // of the tile two before it, and that had waited for the weights of the tile kBuffers before it.
                 static_assert(kScaleRing >= kSlots / 2 + kBuffers);
-                float* const ring = scales[unit / 2 % kScaleRing][kBuffer % 2];
+                auto& ring = scales[unit / 2 % kScaleRing];
                 if constexpr (kBuffer % 2 == 0) {
-                    if (has_scale) ring[scale_key] = ahead_scale[0];
+                    if (has_scale) ring[0][scale_key] = ahead_scale[0];
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&control.scales_full[unit / 2 % kScaleRing]));
                 } else {
@@ -328,7 +329,11 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                         if (scale_round == i) lives = some;
                     }
                     lives = lives >> (lane % kKeysOfRound * kChunks) & ((1u << kChunks) - 1u);
-                    if (has_scale) ring[scale_key] = lives != 0 ? ahead_scale[1] : 0.0f;
+                    if (has_scale) {
+                        const float scale = lives != 0 ? ahead_scale[1] : 0.0f;
+                        ring[1][scale_key] = scale;
+                        ring[2][scale_key] = place_bits(scale);
+                    }
                 }
                 if (unit + kAhead < 2 * tiles) fetch(unit + kAhead, buffer);
                 announce(unit);
@@ -487,6 +492,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             }
             const float* const key_scales = scales[j % kScaleRing][0];
             const float* const value_scales = scales[j % kScaleRing][kScaled ? 1 : 0];
+            const float* const value_bits = scales[j % kScaleRing][kScaled ? 2 : 0];
             if (kScaled) {                                               // the values' scales come with the values
                 ok = wait(control.scales_full[j % kScaleRing], (j / kScaleRing) & 1u) &&
                      wait(control.full[(2 * j + 1) % kSlots], ((2 * j + 1) / kSlots) & 1u);
@@ -496,27 +502,25 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
             if (!ok) break;
             ptx::tc_fence_after();
 
-            // 32 columns of S; those of an 8-bit cache times their key's scale
+            // 32 columns of S; an 8-bit cache's without their key's scale, which the fused multiply-adds below bring in
             const auto load = [&](uint32_t c, uint32_t (&s)[32]) {
                 ptx::tmem_ld_32x32b_x32(column_s + c * 32u, s);
                 ptx::tmem_ld_wait(s);
-                if constexpr (kScaled) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
-                        const float2 lo = __fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y));
-                        const float2 hi = __fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w));
-                        s[i] = __float_as_uint(lo.x); s[i + 1] = __float_as_uint(lo.y); s[i + 2] = __float_as_uint(hi.x); s[i + 3] = __float_as_uint(hi.y);
-                    }
-                }
             };
-            // the largest of 32 columns: of the scores in FP16 without their scale, which is the same for all
+            // the largest of 32 columns: of the scores in FP16 without their scale, which is the same for all; of an 8-bit cache's
+            // scores plus the logarithm of their value's scale
             const auto largest_of = [&](auto careful_case, uint32_t c, const uint32_t (&s)[32], float largest) {
                 constexpr bool careful = decltype(careful_case)::value;
                 float other = largest;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                     float x[4] = {__uint_as_float(s[i]), __uint_as_float(s[i + 1]), __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])};
+                    if constexpr (kScaled) {
+                        const float4 k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i), bits = *reinterpret_cast<const float4*>(value_bits + c * 32u + i);
+                        const float2 lo = __ffma2_rn(make_float2(x[0], x[1]), make_float2(k.x, k.y), make_float2(bits.x, bits.y));
+                        const float2 hi = __ffma2_rn(make_float2(x[2], x[3]), make_float2(k.z, k.w), make_float2(bits.z, bits.w));
+                        x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
+                    }
                     if (careful) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : kNone;
@@ -536,8 +540,10 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     // it is as exact for large scores as for small ones.
                     float2 lo = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), hi = make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
                     const float2 back = make_float2(-shift, -shift);
-                    lo = kScaled ? __fadd2_rn(lo, back) : __ffma2_rn(lo, make_float2(scale, scale), back);
-                    hi = kScaled ? __fadd2_rn(hi, back) : __ffma2_rn(hi, make_float2(scale, scale), back);
+                    float4 k = make_float4(scale, scale, scale, scale);
+                    if constexpr (kScaled) k = *reinterpret_cast<const float4*>(key_scales + c * 32u + i);
+                    lo = __ffma2_rn(lo, make_float2(k.x, k.y), back);
+                    hi = __ffma2_rn(hi, make_float2(k.z, k.w), back);
                     float x[4] = {lo.x, lo.y, hi.x, hi.y};
                     if (careful) {
 #pragma unroll
@@ -552,7 +558,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                     part[1] = __fadd2_rn(part[1], make_float2(x[2], x[3]));
                     if constexpr (kScaled) {
                         const float4 v = *reinterpret_cast<const float4*>(value_scales + c * 32u + i);
-                        x[0] *= v.x; x[1] *= v.y; x[2] *= v.z; x[3] *= v.w;
+                        const float2 a = __fmul2_rn(make_float2(x[0], x[1]), make_float2(v.x, v.y)), b = __fmul2_rn(make_float2(x[2], x[3]), make_float2(v.z, v.w));
+                        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
                         if (careful) {                                   // a hidden key's scale may be anything
 #pragma unroll
                             for (int e = 0; e < 4; ++e) x[e] = c * 32u + i + e < visible ? x[e] : 0.0f;
@@ -571,15 +578,6 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 return done;
             };
             if (warp_active) {
-                float value_bits = 0.0f;                                 // log2 of the tile's largest value scale
-                if constexpr (kScaled) {
-                    float top = 1e-20f;
-#pragma unroll
-                    for (uint32_t i = 0; i < kTileKeys; i += 32) top = fmaxf(top, fabsf(value_scales[i + lane]));
-#pragma unroll
-                    for (int offset = 16; offset != 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-                    value_bits = log2_approx(top);
-                }
                 const bool both = columns > 32u;
                 // Columns 32 to 63 stay in registers until they are weighed; the first 32 too, where there is room for them.
                 constexpr bool kHold = kDim > 64;
@@ -599,8 +597,32 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 // the reference moves where the tile's largest weight would be 2^7 past its place, and in the row's first tile
                 const float unit = kScaled ? 1.0f : scale;
                 const bool first = reference == kNone && largest > kNone;
-                const float base = first ? largest * unit : reference;
-                const float over = fmaf(largest, unit, -base) - fine + value_bits - kWeightBits;
+                float base = first ? largest * unit : reference;
+                float over = fmaf(largest, unit, -base);
+                if constexpr (kScaled) {
+                    // The sum of such a score and a logarithm is rounded too coarsely to place a weight by. Differences of scores
+                    // are exact: again, with the largest score for the reference of a first tile.
+                    if (__any_sync(0xffffffffu, largest > kNone && fabsf(largest) > 1048576.0f)) {
+                        float top = kNone;
+                        over = kNone;
+                        for (uint32_t pass = 0; pass < 2; ++pass) {
+                            for (uint32_t c = 0; c < (both ? 2u : 1u); ++c) {
+                                load(c, s0);
+#pragma unroll
+                                for (uint32_t i = 0; i < 32; ++i) {
+                                    const float x = fmaf(__uint_as_float(s0[i]), key_scales[c * 32u + i], pass == 0 ? 0.0f : -base);
+                                    if (c * 32u + i >= visible) continue;
+                                    if (pass == 0) top = fmaxf(top, x);
+                                    else over = fmaxf(over, x + value_bits[c * 32u + i]);
+                                }
+                            }
+                            base = first ? top : reference;
+                        }
+                        if (largest == kNone) over = kNone;
+                        if (kHold) load(0, s0);                          // s1 is as it was; one buffer has its last columns again
+                    }
+                }
+                over -= fine + kWeightBits;
                 const bool moves = first || over > kSlackBits;
                 if (__any_sync(0xffffffffu, moves)) {
                     float grow = 1.0f;
