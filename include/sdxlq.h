@@ -315,7 +315,8 @@ int sdxlq_kv_cache_read(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const s
  * (sdxlq_shared_prefix_attention_scratch bytes; NULL: the context's workspace, which calls on other streams and captured
  * graphs of the same context share). Results do not depend on the schedule. Weights are halves that resolve 2^-31 of the row's
  * largest weight, in an 8-bit cache (where they are multiplied by their value's scale first, 0 for a vector of zeros) of the largest
- * such product among the keys that the row sees. q, y and their strides are multiples of 16 bytes, as above; y may not overlap the inputs, except that it may be q itself. */
+ * such product among the keys that the row sees. q, y and their strides are multiples of 16 bytes, as above; y may not overlap the
+ * inputs, except that it may be q itself. */
 typedef struct sdxlq_attention_desc {
     const void* q;               /* FP16 [batch, q_tokens, q_heads, head_dim] */
     void* y;                     /* FP16 [batch, q_tokens, q_heads, head_dim] */

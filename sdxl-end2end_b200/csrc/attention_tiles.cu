@@ -686,7 +686,8 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                 ok = values_done() && wait(control.full[unit % kSlots], (unit / kSlots) & 1u);
                 if (!ok) break;
                 bool found = false;
-                for (uint32_t i = threadIdx.x; i < columns * (kDim / 8); i += 32 * kSoftmaxWarps) {
+                // the keys that exist: other warps may still be putting the zeros behind them
+                for (uint32_t i = threadIdx.x; i < values * (kDim / 8); i += 32 * kSoftmaxWarps) {
                     const uint4 x = ptx::ld_shared16(base + swizzled(i / (kDim / 8), i % (kDim / 8), kTileKeys));
                     found = found || half_not_finite(x.x) || half_not_finite(x.y) || half_not_finite(x.z) || half_not_finite(x.w);
                 }
@@ -703,7 +704,7 @@ __global__ void __launch_bounds__(32 * (kSoftmaxWarps + 1 + kLoaderWarps), kBloc
                         float total[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) total[i] = j == 0 ? 0.0f : __uint_as_float(o[i]);
-                        for (uint32_t key = 0; key < columns; ++key) {
+                        for (uint32_t key = 0; key < values; ++key) {
                             uint32_t pair;
                             ptx::tmem_ld_32x32b_x1(column_s + key / 32 * 32 + key % 32 / 2, pair);
                             ptx::tmem_ld_wait(pair);
