@@ -295,7 +295,7 @@ typedef struct sdxlq_kv_tokens {
  *   FP16  copied
  * Tokens behind counts[r], and those whose place lies outside the slot, are not written; the rest of the cache stays as it
  * was. `tokens->k` and `v` must not overlap the cache. Strides that let what is written (here, by sdxlq_kv_cache_read or as
- * attention's y) overlap itself are refused. */
+ * attention's y) overlap itself are refused: in rising order, each has to be at least what head_dim and the smaller ones reach. */
 int sdxlq_kv_cache_write(sdxlq_context* ctx, const sdxlq_kv_cache* cache, const sdxlq_kv_tokens* tokens);
 
 /* Reads tokens back: half_rn(element * scale), saturating. Tokens that sdxlq_kv_cache_write would not write read as zeros. */

@@ -4,6 +4,7 @@
 #include "context.cuh"
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <string>
 
@@ -39,11 +40,18 @@ bool strides_ok(uint64_t bytes, uint64_t a, uint64_t b, uint64_t c) {
     return a <= kMaxStride && b <= kMaxStride && c <= kMaxStride && a * bytes % 16 == 0 && b * bytes % 16 == 0 && c * bytes % 16 == 0;
 }
 
-// Whether heads of `dim` elements lie beside one another in some dimension with these strides, so that writing one writes
-// another.
-bool overlapping(uint64_t dim, const uint64_t (&extent)[3], const uint64_t (&stride)[3]) {
-    for (int axis = 0; axis < 3; ++axis) {
-        if (extent[axis] > 1 && stride[axis] < dim) return true;
+// Whether writing one head of `dim` elements may write another: each stride, in rising order, has to pass over all that the
+// smaller ones reach. (Layouts whose axes interleave without meeting are refused with the others.)
+bool overlapping(uint64_t dim, std::array<uint64_t, 3> extent, std::array<uint64_t, 3> stride) {
+    std::array<int, 3> axis{0, 1, 2};
+    std::sort(axis.begin(), axis.end(), [&](int a, int b) { return stride[a] < stride[b]; });
+    uint64_t reach = dim;
+    for (int i : axis) {
+        if (extent[i] <= 1) continue;
+        if (stride[i] < reach) return true;
+        // strides are at most 2^40 and extents below 2^31: past this, no other stride is large enough
+        if (stride[i] > (uint64_t(1) << 62) / extent[i]) reach = ~uint64_t(0);
+        else reach += stride[i] * (extent[i] - 1);
     }
     return false;
 }
