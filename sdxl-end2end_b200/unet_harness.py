@@ -296,6 +296,8 @@ class UNetHarness:
         self._kv_plan = None
         self._kv_source: Optional[torch.Tensor] = None
         self._temb_plan = None
+        self.generation = 0                # counts the times that memory which forward() reads or writes was replaced:
+                                           # a graph that was captured before is of the memory before
 
     # -- weights ----------------------------------------------------------------------------------
     def _pack(self, values: torch.Tensor) -> Weight:
@@ -422,6 +424,7 @@ class UNetHarness:
         names = [name for name in self.projections if name.endswith(".attn2.to_k") or name.endswith(".attn2.to_v")]
         calls = [LinearCall(self._kv_source, self.projections[name]) for name in names]
         self._kv_plan = self.ops.plan(calls)
+        self.generation += 1
         self._kv = dict(zip(names, self._kv_plan.run()))
         self._kv_caches = {}
         self._fill_kv_caches()
@@ -445,6 +448,7 @@ class UNetHarness:
             self._temb_input = activated.clone()
             calls = [LinearCall(self._temb_input, self.projections[name], self._temb_bias[name]) for name in names]
             self._temb_plan = self.ops.plan(calls)
+            self.generation += 1
             self._temb_outputs = dict(zip(names, [call.y for call in self._temb_plan.calls]))
         self._temb_input.copy_(activated)
         self._temb_plan.run()
@@ -591,8 +595,9 @@ class EulerDenoiser:
     x + ((x - (x - sigma * eps)) / sigma) * (sigma_next - sigma) on FP32 latents
     (euler_step_f16_f32_kernel, :1031-1050, epsilon prediction).
 
-    One step is optionally captured once as a CUDA graph and replayed (the reference captures its
-    denoise loop the same way, src/cuda/denoise_graph.cpp); sigma, the next sigma and the timestep are
+    One step is optionally captured as a CUDA graph and replayed, and captured again where the UNet has replaced memory that it
+    reads (a text context of another shape; the reference captures its denoise loop the same way,
+    src/cuda/denoise_graph.cpp); sigma, the next sigma and the timestep are
     read from a small device tensor that is refreshed before each replay."""
 
     def __init__(self, unet: UNetHarness, images: int, height: int = 1024, width: int = 1024, steps: int = 20,
@@ -614,6 +619,7 @@ class EulerDenoiser:
         if device.type == "cuda":
             self._scalar_table = self._scalar_table.pin_memory()
         self._graph = None
+        self._captured_generation = -1     # of the UNet's memory that the graph is of
         self.step_index = 0
 
     def set_conditioning(self, prompt_embeds: torch.Tensor, pooled: torch.Tensor, time_ids: torch.Tensor) -> None:
@@ -649,8 +655,9 @@ class EulerDenoiser:
         if not self.use_graph:
             self._step_body()
         else:
-            if self._graph is None:
+            if self._graph is None or self._captured_generation != self.unet.generation:
                 self._capture()
+                self._captured_generation = self.unet.generation
             self._graph.replay()
         self.step_index += 1
 
@@ -666,6 +673,7 @@ class EulerDenoiser:
         torch.cuda.current_stream(self.unet.device).wait_stream(side)
         torch.cuda.synchronize(self.unet.device)
         self.latents.copy_(saved)
+        self._graph = None                 # what it held is of no use any more
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._step_body()
