@@ -625,6 +625,9 @@ class EulerDenoiser:
     def set_conditioning(self, prompt_embeds: torch.Tensor, pooled: torch.Tensor, time_ids: torch.Tensor) -> None:
         """prompt_embeds FP16 [2 * images, 77, cross_dim] laid out [uncond x images | cond x images]; with shared-prefix
         attention also [2 * prompts, ..]: each row serves images / prompts consecutive images."""
+        rows = prompt_embeds.shape[0]
+        if rows % 2 != 0 or not self.unet._conditions(rows, 2 * self.images):        # no row serves both halves
+            raise CudaError("CUDA UNet conditioning batch mismatch")
         self.unet._follow_current_stream()
         self.unet.prepare_conditioning(prompt_embeds)
         self.pooled.copy_(pooled)

@@ -74,6 +74,21 @@ def test_a_loop_of_another_batch_on_the_same_unet():
     assert len(captures) == 2
 
 
+@pytest.mark.parametrize("images,shared,rows", [(4, True, 1), (3, True, 3), (4, True, 6), (6, True, 8), (6, True, 3), (4, True, 0), (4, True, 16),
+                                                (4, False, 4), (4, False, 2), (4, False, 9)])
+def test_rows_that_serve_no_prompt_pair(images, shared, rows):
+    """An odd number of rows has one for both the unconditional and the conditional half; others do not divide the batch. What was
+    set before stays."""
+    unet, loop, captures = recording_loop(FakeAttention(), images, **({"attention": "shared_prefix"} if shared else {}))
+    _, _, pooled, time_ids = inputs(2 * images, 1)
+    loop.set_conditioning(context_of(2 * images, 77, 1), pooled, time_ids)
+    source, kept = unet._kv_source, unet._kv_source.clone()
+    with pytest.raises(pkg.CudaError, match="batch mismatch"):
+        loop.set_conditioning(context_of(rows, 77, 2), pooled, time_ids)
+    assert unet._kv_source is source and torch.equal(source, kept)
+    assert unet.generation == 1
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("options", [{}, {"attention": "shared_prefix"}, {"attention": "shared_prefix", "kv_cache": "int8"}])
 def test_captured_loop_follows_the_context(gpu, options):
