@@ -388,6 +388,13 @@ class UNetHarness:
             return self._attention(query, self._kv[f"{block}.attn2.to_k"], self._kv[f"{block}.attn2.to_v"], heads)
         return self.ops.shared_prefix_attention(query.unflatten(2, (heads, -1)), None, self._kv_caches[block]).flatten(2)
 
+    def _heads_of(self, block: str) -> int:
+        """Attention heads of a transformer block, by the level in its name (levels may be of equal width)."""
+        part, level = block.split(".")[:2]
+        if part == "mid_block":
+            return self.config.heads[-1]
+        return self.config.heads[int(level) if part == "down_blocks" else len(self.config.heads) - 1 - int(level)]
+
     def _fill_kv_caches(self) -> None:
         """The context's keys and values as attention reads them: where they were projected (FP16), or quantised."""
         for name, key in self._kv.items():
@@ -395,7 +402,7 @@ class UNetHarness:
                 continue
             block = name[: -len(".attn2.to_k")]
             value = self._kv[f"{block}.attn2.to_v"]
-            heads = self.config.heads[self.config.channels.index(key.shape[2])]
+            heads = self._heads_of(block)
             projected = KVCache.of(key, value, heads)
             if self.kv_type == ScalarType.Float16:
                 self._kv_caches[block] = projected
