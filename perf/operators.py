@@ -159,13 +159,21 @@ def _inputs(case, seed):
     return state
 
 
+def _operators(pkg, made=[]):
+    """The operators on the current stream. A program has one context for all its calls."""
+    if not made:
+        made.append(pkg.Ops(pkg.Context(0, workspace_bytes=1 << 20)))
+    made[0].ctx.set_stream(torch.cuda.current_stream(0))
+    return made[0]
+
+
 def prepare(case, seed):
     state = _inputs(case, seed)
     if own:
         pkg = importlib.import_module("sdxl-end2end_b200")
         types = {"int8": pkg.ScalarType.Int8, "e4m3": pkg.ScalarType.Float8E4M3, "e5m2": pkg.ScalarType.Float8E5M2,
                  "f16": pkg.ScalarType.Float16}
-        state["ops"] = ops = pkg.Ops(pkg.Context(0, workspace_bytes=1 << 20))
+        state["ops"] = ops = _operators(pkg)
         if case["kind"] == "store":
             state["cache"] = ops.kv_cache(case["slots"], case["capacity"], case["heads"], case["dim"], types[case["dtype"]])
         else:
