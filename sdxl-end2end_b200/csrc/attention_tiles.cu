@@ -9,9 +9,9 @@
 // Everything that one tile needs of the one before it is a round trip between the warps (softmax, product, scores: 2.2
 // thousand clocks, of which the SM's exponentials take 512), so what counts is how many tiles an SM has in flight. Heads of
 // 64 take 128 columns of tensor memory and 48 KB, so four CTAs share an SM; heads of up to 128 take 256 columns, two CTAs,
-// each with the scores of two tiles. Measured on the self-attention of 2 x 4096 tokens, 10 heads of 64: tiles of 128
-// keys with two CTAs per SM 226 us, these 139 us (620 TFLOP/s). Taking every fourth exponential as a polynomial on the FMA
-// pipe gave nothing (141 us): the pipe of the exponentials is busy 60 % of the time.
+// each with the scores of two tiles. The self-attention of 2 x 4096 tokens, 10 heads of 64,
+// takes 145 us (593 TFLOP/s); tiles of 128 keys with two CTAs per SM took 1.6 times as long. Taking every fourth exponential as a
+// polynomial on the FMA pipe gave nothing: the pipe of the exponentials is busy half of the time.
 //
 // With M the row's running reference, a weight is 2^(s_j log2 e - M); M is the running maximum minus 6, and only moves when a
 // tile's maximum passes it by more than 2^7: then O, in tensor memory, and the sum are multiplied by 2^(M_old - M). Weights
@@ -19,7 +19,9 @@
 // that the row sees, so that the products are what the halves resolve; O / l is the same for any M.
 //
 // What bounds it: those round trips; for keys of one or two tiles setting up and storing (5 of 7 us of a CTA's life over 77
-// keys: 80 us for 16 x 4096 queries of 10 heads, 2.1 TB/s); for 8-bit caches and heads of 128 the loaders' conversions.
+// keys: 80 us for 16 x 4096 queries of 10 heads, 2.1 TB/s); for 8-bit caches and heads of 128 the loaders' conversions
+// (4 x 333 causal queries over 2333 keys, 16 heads of 80 on 8 in INT8: 86 us). Of these 86 us the search for vectors of zeros takes 4, the
+// maximum over score and value scale 2; taken as one product with the key's scale and one sum each it took 10.
 
 #include "attention.cuh"
 #include "internal.cuh"

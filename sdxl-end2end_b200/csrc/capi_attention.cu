@@ -31,7 +31,7 @@ private:
 };
 
 constexpr uint64_t kMaxExtent = 0x7FFFFFFFull;
-constexpr uint64_t kMaxStride = uint64_t(1) << 40;       // elements: offsets stay within 63 bits for any extents below
+constexpr uint64_t kMaxStride = uint64_t(1) << 40;       // elements: products with the extents of memory that exists stay within 63 bits
 
 bool is_kv_type(int32_t dtype) { return is_fp8(dtype) || dtype == SDXLQ_INT8 || dtype == SDXLQ_FP16; }
 uint64_t element_bytes(int32_t dtype) { return dtype == SDXLQ_FP16 ? 2 : 1; }

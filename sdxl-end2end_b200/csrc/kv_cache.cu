@@ -9,7 +9,7 @@
 // INT8 is that of the exact quotient: r = rne(x * (1 / s)) is at most one off, and the remainder x - r s, exact in
 // one fused multiply-add (r s and x are multiples of units that keep it within 24 bits), says to which side.
 //
-// What bounds it: memory for large copies (16 x 4096 tokens of 10 heads of 64 into INT8 and back: 103 us, 5.0 TB/s), latency for
+// What bounds it: memory for large copies (16 x 4096 tokens of 10 heads of 64 into INT8 and back: 106 us, 4.8 TB/s), latency for
 // small ones (2 x 77 tokens: 4 us a launch). A lane takes 16 bytes of K and of V of one vector, D / 8
 // lanes share a vector's maximum by shuffles. The block's vectors run over tokens first: the FP16 side is then read in
 // whole 128-byte lines and the cache, whose tokens of one head lie behind one another, is written in runs.
