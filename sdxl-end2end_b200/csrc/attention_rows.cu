@@ -377,10 +377,10 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 row_sum[rt][1] *= grow[1];
                 rescale(rt, lower[0], lower[1]);
             }
-            float unit[2] = {1.0f, 1.0f};
+            float unit[2] = {1.0f, 1.0f};                                // 2^(-lift / 2): a lift may be as large as the largest scale's
             if constexpr (kScaled) {
-                unit[0] = exp2_approx(-lift[rt][0]);
-                unit[1] = exp2_approx(-lift[rt][1]);
+                unit[0] = exp2_approx(-0.5f * lift[rt][0]);
+                unit[1] = exp2_approx(-0.5f * lift[rt][1]);
             }
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                     w[c] = exp2_approx(s[rt][tile][c] + kWeightBits);
                     row_sum[rt][c >> 1] += w[c];
                     if constexpr (kScaled) {
-                        const float factor = values.scale[tile / 2 * 4 + tile % 2 * 2 + (c & 1)] * unit[c >> 1];
+                        const float factor = values.scale[tile / 2 * 4 + tile % 2 * 2 + (c & 1)] * unit[c >> 1] * unit[c >> 1];
                         w[c] = s[rt][tile][c] == __int_as_float(0xff800000) ? 0.0f : w[c] * factor;
                     }
                 }
@@ -500,13 +500,13 @@ __global__ void __launch_bounds__(32 * kWarps) attention_rows_kernel(const __gri
                 shared_l[warp * kTileRows + r] = sum;
             }
             float* const row = shared_o + (warp * kTileRows + r) * kPitch;
-            const float unit = kScaled ? exp2_approx(lift[kScaled ? rt : 0][half]) : 1.0f;
+            const float unit = kScaled ? exp2_approx(0.5f * lift[kScaled ? rt : 0][half]) : 1.0f;
 #pragma unroll
             for (int v = 0; v < kDim / 64; ++v) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    row[v * 64 + 16u * t + j] = o[rt][v * 8 + j][2 * half] * unit;
-                    row[v * 64 + 16u * t + 8 + j] = o[rt][v * 8 + j][2 * half + 1] * unit;
+                    row[v * 64 + 16u * t + j] = o[rt][v * 8 + j][2 * half] * unit * unit;
+                    row[v * 64 + 16u * t + 8 + j] = o[rt][v * 8 + j][2 * half + 1] * unit * unit;
                 }
             }
         }

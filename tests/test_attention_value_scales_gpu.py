@@ -157,3 +157,23 @@ def test_huge_scores_and_small_values(gpu, dtype, queries, keys):
             context.check()
             want = exact[1][:, at:at + 1].expand(1, queries, 1, dim)
             assert ((y.double() - want).abs() <= (2 ** -10 + 2 ** -20) * want.abs() + 2 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", EIGHT_BIT)
+@pytest.mark.parametrize("queries", [1, 20, 150])
+@pytest.mark.parametrize("scale", [2.0 ** 90, 2.0 ** 110, 2.0 ** 127])
+def test_the_largest_scales(gpu, dtype, queries, scale):
+    """A value scale near the top of 32 bits on a key that has weight: its values of 1 and more are infinite in FP16, its zeros are not there."""
+    pkg, context, ops = gpu
+    q, k = leaning(queries, 200, 64, at=3)
+    v = normal(128, 1, 200, 2, 64)
+    v[:, 3, :, :32] = 2.0
+    v[:, 3, :, 32:] = 0.0
+    cache, exact = cache_of(pkg, k, v, dtype)
+    scales = cache.v_scales.clone()
+    scales[:, :, 3] = scale
+    odd = pkg.KVCache(cache.k, cache.v, cache.type, cache.k_scales, scales)
+    y = ops.shared_prefix_attention(q, odd)
+    context.check()
+    assert torch.isinf(y[..., :32]).all() and (y[..., :32] > 0).all()
+    assert torch.isfinite(y[..., 32:]).all()
